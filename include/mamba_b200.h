@@ -335,6 +335,151 @@ int mm_linear_fwd(const MMLinearArgs* args, void* workspace, size_t workspace_by
 /* Synchronises `stream`; MM_ERR_TIMEOUT if a pipeline wait of a call on `workspace` ran out. */
 int mm_linear_status(const void* workspace, mm_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Training operators. No counterpart in the reference, which has no backward pass.
+ *
+ * 8-bit activation checkpoints. Every row of `length` values is cut into blocks of
+ * MM_CHECKPOINT8_BLOCK; a block keeps one exponent byte and one signed byte per value:
+ *   e    = the least integer >= -126 with 127 * 2^e >= max |x| over the block (-126 for a block of zeros)
+ *   code = x * 2^-e rounded to the nearest integer, ties to even (|code| <= 127);  exponent byte = e + 127
+ * so a value is off by at most 2^(e-1), and code * 2^e is exact in every element type (where it passes
+ * the type's largest finite value, that value is restored). A block that holds an infinity or a NaN gets
+ * the exponent byte 255 and is restored as NaN.
+ * x: (batch, dim, length) of `dtype`, codes alike in int8, exponents (batch, dim, ceil(length / 32)) in
+ * uint8, any element strides. Vectorised paths: every tensor contiguous along time, rows of x 16-byte and
+ * rows of codes 8-byte aligned; or every tensor contiguous along channels. Pack reads x and writes the
+ * rest, unpack the other way round.
+ * ------------------------------------------------------------------------------------------- */
+#define MM_CHECKPOINT8_BLOCK 32
+typedef struct MMCheckpoint8Args {
+  void* x;
+  int8_t* codes;
+  uint8_t* exponents;
+  int64_t dtype;
+  int64_t batch, dim, length;
+  int64_t x_stride[3];
+  int64_t codes_stride[3];
+  int64_t exponents_stride[3];
+} MMCheckpoint8Args;
+
+int mm_checkpoint8_pack(const MMCheckpoint8Args* args, mm_stream_t stream);
+int mm_checkpoint8_unpack(const MMCheckpoint8Args* args, mm_stream_t stream);
+
+/* mm_causal_conv1d_fwd (out from the given x) and mm_checkpoint8_pack of x in one pass over x. width must
+ * be 4. `codes` and `exponents` as above. */
+typedef struct MMConvCheckpointArgs {
+  const void* x;
+  const float* weight; /* (dim, 4) contiguous */
+  const float* bias;   /* may be NULL */
+  void* out;
+  int8_t* codes;
+  uint8_t* exponents;
+  int64_t dtype;
+  int64_t batch, dim, seqlen, width;
+  int64_t x_stride[3];
+  int64_t out_stride[3];
+  int64_t codes_stride[3];
+  int64_t exponents_stride[3];
+  int64_t silu;
+} MMConvCheckpointArgs;
+
+int mm_causal_conv1d_fwd_checkpoint8(const MMConvCheckpointArgs* args, mm_stream_t stream);
+
+/* Gradient of mm_causal_conv1d_fwd, at the input x or (x == NULL) at the values its checkpoint stands for:
+ *   pre[t] = bias + sum_k weight[k] x[t-3+k];  dpre = dout * silu'(pre)  (dout without silu)
+ *   dx[t] = sum_k weight[k] dpre[t+3-k];  dweight[k] = sum_{b,t} dpre[t] x[t-3+k];  dbias = sum_{b,t} dpre[t]
+ * dout, dx: (batch, dim, seqlen) of `dtype`, any strides; dweight (dim, 4), dbias (dim,) fp32 contiguous,
+ * dbias may be NULL. Sums over (b, t) are taken in a fixed order: equal calls give equal bits. */
+typedef struct MMConvBwdArgs {
+  const void* x; /* NULL: codes / exponents are read instead */
+  const int8_t* codes;
+  const uint8_t* exponents;
+  const float* weight;
+  const float* bias; /* may be NULL */
+  const void* dout;
+  void* dx;
+  float* dweight;
+  float* dbias; /* may be NULL */
+  int64_t dtype;
+  int64_t batch, dim, seqlen, width;
+  int64_t x_stride[3];
+  int64_t codes_stride[3];
+  int64_t exponents_stride[3];
+  int64_t dout_stride[3];
+  int64_t dx_stride[3];
+  int64_t silu;
+} MMConvBwdArgs;
+
+int mm_causal_conv1d_bwd_workspace_size(const MMConvBwdArgs* args, size_t* bytes);
+int mm_causal_conv1d_bwd(const MMConvBwdArgs* args, void* workspace, size_t workspace_bytes, mm_stream_t stream);
+
+/* Preference loss over pairs of answers, from logits. Rows 0 .. pairs-1 are the chosen answers, rows
+ * pairs .. 2*pairs-1 the rejected ones of the same pairs; a token whose label is `ignore_index` is no part
+ * of its answer (an answer may have no token left: its log-probability is 0).
+ *   logp[r] = sum over the row's answer tokens of logits[r,t,label] - logsumexp_v logits[r,t,v]
+ *   chosen[i] = beta (logp[i] - ref[i]);  rejected[i] = beta (logp[pairs+i] - ref[pairs+i]);  m = chosen - rejected
+ *   loss = mean_i of -(1 - smoothing) log sigmoid(m[i]) - smoothing log sigmoid(-m[i])
+ * logits: (2*pairs, length, vocab) of `dtype`, strides of rows and tokens free, vocab contiguous; labels
+ * (2*pairs, length) int64, contiguous; ref (2*pairs,) fp32. A label that is neither ignore_index nor in
+ * [0, vocab) makes its row's log-probability NaN. stats: fp32 (2*pairs, length, 2), the largest logit of each
+ * token and the sum of exp(logit - largest), written by the forward call and read by the backward one (ignored
+ * tokens' are neither); slope: fp32 (2*pairs,), d loss / d logp[r], likewise.
+ * The backward call writes dlogits (contiguous rows of vocab, strides free; zeros for ignored tokens):
+ *   dlogits[r,t,v] = grad_loss * slope[r] * ((v == label) - softmax(logits[r,t,:])[v])
+ * grad_loss: one fp32 value on the device. */
+typedef struct MMPreferenceArgs {
+  const void* logits;
+  const int64_t* labels;
+  const float* ref;
+  float* loss;     /* 1 */
+  float* chosen;   /* pairs */
+  float* rejected; /* pairs */
+  float* stats;
+  float* slope;
+  const float* grad_loss; /* backward only */
+  void* dlogits;          /* backward only */
+  int64_t dtype;
+  int64_t pairs, length, vocab;
+  int64_t logits_stride[2];
+  int64_t dlogits_stride[2];
+  int64_t ignore_index;
+  double beta, smoothing;
+} MMPreferenceArgs;
+
+int mm_preference_loss_workspace_size(const MMPreferenceArgs* args, size_t* bytes);
+int mm_preference_loss_fwd(const MMPreferenceArgs* args, void* workspace, size_t workspace_bytes,
+                           mm_stream_t stream);
+int mm_preference_loss_bwd(const MMPreferenceArgs* args, mm_stream_t stream);
+
+/* Gradient of mm_selective_scan_fwd. `fwd` holds the forward call's inputs (its y, state_out, piece_tiles and
+ * options are not read); nothing else is kept from the forward pass.
+ *   dy: (batch, dim, seqlen) of the forward's dtype; dstate: gradient of the last state, fp32 (batch, dim, dstate)
+ *   contiguous, or NULL; du, ddelta, dz alike (dz when z is given); dB, dC: (batch, dstate, seqlen) of the dtype;
+ *   dA (dim, dstate), dD (dim,), ddelta_bias (dim,): fp32 contiguous; dD / ddelta_bias may be NULL.
+ * All strides free. Sums are taken in a fixed order: equal calls give equal bits. */
+typedef struct MMScanBwdArgs {
+  MMScanArgs fwd;
+  const void* dy;
+  const float* dstate; /* may be NULL */
+  void* du;
+  void* ddelta;
+  float* dA;
+  void* dB;
+  void* dC;
+  float* dD; /* may be NULL */
+  void* dz;  /* NULL without z */
+  float* ddelta_bias; /* may be NULL */
+  int64_t dy_stride[3];
+  int64_t du_stride[3];
+  int64_t ddelta_stride[3];
+  int64_t dz_stride[3];
+  int64_t dB_stride[3];
+  int64_t dC_stride[3];
+} MMScanBwdArgs;
+
+int mm_selective_scan_bwd_workspace_size(const MMScanBwdArgs* args, size_t* bytes);
+int mm_selective_scan_bwd(const MMScanBwdArgs* args, void* workspace, size_t workspace_bytes, mm_stream_t stream);
+
 const char* mm_version(void);
 
 #ifdef __cplusplus

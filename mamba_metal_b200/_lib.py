@@ -101,6 +101,47 @@ class MMLinearArgs(ctypes.Structure):
     ]
 
 
+class MMCheckpoint8Args(ctypes.Structure):
+    _fields_ = [
+        ("x", _p), ("codes", _p), ("exponents", _p), ("dtype", _i64), ("batch", _i64), ("dim", _i64),
+        ("length", _i64), ("x_stride", _i64 * 3), ("codes_stride", _i64 * 3), ("exponents_stride", _i64 * 3),
+    ]
+
+
+class MMConvCheckpointArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _p), ("weight", _p), ("bias", _p), ("out", _p), ("codes", _p), ("exponents", _p), ("dtype", _i64),
+        ("batch", _i64), ("dim", _i64), ("seqlen", _i64), ("width", _i64), ("x_stride", _i64 * 3),
+        ("out_stride", _i64 * 3), ("codes_stride", _i64 * 3), ("exponents_stride", _i64 * 3), ("silu", _i64),
+    ]
+
+
+class MMConvBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _p), ("codes", _p), ("exponents", _p), ("weight", _p), ("bias", _p), ("dout", _p), ("dx", _p),
+        ("dweight", _p), ("dbias", _p), ("dtype", _i64), ("batch", _i64), ("dim", _i64), ("seqlen", _i64),
+        ("width", _i64), ("x_stride", _i64 * 3), ("codes_stride", _i64 * 3), ("exponents_stride", _i64 * 3),
+        ("dout_stride", _i64 * 3), ("dx_stride", _i64 * 3), ("silu", _i64),
+    ]
+
+
+class MMPreferenceArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", _p), ("labels", _p), ("ref", _p), ("loss", _p), ("chosen", _p), ("rejected", _p), ("stats", _p),
+        ("slope", _p), ("grad_loss", _p), ("dlogits", _p), ("dtype", _i64), ("pairs", _i64), ("length", _i64),
+        ("vocab", _i64), ("logits_stride", _i64 * 2), ("dlogits_stride", _i64 * 2), ("ignore_index", _i64),
+        ("beta", ctypes.c_double), ("smoothing", ctypes.c_double),
+    ]
+
+
+class MMScanBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", MMScanArgs), ("dy", _p), ("dstate", _p), ("du", _p), ("ddelta", _p), ("dA", _p), ("dB", _p),
+        ("dC", _p), ("dD", _p), ("dz", _p), ("ddelta_bias", _p), ("dy_stride", _i64 * 3), ("du_stride", _i64 * 3),
+        ("ddelta_stride", _i64 * 3), ("dz_stride", _i64 * 3), ("dB_stride", _i64 * 3), ("dC_stride", _i64 * 3),
+    ]
+
+
 _SIGNATURES = {
     "mm_selective_scan_workspace_size": ([ctypes.POINTER(MMScanArgs), ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "mm_selective_scan_fwd": ([ctypes.POINTER(MMScanArgs), _p, ctypes.c_size_t, _p], ctypes.c_int),
@@ -117,6 +158,19 @@ _SIGNATURES = {
     "mm_linear_workspace_size": ([ctypes.POINTER(MMLinearArgs), ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "mm_linear_fwd": ([ctypes.POINTER(MMLinearArgs), _p, ctypes.c_size_t, _p], ctypes.c_int),
     "mm_linear_status": ([_p, _p], ctypes.c_int),
+    "mm_checkpoint8_pack": ([ctypes.POINTER(MMCheckpoint8Args), _p], ctypes.c_int),
+    "mm_checkpoint8_unpack": ([ctypes.POINTER(MMCheckpoint8Args), _p], ctypes.c_int),
+    "mm_causal_conv1d_fwd_checkpoint8": ([ctypes.POINTER(MMConvCheckpointArgs), _p], ctypes.c_int),
+    "mm_causal_conv1d_bwd_workspace_size": ([ctypes.POINTER(MMConvBwdArgs), ctypes.POINTER(ctypes.c_size_t)],
+                                            ctypes.c_int),
+    "mm_causal_conv1d_bwd": ([ctypes.POINTER(MMConvBwdArgs), _p, ctypes.c_size_t, _p], ctypes.c_int),
+    "mm_preference_loss_workspace_size": ([ctypes.POINTER(MMPreferenceArgs), ctypes.POINTER(ctypes.c_size_t)],
+                                          ctypes.c_int),
+    "mm_preference_loss_fwd": ([ctypes.POINTER(MMPreferenceArgs), _p, ctypes.c_size_t, _p], ctypes.c_int),
+    "mm_preference_loss_bwd": ([ctypes.POINTER(MMPreferenceArgs), _p], ctypes.c_int),
+    "mm_selective_scan_bwd_workspace_size": ([ctypes.POINTER(MMScanBwdArgs), ctypes.POINTER(ctypes.c_size_t)],
+                                             ctypes.c_int),
+    "mm_selective_scan_bwd": ([ctypes.POINTER(MMScanBwdArgs), _p, ctypes.c_size_t, _p], ctypes.c_int),
     "mm_version": ([], ctypes.c_char_p),
 }
 

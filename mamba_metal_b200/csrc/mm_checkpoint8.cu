@@ -1,0 +1,166 @@
+// Packing and unpacking of 8-bit activation checkpoints. Memory-bound: a packed value moves its own bytes
+// once, one byte of code and 1/32 byte of exponent.
+#include "mm_checkpoint8.cuh"
+
+namespace mm {
+namespace ck {
+
+struct Params {
+  void* x;
+  int8_t* codes;
+  uint8_t* exps;
+  long long xs[3], cs[3], es[3];
+  long long rows;
+  int dim, length;
+};
+
+// Time contiguous: a lane takes 8 consecutive values, so four lanes share a block and agree on its maximum by
+// two shuffles. VEC: 16-byte loads of x and 8-byte stores of codes. A warp covers 256 values of one row.
+template <typename T, bool PACK, bool VEC>
+__global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per_row) {
+  const int lane = threadIdx.x & 31;
+  const long long gw = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (gw >= p.rows * warps_per_row) return;
+  const long long row = gw / warps_per_row;
+  const int t0 = ((int)(gw % warps_per_row) * 32 + lane) * 8;
+  const long long b = row / p.dim, d = row % p.dim;
+  T* x = static_cast<T*>(p.x) + b * p.xs[0] + d * p.xs[1] + (long long)t0 * p.xs[2];
+  int8_t* codes = p.codes + b * p.cs[0] + d * p.cs[1] + (long long)t0 * p.cs[2];
+  uint8_t* exps = p.exps + b * p.es[0] + d * p.es[1] + (long long)(t0 / kCkBlock) * p.es[2];
+  const int n = min(8, p.length - t0);  // values of this lane; none or fewer than none past the row's end
+  float v[8];
+  if (PACK) {
+    if (VEC && n == 8) {
+      ck_load8<T>(x, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = k < n ? ld_f32(x + k * p.xs[2]) : 0.f;
+    }
+    unsigned m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = max(m, ck_abs_bits(v[k]));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    if (n <= 0) return;
+    const unsigned byte = ck_exponent(m);
+    const float inv = ck_inverse_scale(byte);
+    if ((lane & 3) == 0) *exps = (uint8_t)byte;
+    if (VEC && n == 8) {
+      uint2 w;
+      w.x = ck_pack4(ck_code(v[0], inv), ck_code(v[1], inv), ck_code(v[2], inv), ck_code(v[3], inv));
+      w.y = ck_pack4(ck_code(v[4], inv), ck_code(v[5], inv), ck_code(v[6], inv), ck_code(v[7], inv));
+      __stcs(reinterpret_cast<uint2*>(codes), w);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < n) codes[k * p.cs[2]] = (int8_t)ck_code(v[k], inv);
+    }
+  } else {
+    if (n <= 0) return;
+    const float scale = ck_scale(*exps);
+    if (VEC && n == 8) {
+      const uint2 w = __ldcs(reinterpret_cast<const uint2*>(codes));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] = ck_restore<T>(ck_byte(w.x, k), scale);
+        v[k + 4] = ck_restore<T>(ck_byte(w.y, k), scale);
+      }
+      ck_store8<T>(x, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < n) st_f32(x + k * p.xs[2], ck_restore<T>(codes[k * p.cs[2]], scale));
+    }
+  }
+}
+
+// Channels contiguous: a thread takes one block of one channel, so a warp's accesses run along channels.
+template <typename T, bool PACK>
+__global__ void __launch_bounds__(256) columns_kernel(const Params p, int blocks) {
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long long batch = p.rows / p.dim;
+  if (i >= batch * blocks * p.dim) return;
+  const long long d = i % p.dim, k = i / p.dim % blocks, b = i / p.dim / blocks;
+  const int t0 = (int)k * kCkBlock, n = min(kCkBlock, p.length - t0);
+  T* x = static_cast<T*>(p.x) + b * p.xs[0] + d * p.xs[1] + (long long)t0 * p.xs[2];
+  int8_t* codes = p.codes + b * p.cs[0] + d * p.cs[1] + (long long)t0 * p.cs[2];
+  uint8_t* exps = p.exps + b * p.es[0] + d * p.es[1] + k * p.es[2];
+  if (PACK) {
+    T v[kCkBlock];
+    unsigned m = 0;
+#pragma unroll
+    for (int t = 0; t < kCkBlock; ++t) {
+      v[t] = t < n ? x[t * p.xs[2]] : ElemTraits<T>::from_f32(0.f);
+      m = max(m, ck_abs_bits(ElemTraits<T>::to_f32(v[t])));
+    }
+    const unsigned byte = ck_exponent(m);
+    const float inv = ck_inverse_scale(byte);
+    *exps = (uint8_t)byte;
+#pragma unroll
+    for (int t = 0; t < kCkBlock; ++t)
+      if (t < n) codes[t * p.cs[2]] = (int8_t)ck_code(ElemTraits<T>::to_f32(v[t]), inv);
+  } else {
+    const float scale = ck_scale(*exps);
+#pragma unroll 8
+    for (int t = 0; t < n; ++t) st_f32(x + t * p.xs[2], ck_restore<T>(codes[t * p.cs[2]], scale));
+  }
+}
+
+template <typename T, bool PACK> int launch(const MMCheckpoint8Args* a, cudaStream_t s) {
+  Params p;
+  p.x = a->x;
+  p.codes = a->codes;
+  p.exps = a->exponents;
+  for (int i = 0; i < 3; ++i) {
+    p.xs[i] = a->x_stride[i];
+    p.cs[i] = a->codes_stride[i];
+    p.es[i] = a->exponents_stride[i];
+  }
+  p.rows = a->batch * a->dim;
+  p.dim = (int)a->dim;
+  p.length = (int)a->length;
+  const bool columns = a->dim > 1 && a->length > 1 && p.xs[1] == 1 && p.cs[1] == 1 && p.xs[2] != 1;
+  if (columns) {
+    const int blocks = (int)((a->length + kCkBlock - 1) / kCkBlock);
+    const long long grid = (p.rows * blocks + 255) / 256;
+    if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
+    columns_kernel<T, PACK><<<(unsigned)grid, 256, 0, s>>>(p, blocks);
+  } else {
+    const int wpr = (int)((a->length + 255) / 256);
+    const long long grid = (p.rows * wpr + 7) / 8;
+    if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
+    const bool vec = (p.xs[2] == 1 && p.cs[2] == 1) &&
+                     ck_rows_aligned(a->x, a->x_stride, a->batch, a->dim, (int)sizeof(T), 16) &&
+                     ck_rows_aligned(a->codes, a->codes_stride, a->batch, a->dim, 1, 8);
+    if (vec)
+      rows_kernel<T, PACK, true><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
+    else
+      rows_kernel<T, PACK, false><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
+  }
+  return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
+}
+
+template <bool PACK> int dispatch(const MMCheckpoint8Args* a, mm_stream_t stream) {
+  if (!a) return MM_ERR_ARG;
+  if (!dtype_size(a->dtype)) return MM_ERR_DTYPE;
+  if (a->batch < 0 || a->dim < 0 || a->length < 0 || a->dim > 0x7fffffffLL || a->length > 0x7fffffffLL - 512)
+    return MM_ERR_SHAPE;
+  if (a->batch == 0 || a->dim == 0 || a->length == 0) return MM_OK;
+  if (!a->x || !a->codes || !a->exponents) return MM_ERR_ARG;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (a->dtype) {
+    case MM_F32: return launch<float, PACK>(a, s);
+    case MM_F16: return launch<__half, PACK>(a, s);
+    default: return launch<__nv_bfloat16, PACK>(a, s);
+  }
+}
+
+}  // namespace ck
+}  // namespace mm
+
+extern "C" int mm_checkpoint8_pack(const MMCheckpoint8Args* a, mm_stream_t stream) {
+  return mm::ck::dispatch<true>(a, stream);
+}
+extern "C" int mm_checkpoint8_unpack(const MMCheckpoint8Args* a, mm_stream_t stream) {
+  return mm::ck::dispatch<false>(a, stream);
+}

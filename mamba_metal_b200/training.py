@@ -1,0 +1,417 @@
+"""Differentiable counterparts of the package's operators, and what a training step needs beside them: 8-bit
+activation checkpoints and the preference loss. No counterpart in the reference, which has no backward pass.
+
+``selective_scan`` and ``causal_conv1d`` take the arguments of the functions of the same name in the package and
+compute the same values; gradients flow to every floating-point input that asks for them. They are functions of
+their own so that the package's inference functions keep returning tensors without a graph. Everything runs in
+libmamba_b200.so on the current stream of the tensors' device; there is no CPU path. The backward passes can
+be differentiated once, and equal calls give equal bits.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from mamba_metal_b200 import _lib, ops
+from mamba_metal_b200.selective_scan import MAX_DSTATE, _scan_dtype, selective_scan_into
+
+CHECKPOINT8_BLOCK = 32  # values of a row that share an exponent (MM_CHECKPOINT8_BLOCK)
+
+
+def _by_channel(t: torch.Tensor) -> bool:
+    """Whether a (..., channels, time) view is laid out with the channels contiguous."""
+    return t.shape[-2] > 1 and t.shape[-1] > 1 and t.stride(-2) == 1 and t.stride(-1) != 1
+
+
+def _empty(shape, dtype, device, by_channel: bool) -> torch.Tensor:
+    b, d, n = shape
+    if by_channel:
+        return torch.empty((b, n, d), dtype=dtype, device=device).transpose(1, 2)
+    return torch.empty((b, d, n), dtype=dtype, device=device)
+
+
+def _laid_out(t: torch.Tensor, by_channel: bool) -> torch.Tensor:
+    """``t`` (batch, channels, time) with the wanted axis contiguous; a gradient can arrive in any layout (of a sum,
+    for instance, with stride 0)."""
+    if by_channel:
+        return t if t.stride(1) == 1 else t.transpose(1, 2).contiguous().transpose(1, 2)
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def _f32(t: torch.Tensor | None) -> torch.Tensor | None:
+    return None if t is None else t.detach().float().contiguous()
+
+
+def _like(grad: torch.Tensor | None, t: torch.Tensor | None) -> torch.Tensor | None:
+    return None if t is None else grad.reshape(t.shape).to(t.dtype)
+
+
+# ---- 8-bit activation checkpoints --------------------------------------------------------------------------
+
+
+def _checkpoint_args(x, codes, exponents):
+    a = _lib.MMCheckpoint8Args()
+    a.x, a.codes, a.exponents = x.data_ptr(), codes.data_ptr(), exponents.data_ptr()
+    a.dtype = _lib.DTYPE_CODE[x.dtype]
+    a.batch, a.dim, a.length = x.shape
+    a.x_stride, a.codes_stride, a.exponents_stride = (_lib.strides3(t) for t in (x, codes, exponents))
+    return a
+
+
+def _checkpoint_buffers(shape, device, by_channel: bool):
+    """Codes and exponents for a (batch, channels, time) tensor, laid out like it. Rows of codes start on multiples
+    of the block, so that they can be written and read in vectors whatever the length."""
+    b, d, n = shape
+    blocks = -(-n // CHECKPOINT8_BLOCK)
+    exponents = _empty((b, d, blocks), torch.uint8, device, by_channel)
+    if by_channel:
+        return _empty(shape, torch.int8, device, True), exponents
+    return torch.empty((b, d, blocks * CHECKPOINT8_BLOCK), dtype=torch.int8, device=device)[..., :n], exponents
+
+
+@dataclass(frozen=True)
+class Checkpoint8:
+    """A tensor held in 8 bits: ``codes`` (int8, the tensor's shape) and ``exponents`` (uint8, one per 32 values of the
+    last axis). A value stands for ``code * 2 ** (exponent - 127)``; exponent 255 marks a block that held an infinity
+    or a NaN, and stands for NaN. ``dtype`` is the type of the tensor that was packed."""
+
+    codes: torch.Tensor
+    exponents: torch.Tensor
+    dtype: torch.dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.exponents.numel()
+
+    def restore(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The values, in ``dtype`` (default: the packed tensor's), laid out like the packed tensor. Exact, but for
+        values past the type's largest finite one, which is returned instead."""
+        dtype = dtype or self.dtype
+        if dtype not in _lib.DTYPE_CODE:
+            raise TypeError(f"unsupported dtype {dtype}")
+        codes, exponents = _rows3(self.codes), _rows3(self.exponents)
+        dev = _lib.require_cuda(codes, exponents)
+        out = _empty(codes.shape, dtype, dev, _by_channel(codes))
+        with torch.cuda.device(dev):
+            rc = _lib.lib().mm_checkpoint8_unpack(ctypes.byref(_checkpoint_args(out, codes, exponents)),
+                                                  _lib.stream_handle(dev))
+        _lib.check(rc, "mm_checkpoint8_unpack")
+        return out.view(self.shape) if self.codes.dim() != 3 else out
+
+
+def _rows3(t: torch.Tensor) -> torch.Tensor:
+    """(..., length) as (batch, rows, length), a view for up to three axes."""
+    if t.dim() > 3:
+        return t.flatten(0, -3)
+    return t.reshape((1,) * (3 - t.dim()) + tuple(t.shape)) if t.dim() < 3 else t
+
+
+def checkpoint8(x: torch.Tensor) -> Checkpoint8:
+    """Packs ``x`` (float32, float16 or bfloat16, one axis or more) into 8 bits a value: blocks of 32 values of the last
+    axis share the smallest power of two of which 127 reach their largest magnitude, and every value becomes a whole
+    multiple of it, ties to even. No value moves by more than half that power of two, 1/128 of the block's
+    largest magnitude at most."""
+    assert x.dim() >= 1, "a checkpoint holds a tensor of one axis or more"
+    if x.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    dev = _lib.require_cuda(x)
+    rows = _rows3(x.detach())
+    codes, exponents = _checkpoint_buffers(rows.shape, dev, _by_channel(rows))
+    with torch.cuda.device(dev):
+        rc = _lib.lib().mm_checkpoint8_pack(ctypes.byref(_checkpoint_args(rows, codes, exponents)),
+                                            _lib.stream_handle(dev))
+    _lib.check(rc, "mm_checkpoint8_pack")
+    if x.dim() < 3:
+        codes, exponents = codes[(0,) * (3 - x.dim())], exponents[(0,) * (3 - x.dim())]
+    elif x.dim() > 3:
+        codes, exponents = codes.unflatten(0, x.shape[:-2]), exponents.unflatten(0, x.shape[:-2])
+    return Checkpoint8(codes, exponents, x.dtype)
+
+
+# ---- causal conv1d -----------------------------------------------------------------------------------------
+
+
+def conv1d_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, *, silu: bool = True):
+    """``causal_conv1d`` and ``checkpoint8`` of its input in one pass over ``x`` (batch, dim, seqlen). Returns
+    (out, checkpoint); no graph."""
+    dim = x.shape[1]
+    assert x.dim() == 3 and weight.numel() == dim * ops.D_CONV and weight.shape[0] == dim, "only d_conv == 4 is implemented"
+    assert bias is None or tuple(bias.shape) == (dim,)
+    if x.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    dev = _lib.require_cuda(x, weight, bias)
+    w, b = _f32(weight), _f32(bias)
+    by_channel = _by_channel(x)
+    out = _empty(x.shape, x.dtype, dev, by_channel)
+    codes, exponents = _checkpoint_buffers(x.shape, dev, by_channel)
+    a = _lib.MMConvCheckpointArgs()
+    a.x, a.weight, a.bias, a.out = x.data_ptr(), w.data_ptr(), _lib.ptr(b), out.data_ptr()
+    a.codes, a.exponents = codes.data_ptr(), exponents.data_ptr()
+    a.dtype = _lib.DTYPE_CODE[x.dtype]
+    a.batch, a.dim, a.seqlen, a.width = *x.shape, ops.D_CONV
+    a.x_stride, a.out_stride, a.codes_stride, a.exponents_stride = (_lib.strides3(t) for t in (x, out, codes, exponents))
+    a.silu = int(bool(silu))
+    with torch.cuda.device(dev):
+        rc = _lib.lib().mm_causal_conv1d_fwd_checkpoint8(ctypes.byref(a), _lib.stream_handle(dev))
+    _lib.check(rc, "mm_causal_conv1d_fwd_checkpoint8")
+    return out, Checkpoint8(codes, exponents, x.dtype)
+
+
+def causal_conv1d_backward(dout: torch.Tensor, x: torch.Tensor | Checkpoint8, weight: torch.Tensor,
+                           bias: torch.Tensor | None, *, silu: bool = True):
+    """Gradient of ``causal_conv1d`` at ``x``, or at the values that a checkpoint of it stands for: (dx of dout's
+    dtype, dweight (dim, 4) float32, dbias (dim,) float32)."""
+    held = isinstance(x, Checkpoint8)
+    src = x.codes if held else x
+    batch, dim, seqlen = src.shape
+    assert dout.shape == src.shape and dout.dtype == x.dtype
+    assert weight.numel() == dim * ops.D_CONV and (bias is None or tuple(bias.shape) == (dim,))
+    if dout.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {dout.dtype}")
+    dev = _lib.require_cuda(dout, src, weight, bias)
+    w, b = _f32(weight), _f32(bias)
+    by_channel = _by_channel(src)
+    dout = _laid_out(dout, by_channel)
+    dx = _empty(src.shape, dout.dtype, dev, by_channel)
+    dw = torch.empty((dim, ops.D_CONV), dtype=torch.float32, device=dev)
+    db = torch.empty((dim,), dtype=torch.float32, device=dev)
+    a = _lib.MMConvBwdArgs()
+    if held:
+        a.codes, a.exponents = src.data_ptr(), x.exponents.data_ptr()
+        a.codes_stride, a.exponents_stride = _lib.strides3(src), _lib.strides3(x.exponents)
+    else:
+        a.x, a.x_stride = src.data_ptr(), _lib.strides3(src)
+    a.weight, a.bias, a.dout, a.dx = w.data_ptr(), _lib.ptr(b), dout.data_ptr(), dx.data_ptr()
+    a.dweight, a.dbias = dw.data_ptr(), db.data_ptr()
+    a.dtype = _lib.DTYPE_CODE[dout.dtype]
+    a.batch, a.dim, a.seqlen, a.width = batch, dim, seqlen, ops.D_CONV
+    a.dout_stride, a.dx_stride = _lib.strides3(dout), _lib.strides3(dx)
+    a.silu = int(bool(silu))
+    lib = _lib.lib()
+    nbytes = ctypes.c_size_t(0)
+    _lib.check(lib.mm_causal_conv1d_bwd_workspace_size(ctypes.byref(a), ctypes.byref(nbytes)),
+               "mm_causal_conv1d_bwd_workspace_size")
+    ws = torch.empty(int(nbytes.value), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        rc = lib.mm_causal_conv1d_bwd(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
+    _lib.check(rc, "mm_causal_conv1d_bwd")
+    return dx, dw, db
+
+
+class _CausalConv1d(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, silu, held):
+        ctx.silu, ctx.held = silu, held
+        if held:
+            out, c = conv1d_checkpoint8(x, weight, bias, silu=silu)
+            ctx.save_for_backward(c.codes, c.exponents, weight, bias)
+        else:
+            out = _empty(x.shape, x.dtype, x.device, _by_channel(x))
+            ops.causal_conv1d(x, weight, bias, silu=silu, out=out)
+            ctx.save_for_backward(x, None, weight, bias)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        src, exponents, weight, bias = ctx.saved_tensors
+        if ctx.held:
+            src = Checkpoint8(src, exponents, dout.dtype)
+        dx, dw, db = causal_conv1d_backward(dout, src, weight, bias, silu=ctx.silu)
+        return dx, _like(dw, weight), _like(db, bias), None, None
+
+
+def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, silu: bool = True,
+                  checkpoint8: bool = False) -> torch.Tensor:
+    """Differentiable ``mamba_metal_b200.causal_conv1d``: x (batch, dim, seqlen), weight (dim, 1, 4) or (dim, 4), bias
+    (dim,) or None. The output and dx are laid out like ``x``. With ``checkpoint8`` the backward pass is given
+    ``x`` in 8 bits (made in the forward pass, see :func:`checkpoint8`) in place of ``x`` itself: the output is
+    the same, the gradients are those at the values that the checkpoint stands for."""
+    _lib.require_cuda(x, weight, bias)
+    assert x.dim() == 3 and weight.shape[0] == x.shape[1] and weight.numel() == x.shape[1] * ops.D_CONV, \
+        "only d_conv == 4 is implemented"
+    assert bias is None or tuple(bias.shape) == (x.shape[1],)
+    return _CausalConv1d.apply(x, weight, bias, bool(silu), bool(checkpoint8))
+
+
+# ---- selective scan ----------------------------------------------------------------------------------------
+
+
+def selective_scan_backward(dy: torch.Tensor, u, delta, A, B, C, *, D=None, z=None, delta_bias=None,
+                            delta_softplus: bool = False, dstate: torch.Tensor | None = None) -> dict:
+    """Gradient of ``selective_scan`` for given dy (batch, dim, seqlen) and, optionally, dstate (batch, dim, dstate) of
+    the last state. All activations share one dtype; A, D and delta_bias are float32. Returns a dict of "u", "delta",
+    "B", "C", "z" (that dtype; "z" None without z) and "A", "D", "delta_bias" (float32; None where not given)."""
+    dev = _lib.require_cuda(dy, u, delta, A, B, C, D, z, delta_bias, dstate)
+    batch, dim, seqlen = u.shape
+    n = A.shape[1]
+    assert dy.shape == u.shape == delta.shape and tuple(B.shape) == (batch, n, seqlen) == tuple(C.shape)
+    assert (z is None or z.shape == u.shape) and tuple(A.shape) == (dim, n) and n <= MAX_DSTATE
+    for t in (delta, B, C, z, dy):
+        assert t is None or t.dtype == u.dtype
+    for t, shape in ((D, (dim,)), (delta_bias, (dim,)), (dstate, (batch, dim, n))):
+        assert t is None or (t.dtype == torch.float32 and tuple(t.shape) == shape and t.is_contiguous())
+    assert A.dtype == torch.float32
+    if u.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {u.dtype}")
+    by_channel = _by_channel(u)
+    dy = _laid_out(dy, by_channel)
+    act = lambda: _empty(u.shape, u.dtype, dev, by_channel)
+    f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)
+    g = {"u": act(), "delta": act(), "z": None if z is None else act(), "A": f32(dim, n),
+         "B": _empty(B.shape, u.dtype, dev, _by_channel(B)), "C": _empty(C.shape, u.dtype, dev, _by_channel(C)),
+         "D": None if D is None else f32(dim), "delta_bias": None if delta_bias is None else f32(dim)}
+    a = _lib.MMScanBwdArgs()
+    f = a.fwd
+    f.u, f.delta, f.A, f.B, f.C, f.D, f.z, f.delta_bias = (_lib.ptr(t) for t in (u, delta, A, B, C, D, z, delta_bias))
+    f.dtype = _lib.DTYPE_CODE[u.dtype]
+    f.batch, f.dim, f.dstate, f.seqlen = batch, dim, n, seqlen
+    f.u_stride, f.delta_stride, f.z_stride, f.B_stride, f.C_stride = (_lib.strides3(t) for t in (u, delta, z, B, C))
+    f.A_stride = (ctypes.c_int64 * 2)(*A.stride())
+    f.delta_softplus = int(bool(delta_softplus))
+    a.dy, a.dstate = dy.data_ptr(), _lib.ptr(dstate)
+    a.du, a.ddelta, a.dA, a.dB, a.dC = (g[k].data_ptr() for k in ("u", "delta", "A", "B", "C"))
+    a.dD, a.dz, a.ddelta_bias = (_lib.ptr(g[k]) for k in ("D", "z", "delta_bias"))
+    a.dy_stride, a.du_stride, a.ddelta_stride, a.dz_stride, a.dB_stride, a.dC_stride = \
+        (_lib.strides3(t) for t in (dy, g["u"], g["delta"], g["z"], g["B"], g["C"]))
+    lib = _lib.lib()
+    nbytes = ctypes.c_size_t(0)
+    _lib.check(lib.mm_selective_scan_bwd_workspace_size(ctypes.byref(a), ctypes.byref(nbytes)),
+               "mm_selective_scan_bwd_workspace_size")
+    ws = torch.empty(int(nbytes.value), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        rc = lib.mm_selective_scan_bwd(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
+    _lib.check(rc, "mm_selective_scan_bwd")
+    return g
+
+
+class _SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, delta, A, B, C, D, z, delta_bias, softplus):
+        ctx.set_materialize_grads(False)
+        dtype = _scan_dtype(u, delta, B, C, z)
+        cast = lambda t: None if t is None else t.detach().to(dtype)
+        uc, dc, Bc, Cc, zc = map(cast, (u, delta, B, C, z))
+        Af, Df, bf = A.detach().float(), _f32(D), _f32(delta_bias)
+        batch, dim, seqlen = u.shape
+        y = _empty(u.shape, dtype, u.device, _by_channel(u))
+        state = torch.zeros if u.numel() == 0 else torch.empty  # a scan over nothing leaves the state at zero
+        state = state((batch, dim, A.shape[1]), dtype=torch.float32, device=u.device)
+        if u.numel():
+            selective_scan_into(uc, dc, Af, Bc, Cc, Df, zc, y, state, softplus, delta_bias=bf)
+        ctx.softplus = softplus
+        ctx.dtypes = tuple(None if t is None else t.dtype for t in (u, delta, A, B, C, D, z, delta_bias))
+        ctx.save_for_backward(uc, dc, Af, Bc, Cc, Df, zc, bf)
+        return y.to(u.dtype), state
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dstate):
+        u, delta, A, B, C, D, z, bias = ctx.saved_tensors
+        if dy is None and dstate is None:
+            return (None,) * 9
+        dy = torch.zeros_like(u) if dy is None else dy.to(u.dtype)
+        g = selective_scan_backward(dy, u, delta, A, B, C, D=D, z=z, delta_bias=bias, delta_softplus=ctx.softplus,
+                                    dstate=_f32(dstate))
+        names = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")
+        return (*(None if t is None else g[k].to(t) for k, t in zip(names, ctx.dtypes)), None)
+
+
+def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
+                   D: torch.Tensor | None = None, z: torch.Tensor | None = None,
+                   delta_bias: torch.Tensor | None = None, delta_softplus: bool = False, return_state: bool = False):
+    """Differentiable ``mamba_metal_b200.selective_scan``: shapes, dtypes and results as there, and ``delta_bias``
+    (dim,), added to delta before softplus. The last state is differentiable too. y and the gradients of u, delta
+    and z are laid out like u. The backward pass keeps the inputs and nothing else: it recomputes the states."""
+    batch, dim, seqlen = u.shape
+    _, dstate = A.shape
+    assert delta.shape == u.shape
+    assert tuple(B.shape) == (batch, dstate, seqlen) == tuple(C.shape)
+    assert A.shape[0] == dim and dstate <= MAX_DSTATE
+    assert z is None or z.shape == u.shape
+    assert D is None or tuple(D.shape) == (dim,)
+    assert delta_bias is None or tuple(delta_bias.shape) == (dim,)
+    _lib.require_cuda(u, delta, A, B, C, D, z, delta_bias)
+    y, state = _SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, bool(delta_softplus))
+    return (y, state) if return_state else y
+
+
+# ---- preference loss ---------------------------------------------------------------------------------------
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, ref, beta, smoothing, ignore_index):
+        rows, length, vocab = logits.shape
+        dev, pairs = logits.device, rows // 2
+        f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)
+        loss, chosen, rejected, stats, slope = f32(), f32(pairs), f32(pairs), f32(rows, length, 2), f32(rows)
+        x = logits.detach()
+        if vocab > 1 and x.stride(2) != 1:
+            x = x.contiguous()
+        a = _lib.MMPreferenceArgs()
+        a.logits, a.labels, a.ref = x.data_ptr(), labels.data_ptr(), ref.data_ptr()
+        a.loss, a.chosen, a.rejected, a.stats, a.slope = (t.data_ptr() for t in (loss, chosen, rejected, stats, slope))
+        a.dtype = _lib.DTYPE_CODE[x.dtype]
+        a.pairs, a.length, a.vocab = pairs, length, vocab
+        a.logits_stride = (ctypes.c_int64 * 2)(*x.stride()[:2])
+        a.ignore_index, a.beta, a.smoothing = ignore_index, beta, smoothing
+        lib = _lib.lib()
+        nbytes = ctypes.c_size_t(0)
+        _lib.check(lib.mm_preference_loss_workspace_size(ctypes.byref(a), ctypes.byref(nbytes)),
+                   "mm_preference_loss_workspace_size")
+        ws = torch.empty(int(nbytes.value), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            rc = lib.mm_preference_loss_fwd(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
+        _lib.check(rc, "mm_preference_loss_fwd")
+        ctx.args = a
+        ctx.save_for_backward(x, labels, stats, slope)
+        ctx.mark_non_differentiable(chosen, rejected)
+        return loss, chosen, rejected
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss, *_):
+        x, labels, stats, slope = ctx.saved_tensors
+        grad = grad_loss.float().contiguous()
+        dlogits = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        a = ctx.args
+        a.logits, a.labels, a.stats, a.slope = (t.data_ptr() for t in (x, labels, stats, slope))
+        a.grad_loss, a.dlogits = grad.data_ptr(), dlogits.data_ptr()
+        a.dlogits_stride = (ctypes.c_int64 * 2)(*dlogits.stride()[:2])
+        with torch.cuda.device(x.device):
+            rc = _lib.lib().mm_preference_loss_bwd(ctypes.byref(a), _lib.stream_handle(x.device))
+        _lib.check(rc, "mm_preference_loss_bwd")
+        return dlogits, None, None, None, None, None
+
+
+def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch.Tensor, *, beta: float = 0.1,
+                    label_smoothing: float = 0.0, ignore_index: int = -100):
+    """Preference loss over pairs of answers, from the policy's logits (2 * pairs, length, vocab): rows 0 .. pairs-1 are the
+    chosen answers, the rest the rejected ones of the same pairs. ``labels`` (2 * pairs, length) int64 are the tokens
+    that the logits are to predict (already shifted), ``ignore_index`` where a token is no part of the answer.
+    ``ref_logps`` (2 * pairs,) are the answers' log-probabilities under the reference model.
+
+    With r = beta * (logp - ref_logp) of an answer and m = r_chosen - r_rejected, the loss is the mean over the pairs of
+    -(1 - label_smoothing) * log sigmoid(m) - label_smoothing * log sigmoid(-m). Returns (loss, chosen, rejected): a
+    float32 scalar, differentiable in the logits, and the (pairs,) float32 values of r, which are not. The answers'
+    log-probabilities are sums over tokens; of an answer without tokens it is 0. Logits of ignored tokens are not
+    read. A label outside the vocabulary makes its pair's values, and the loss, NaN."""
+    assert logits.dim() == 3 and logits.shape[0] >= 2 and logits.shape[0] % 2 == 0 and logits.shape[2] >= 1, \
+        "logits are (2 * pairs, length, vocab)"
+    assert labels.shape == logits.shape[:2] and tuple(ref_logps.shape) == (logits.shape[0],)
+    assert labels.dtype == torch.int64 and ref_logps.is_floating_point()
+    assert 0.0 <= label_smoothing <= 0.5 and beta > 0.0
+    if logits.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {logits.dtype}")
+    _lib.require_cuda(logits, labels, ref_logps)
+    return _PreferenceLoss.apply(logits, labels.contiguous(), _f32(ref_logps), float(beta), float(label_smoothing),
+                                 int(ignore_index))

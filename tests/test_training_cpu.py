@@ -1,0 +1,98 @@
+"""Training operators: refusals and host-side plans that need no GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+from mamba_metal_b200 import _lib, training
+
+
+def size_of(fn, a):
+    n = ctypes.c_size_t(0)
+    return fn(ctypes.byref(a), ctypes.byref(n)), n.value
+
+
+def test_struct_layouts_are_padding_free():
+    scan = 9 + 5 + 6 * 3 + 2 + 3 + 1
+    for s, n in ((_lib.MMCheckpoint8Args, 3 + 4 + 9), (_lib.MMConvCheckpointArgs, 6 + 5 + 12 + 1),
+                 (_lib.MMConvBwdArgs, 9 + 5 + 15 + 1), (_lib.MMPreferenceArgs, 10 + 4 + 4 + 1 + 2),
+                 (_lib.MMScanBwdArgs, scan + 10 + 18)):
+        assert ctypes.sizeof(s) == 8 * n, s.__name__
+
+
+def test_cpu_tensors_are_refused():
+    u, A, B = torch.zeros(1, 2, 8), torch.zeros(2, 4), torch.zeros(1, 4, 8)
+    for call in (lambda: training.selective_scan(u, u, A, B, B), lambda: training.causal_conv1d(u, torch.zeros(2, 4)),
+                 lambda: training.selective_scan_backward(u, u, u, A, B, B),
+                 lambda: training.causal_conv1d_backward(u, u, torch.zeros(2, 4), None),
+                 lambda: training.checkpoint8(u), lambda: training.conv1d_checkpoint8(u, torch.zeros(2, 4), None),
+                 lambda: training.Checkpoint8(u.to(torch.int8), torch.zeros(1, 2, 1, dtype=torch.uint8), u.dtype).restore(),
+                 lambda: training.preference_loss(torch.zeros(2, 3, 5), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2))):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+def test_shapes_and_types_are_checked():
+    u, A, B = torch.zeros(1, 2, 8), torch.zeros(2, 4), torch.zeros(1, 4, 8)
+    bad = [lambda: training.selective_scan(u, u[..., 1:], A, B, B), lambda: training.selective_scan(u, u, A, B, B[..., 1:]),
+           lambda: training.selective_scan(u, u, torch.zeros(3, 4), B, B),
+           lambda: training.selective_scan(u, u, torch.zeros(2, 65), torch.zeros(1, 65, 8), torch.zeros(1, 65, 8)),
+           lambda: training.selective_scan(u, u, A, B, B, D=torch.zeros(3)),
+           lambda: training.selective_scan(u, u, A, B, B, z=u[:, :1]),
+           lambda: training.selective_scan(u, u, A, B, B, delta_bias=torch.zeros(1)),
+           lambda: training.conv1d_checkpoint8(u, torch.zeros(2, 3), None),
+           lambda: training.conv1d_checkpoint8(u, torch.zeros(2, 4), torch.zeros(3)),
+           lambda: training.causal_conv1d_backward(u[..., 1:], u, torch.zeros(2, 4), None),
+           lambda: training.checkpoint8(torch.zeros(()))]
+    labels = torch.zeros(2, 3, dtype=torch.int64)
+    bad += [lambda: training.preference_loss(torch.zeros(3, 3, 5), labels, torch.zeros(3)),
+            lambda: training.preference_loss(torch.zeros(2, 3, 5), labels[:, :2], torch.zeros(2)),
+            lambda: training.preference_loss(torch.zeros(2, 3, 5), labels.int(), torch.zeros(2)),
+            lambda: training.preference_loss(torch.zeros(2, 3, 5), labels, torch.zeros(1)),
+            lambda: training.preference_loss(torch.zeros(2, 3, 5), labels, torch.zeros(2), beta=0.0),
+            lambda: training.preference_loss(torch.zeros(2, 3, 5), labels, torch.zeros(2), label_smoothing=0.6)]
+    for call in bad:
+        with pytest.raises(AssertionError):
+            call()
+    for call in (lambda: training.checkpoint8(u.double()), lambda: training.checkpoint8(u.long()),
+                 lambda: training.conv1d_checkpoint8(u.double(), torch.zeros(2, 4), None),
+                 lambda: training.preference_loss(torch.zeros(2, 3, 5, dtype=torch.float64), labels, torch.zeros(2))):
+        with pytest.raises(TypeError):
+            call()
+
+
+def test_c_entries_refuse():
+    lib = _lib.lib()
+    c = _lib.MMCheckpoint8Args()
+    c.dtype, c.batch, c.dim, c.length = 5, 1, 1, 1
+    assert lib.mm_checkpoint8_pack(ctypes.byref(c), None) == -3
+    c.dtype, c.length = 1, -1
+    assert lib.mm_checkpoint8_unpack(ctypes.byref(c), None) == -2
+    c.length = 1
+    assert lib.mm_checkpoint8_pack(ctypes.byref(c), None) == -1
+    assert lib.mm_checkpoint8_pack(None, None) == -1
+    v = _lib.MMConvBwdArgs()
+    v.dtype, v.batch, v.dim, v.seqlen, v.width = 1, 1, 8, 16, 3
+    assert size_of(lib.mm_causal_conv1d_bwd_workspace_size, v)[0] == -2
+    v.width = 4
+    assert lib.mm_causal_conv1d_bwd(ctypes.byref(v), None, 0, None) == -1
+    f = _lib.MMConvCheckpointArgs()
+    f.dtype, f.batch, f.dim, f.seqlen, f.width = 1, 1, 8, 16, 4
+    assert lib.mm_causal_conv1d_fwd_checkpoint8(ctypes.byref(f), None) == -1
+    p = _lib.MMPreferenceArgs()
+    p.dtype, p.pairs, p.length, p.vocab = 2, 0, 3, 5
+    assert size_of(lib.mm_preference_loss_workspace_size, p)[0] == -2
+    p.pairs = 1
+    assert lib.mm_preference_loss_fwd(ctypes.byref(p), None, 0, None) == -1
+    assert lib.mm_preference_loss_bwd(ctypes.byref(p), None) == -1
+    s = _lib.MMScanBwdArgs()
+    s.fwd.dtype, s.fwd.batch, s.fwd.dim, s.fwd.dstate, s.fwd.seqlen = 1, 1, 8, 65, 16
+    assert size_of(lib.mm_selective_scan_bwd_workspace_size, s)[0] == -2
+    s.fwd.dstate, s.fwd.dtype = 16, 7
+    assert size_of(lib.mm_selective_scan_bwd_workspace_size, s)[0] == -3
+    s.fwd.dtype = 2
+    assert lib.mm_selective_scan_bwd(ctypes.byref(s), None, 0, None) == -1
+    rc, one = size_of(lib.mm_selective_scan_bwd_workspace_size, s)
+    s.fwd.seqlen = 65
+    assert rc == 0 and size_of(lib.mm_selective_scan_bwd_workspace_size, s)[1] > one > 0
