@@ -34,7 +34,8 @@ struct Params {
   int batch, dim, dstate_n, seqlen;
   int softplus;
   int vec;        // every activation's rows are contiguous in time and 16-byte aligned
-  int by_channel; // activations are contiguous along channels
+  int by_channel; // u is contiguous along channels
+  int ahead;      // grad_kernel copies its raw inputs ahead: all contiguous along one axis, rows 16-byte aligned
   // workspace
   float *hst, *kst, *sum_d;  // (batch, chunks, dim, np): states and k; (batch, chunks, dim)
   float *pB, *pC;            // (batch, groups, chunks, passes, 16, 64)
@@ -53,12 +54,26 @@ MM_DEV Gate gate_of(float z) {
   const float s = rcp(1.f + ex2(-z * kLog2e));
   return Gate{z * s, s * fmaf(z, 1.f - s, 1.f)};
 }
-// softplus with the forward's cutoff; log1pf keeps small steps' relative accuracy
-MM_DEV float step_of(float raw, int softplus) { return softplus && raw <= 20.f ? log1pf(expf(raw)) : raw; }
+// exp(x) for x <= 20: 2^(x log2 e) with the product's rounding error carried along
+MM_DEV float exp_of(float x) {
+  const float y = x * kLog2e;
+  const float rest = fmaf(x, 1.925963033e-8f, fmaf(x, kLog2e, -y));  // the second word of log2 e
+  const float e = ex2(y);
+  return fmaf(e, rest * kLn2, e);
+}
+// softplus with the forward's cutoff at 20, without a branch (eight of them run side by side). log(1 + e): below
+// e = 0.4 as 2 artanh(e / (2 + e)), whose series keeps the relative accuracy of small steps (truncated below
+// 1e-7); above, where the result is no longer small against 1, as lg2(1 + e).
+MM_DEV float step_of(float raw, int softplus) {
+  const float e = exp_of(fminf(raw, 20.f));
+  const float s = e * rcp(2.f + e), z = s * s;
+  const float small = s * fmaf(z, fmaf(z, fmaf(z, 0.285714286f, 0.4f), 0.666666667f), 2.f);
+  const float r = e < 0.4f ? small : lg2(1.f + e) * kLn2;
+  return softplus && raw <= 20.f ? r : raw;
+}
 MM_DEV float step_slope(float raw, int softplus) {
-  if (!softplus || raw > 20.f) return 1.f;
-  const float e = expf(raw);
-  return e * rcp(1.f + e);
+  const float e = exp_of(fminf(raw, 20.f));
+  return softplus && raw <= 20.f ? e * rcp(1.f + e) : 1.f;
 }
 
 // Eight consecutive steps of one channel; n of them exist
@@ -99,31 +114,38 @@ template <typename T> MM_DEV void store_steps(T* p, long long s, bool vec, int n
 
 // Where a thread's unit (eight steps of a channel) of a staged tile lies. Lanes run along whichever of time and
 // channels is contiguous in memory.
-MM_DEV void unit_of(int i, int by_channel, int& ch, int& seg) {
+template <int CH> MM_DEV void unit_of(int i, int by_channel, int& ch, int& seg) {
   if (by_channel) {
-    ch = i % kCh;
-    seg = i / kCh;
+    ch = i % CH;
+    seg = i / CH;
   } else {
     seg = i % (kT / kK);
     ch = i / (kT / kK);
   }
 }
 
-// d, d u and e of a unit (zeros where there are no steps: a = 1 there, so states and k pass through)
-template <typename T, bool HAS_Z>
-MM_DEV void stage_unit(const Params& p, int b, int d, int t, float (&dt)[kK], float (&dtu)[kK], float (&e)[kK]) {
+// The raw values of a unit, so that several units' loads can be in flight before the first is worked on
+struct Raw {
+  float dt[kK], u[kK], e[kK], g[kK];
+};
+template <typename T, bool HAS_Z> MM_DEV void load_unit(const Params& p, int b, int d, int t, Raw& r) {
   const int n = min(kK, p.seqlen - t);
-  float u[kK], g[kK];
-  load_steps(static_cast<const T*>(p.delta) + b * p.ds[0] + d * p.ds[1] + t * p.ds[2], p.ds[2], p.vec, n, dt);
-  load_steps(static_cast<const T*>(p.u) + b * p.us[0] + d * p.us[1] + t * p.us[2], p.us[2], p.vec, n, u);
-  load_steps(static_cast<const T*>(p.dy) + b * p.ys[0] + d * p.ys[1] + t * p.ys[2], p.ys[2], p.vec, n, e);
-  if (HAS_Z) load_steps(static_cast<const T*>(p.z) + b * p.zs[0] + d * p.zs[1] + t * p.zs[2], p.zs[2], p.vec, n, g);
+  load_steps(static_cast<const T*>(p.delta) + b * p.ds[0] + d * p.ds[1] + t * p.ds[2], p.ds[2], p.vec, n, r.dt);
+  load_steps(static_cast<const T*>(p.u) + b * p.us[0] + d * p.us[1] + t * p.us[2], p.us[2], p.vec, n, r.u);
+  load_steps(static_cast<const T*>(p.dy) + b * p.ys[0] + d * p.ys[1] + t * p.ys[2], p.ys[2], p.vec, n, r.e);
+  if (HAS_Z) load_steps(static_cast<const T*>(p.z) + b * p.zs[0] + d * p.zs[1] + t * p.zs[2], p.zs[2], p.vec, n, r.g);
+}
+
+// d, d u and e (zeros where there are no steps: a = 1 there, so states and k pass through)
+template <bool HAS_Z>
+MM_DEV void stage_unit(const Params& p, int d, int t, const Raw& r, float (&dt)[kK], float (&dtu)[kK], float (&e)[kK]) {
+  const int n = min(kK, p.seqlen - t);
   const float bias = p.bias ? p.bias[d] : 0.f;
 #pragma unroll
   for (int k = 0; k < kK; ++k) {
-    dt[k] = k < n ? step_of(dt[k] + bias, p.softplus) : 0.f;
-    dtu[k] = dt[k] * u[k];
-    if (HAS_Z) e[k] *= gate_of(g[k]).silu;
+    dt[k] = k < n ? step_of(r.dt[k] + bias, p.softplus) : 0.f;
+    dtu[k] = dt[k] * r.u[k];
+    e[k] = HAS_Z ? r.e[k] * gate_of(r.g[k]).silu : r.e[k];
   }
 }
 
@@ -132,6 +154,19 @@ MM_DEV f2_t ex2_pair(f2_t x) {
   return f2_pack(ex2(v.x), ex2(v.y));
 }
 MM_DEV f2_t dup(float x) { return f2_pack(x, x); }
+#ifdef V_DUP
+MM_DEV f2_t mul1(f2_t a, float x) { return f2_mul(a, dup(x)); }
+MM_DEV f2_t fma1(f2_t a, float x, f2_t c) { return f2_fma(a, dup(x), c); }
+#else
+MM_DEV f2_t mul1(f2_t a, float x) {
+  const float2 v = f2_unpack(a);
+  return f2_pack(v.x * x, v.y * x);
+}
+MM_DEV f2_t fma1(f2_t a, float x, f2_t c) {
+  const float2 v = f2_unpack(a), w = f2_unpack(c);
+  return f2_pack(fmaf(v.x, x, w.x), fmaf(v.y, x, w.y));
+}
+#endif
 
 // Four consecutive states' entries of a (dim, dstate)-shaped row; zeros past the last state
 MM_DEV float4 load_A(const Params& p, int d, int n0) {
@@ -166,10 +201,12 @@ __global__ void __launch_bounds__(kCarryThreads) carry_kernel(const Params p) {
   const int c = (int)(bc % p.chunks), b = (int)(bc / p.chunks), t0 = c * kT;
   for (int i = threadIdx.x; i < kCh * kT / kK; i += kCarryThreads) {
     int ch, seg;
-    unit_of(i, p.by_channel, ch, seg);
+    unit_of<kCh>(i, p.by_channel, ch, seg);
     float dt[kK], dtu[kK], e[kK];
     if (d0 + ch < p.dim) {
-      stage_unit<T, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, dt, dtu, e);
+      Raw r;
+      load_unit<T, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, r);
+      stage_unit<HAS_Z>(p, d0 + ch, t0 + seg * kK, r, dt, dtu, e);
     } else {
 #pragma unroll
       for (int k = 0; k < kK; ++k) dt[k] = dtu[k] = e[k] = 0.f;
@@ -258,9 +295,62 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
 // runs its steps from zero, a scan over the eight segments gives its true start, and a second run the values;
 // the same backwards. B, C and the sums for dB and dC stay in registers over all channels, so the sum over
 // channels costs nothing but the final one over warps; sums over states go across the four quads.
+#ifndef V_GCH
+#define V_GCH 32
+#endif
+#ifndef V_OCC
+#define V_OCC 2
+#endif
+constexpr int kGCh = V_GCH;      // channels staged at a time
 constexpr int kGradWarps = 4;
 constexpr int kGradThreads = kGradWarps * 32;
-constexpr int kGradSmem = 6 * kCh * kPitch * (int)sizeof(float);
+constexpr int kGradSmem = 5 * kGCh * kPitch * (int)sizeof(float);  // and the raw buffers
+static_assert(kGradThreads == kGCh * kNB / 4, "a thread per channel and four states");
+
+// The raw tile of one array in shared memory, [channel][step] or, contiguous along channels, [step][channel]
+constexpr int kRawOne = kGCh * kT;
+constexpr int kRaw = 4 * kRawOne;
+
+MM_DEV void cp_async16_part(void* dst, const void* src, int bytes) {  // zeros after the first `bytes`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+// Starts copying a tile's raw inputs; one commit group. Channels and steps that do not exist arrive as zeros.
+template <typename T>
+MM_DEV void copy_one(const void* base, const long long (&st)[3], const Params& p, int b, int t0, int d0, T* raw) {
+  const T* x = static_cast<const T*>(base) + b * st[0] + d0 * st[1] + t0 * st[2];
+  constexpr int per = 16 / (int)sizeof(T);
+  const int width = min(p.width, p.dim - d0), steps = min(kT, p.seqlen - t0);
+#pragma unroll
+  for (int i = threadIdx.x; i < kRawOne / per; i += kGradThreads) {
+    const int row = p.by_channel ? i / (kGCh / per) : i / (kT / per);
+    const int col = (p.by_channel ? i % (kGCh / per) : i % (kT / per)) * per;
+    const int n = p.by_channel ? (row < steps ? width - col : 0) : (row < width ? steps - col : 0);
+    const T* src = n > 0 ? x + row * (p.by_channel ? st[2] : st[1]) + col : x;
+    cp_async16_part(raw + i * per, src, min(max(n, 0), per) * (int)sizeof(T));
+  }
+}
+template <typename T, bool HAS_Z> MM_DEV void copy_ahead(const Params& p, int b, int t0, int d0, T* raw) {
+  if (d0 < p.dim) {
+    copy_one(p.delta, p.ds, p, b, t0, d0, raw);
+    copy_one(p.u, p.us, p, b, t0, d0, raw + kRawOne);
+    copy_one(p.dy, p.ys, p, b, t0, d0, raw + 2 * kRawOne);
+    if (HAS_Z) copy_one(p.z, p.zs, p, b, t0, d0, raw + 3 * kRawOne);
+  }
+  cp_async_commit();
+}
+template <typename T, bool HAS_Z>
+MM_DEV void load_unit(const Params& p, int b, int d, int t, Raw& r, const T* raw, int ch, int seg) {
+  if (!p.ahead) {
+    load_unit<T, HAS_Z>(p, b, d, t, r);
+    return;
+  }
+  const T* x = raw + (p.by_channel ? seg * kK * kGCh + ch : ch * kT + seg * kK);
+  const int st = p.by_channel ? kGCh : 1;
+  load_steps(x, st, !p.by_channel, kK, r.dt);
+  load_steps(x + kRawOne, st, !p.by_channel, kK, r.u);
+  load_steps(x + 2 * kRawOne, st, !p.by_channel, kK, r.e);
+  if (HAS_Z) load_steps(x + 3 * kRawOne, st, !p.by_channel, kK, r.g);
+}
 
 // Position of step t in a staged row: quarter rows of every segment lie side by side, so that the eight
 // segments' 16-byte reads fall into different banks.
@@ -296,14 +386,21 @@ MM_DEV float2 sum_quads(const float (&v)[kK], int q) {
 }
 
 template <typename T, bool HAS_Z>
-__global__ void __launch_bounds__(kGradThreads, 2) grad_kernel(const Params p) {
+__global__ void __launch_bounds__(kGradThreads, V_OCC) grad_kernel(const Params p) {
   extern __shared__ float4 smem4[];
   float* sd = reinterpret_cast<float*>(smem4);  // [channel][step] each
-  float* sdu = sd + kCh * kPitch;
-  float* se = sdu + kCh * kPitch;
-  float* s1 = se + kCh * kPitch;   // sum_n g B
-  float* s2 = s1 + kCh * kPitch;   // sum_n A log2(e) w
-  float* s3 = s2 + kCh * kPitch;   // sum_n C h
+  float* sdu = sd + kGCh * kPitch;
+  float* se = sdu + kGCh * kPitch;
+  float* s2 = se + kGCh * kPitch;  // sum_n A w
+  float* s3 = s2 + kGCh * kPitch;  // sum_n C h
+  T* raw = reinterpret_cast<T*>(s3 + kGCh * kPitch);  // two buffers of the raw delta, u, dy, z
+  float* more = reinterpret_cast<float*>(raw + 2 * kRaw);
+  // sum_n g B, and rows of [A, state, k][16 states]: where one pass takes all states, in the place of the d u
+  // that the same lanes have read, and of the sums that the same warp has yet to write
+  const bool once = p.passes == 1;
+  float* s1 = once ? sdu : more;
+  float* in = once ? s2 : more + kGCh * kPitch;
+  __shared__ float sums[2][kGCh][kT / kK];  // of dD and ddelta, per segment
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane & 3, s = lane >> 2;
   const int group = (int)(blockIdx.x % p.groups);
   const long long bc = blockIdx.x / p.groups;
@@ -322,18 +419,46 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_kernel(const Params p) {
       Cv[i][1] = f2_pack(y.z, y.w);
       accB[i][0] = accB[i][1] = accC[i][0] = accC[i][1] = dup(0.f);
     }
+    if (pass == 0 && p.ahead) copy_ahead<T, HAS_Z>(p, b, t0, group * p.tiles * p.width, raw);
     for (int tile = 0; tile < p.tiles; ++tile) {
       const int d0 = (group * p.tiles + tile) * p.width;
       const int width = min(p.width, p.dim - d0);  // channels of this tile; none past the last
       if (width <= 0) break;
+      T* now = raw + (tile & 1) * kRaw;
+      __syncthreads();  // the tile before has been read
+      // of this pass's states, for every channel: A, the incoming state and k (one of each per thread)
+      const int jc = threadIdx.x / 4, jn = pass * kNB + 4 * (threadIdx.x % 4);
+      float4 jA = f4(0.f, 0.f, 0.f, 0.f), jh = jA, jk = jA;
+      if (jc < width) {
+        jA = load_A(p, d0 + jc, jn);
+        if (p.chunks > 1) {
+          const long long at = (bc * p.dim + d0 + jc) * p.np + jn;
+          if (jn < p.np) {
+            jh = *reinterpret_cast<const float4*>(p.hst + at);
+            jk = *reinterpret_cast<const float4*>(p.kst + at);
+          }
+        } else if (p.dstate) {
+          const float* x = p.dstate + ((long long)b * p.dim + d0 + jc) * p.dstate_n + jn;
+          const int m = p.dstate_n - jn;
+          jk = f4(m > 0 ? x[0] : 0.f, m > 1 ? x[1] : 0.f, m > 2 ? x[2] : 0.f, m > 3 ? x[3] : 0.f);
+        }
+      }
       if (pass == 0) {
-        __syncthreads();  // the tile before has been read
-        for (int i = threadIdx.x; i < kCh * kT / kK; i += kGradThreads) {
+        if (p.ahead) {
+          if (tile + 1 < p.tiles) copy_ahead<T, HAS_Z>(p, b, t0, d0 + p.width, raw + ((tile + 1) & 1) * kRaw);
+          else cp_async_commit();
+          cp_async_wait<1>();
+          __syncthreads();
+        }
+#pragma unroll
+        for (int i = threadIdx.x; i < kGCh * kT / kK; i += kGradThreads) {
           int ch, seg;
-          unit_of(i, p.by_channel, ch, seg);
+          unit_of<kGCh>(i, p.by_channel, ch, seg);
           if (ch >= width) continue;
           float dt[kK], dtu[kK], e[kK];
-          stage_unit<T, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, dt, dtu, e);
+          Raw r;
+          load_unit<T, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, r, now, ch, seg);
+          stage_unit<HAS_Z>(p, d0 + ch, t0 + seg * kK, r, dt, dtu, e);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int at = ch * kPitch + at_step(seg, h);
@@ -342,29 +467,18 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_kernel(const Params p) {
             *reinterpret_cast<float4*>(se + at) = f4(e[4 * h], e[4 * h + 1], e[4 * h + 2], e[4 * h + 3]);
           }
         }
-        __syncthreads();
       }
+      float* j = in + jc * kPitch + 4 * (threadIdx.x % 4);
+      *reinterpret_cast<float4*>(j) = jA;
+      *reinterpret_cast<float4*>(j + kNB) = jh;
+      *reinterpret_cast<float4*>(j + 2 * kNB) = jk;
+      __syncthreads();
       for (int ch = warp; ch < width; ch += kGradWarps) {
         const int d = d0 + ch;
-        const float4 A = load_A(p, d, n0);
-        const f2_t A2[2] = {f2_mul(f2_pack(A.x, A.y), dup(kLog2e)), f2_mul(f2_pack(A.z, A.w), dup(kLog2e))};
-        f2_t first[2] = {dup(0.f), dup(0.f)}, last[2] = {dup(0.f), dup(0.f)};
-        if (n0 < p.np) {
-          const long long at = (bc * p.dim + d) * p.np + n0;
-          if (p.chunks > 1) {
-            const float4 x = *reinterpret_cast<const float4*>(p.hst + at);
-            const float4 y = *reinterpret_cast<const float4*>(p.kst + at);
-            first[0] = f2_pack(x.x, x.y);
-            first[1] = f2_pack(x.z, x.w);
-            last[0] = f2_pack(y.x, y.y);
-            last[1] = f2_pack(y.z, y.w);
-          } else if (p.dstate) {
-            const float* x = p.dstate + ((long long)b * p.dim + d) * p.dstate_n + n0;
-            const int n = p.dstate_n - n0;
-            last[0] = f2_pack(n > 0 ? x[0] : 0.f, n > 1 ? x[1] : 0.f);
-            last[1] = f2_pack(n > 2 ? x[2] : 0.f, n > 3 ? x[3] : 0.f);
-          }
-        }
+        const float4* row = reinterpret_cast<const float4*>(in + ch * kPitch);
+        const float4 xA = row[q], xh = row[kNB / 4 + q], xk = row[2 * kNB / 4 + q];
+        const f2_t A2[2] = {f2_mul(f2_pack(xA.x, xA.y), dup(kLog2e)), f2_mul(f2_pack(xA.z, xA.w), dup(kLog2e))};
+        const f2_t first[2] = {f2_pack(xh.x, xh.y), f2_pack(xh.z, xh.w)}, last[2] = {f2_pack(xk.x, xk.y), f2_pack(xk.z, xk.w)};
         float dt[kK], dtu[kK], e[kK];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -382,59 +496,34 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_kernel(const Params p) {
         f2_t a[kK][2], ah[kK][2], P[2], Q[2], h[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          Q[j] = P[j] = ex2_pair(f2_mul(dup(sum), A2[j]));
+          Q[j] = P[j] = ex2_pair(mul1(A2[j], sum));
           h[j] = s == 0 ? first[j] : dup(0.f);
         }
-        // forwards: from zero, then across segments, then again
-#pragma unroll
-        for (int i = 0; i < kK; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            a[i][j] = ex2_pair(f2_mul(dup(dt[i]), A2[j]));
-            h[j] = f2_fma(a[i][j], h[j], f2_mul(dup(dtu[i]), Bv[i][j]));
-          }
-#pragma unroll
-        for (int by = 1; by < 8; by *= 2)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const f2_t hb = shfl_up2(h[j], 4 * by), Pb = shfl_up2(P[j], 4 * by);
-            if (s >= by) {
-              h[j] = f2_fma(P[j], hb, h[j]);
-              P[j] = f2_mul(P[j], Pb);
-            }
-          }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const f2_t hb = shfl_up2(h[j], 4);
-          h[j] = s == 0 ? first[j] : hb;
-        }
-        float v3[kK];
-#pragma unroll
-        for (int i = 0; i < kK; ++i) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            ah[i][j] = f2_mul(a[i][j], h[j]);
-            h[j] = f2_fma(dup(dtu[i]), Bv[i][j], ah[i][j]);
-            accC[i][j] = f2_fma(h[j], dup(e[i]), accC[i][j]);
-          }
-          if (HAS_Z) {
-            const float2 x = f2_unpack(f2_fma(h[0], Cv[i][0], f2_mul(h[1], Cv[i][1])));
-            v3[i] = x.x + x.y;
-          }
-        }
-        // backwards
+        // both directions from zero (neither needs the other), then across segments
         f2_t k[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) k[j] = s == 7 ? last[j] : dup(0.f);
 #pragma unroll
-        for (int i = kK - 1; i >= 0; --i)
+        for (int i = 0; i < kK; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) k[j] = f2_mul(a[i][j], f2_fma(Cv[i][j], dup(e[i]), k[j]));
+          for (int j = 0; j < 2; ++j) a[i][j] = ex2_pair(mul1(A2[j], dt[i]));
+#pragma unroll
+        for (int i = 0; i < kK; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            h[j] = f2_fma(a[i][j], h[j], mul1(Bv[i][j], dtu[i]));
+            k[j] = f2_mul(a[kK - 1 - i][j], fma1(Cv[kK - 1 - i][j], e[kK - 1 - i], k[j]));
+          }
 #pragma unroll
         for (int by = 1; by < 8; by *= 2)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const f2_t kb = shfl_down2(k[j], 4 * by), Qb = shfl_down2(Q[j], 4 * by);
+            const f2_t hb = shfl_up2(h[j], 4 * by), kb = shfl_down2(k[j], 4 * by);
+            const f2_t Pb = shfl_up2(P[j], 4 * by), Qb = shfl_down2(Q[j], 4 * by);
+            if (s >= by) {
+              h[j] = f2_fma(P[j], hb, h[j]);
+              P[j] = f2_mul(P[j], Pb);
+            }
             if (s + by < 8) {
               k[j] = f2_fma(Q[j], kb, k[j]);
               Q[j] = f2_mul(Q[j], Qb);
@@ -442,8 +531,23 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_kernel(const Params p) {
           }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const f2_t kb = shfl_down2(k[j], 4);
+          const f2_t hb = shfl_up2(h[j], 4), kb = shfl_down2(k[j], 4);
+          h[j] = s == 0 ? first[j] : hb;
           k[j] = s == 7 ? last[j] : kb;
+        }
+        float v3[kK];
+#pragma unroll
+        for (int i = 0; i < kK; ++i) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            ah[i][j] = f2_mul(a[i][j], h[j]);
+            h[j] = fma1(Bv[i][j], dtu[i], ah[i][j]);
+            accC[i][j] = fma1(h[j], e[i], accC[i][j]);
+          }
+          if (HAS_Z) {
+            const float2 x = f2_unpack(f2_fma(h[0], Cv[i][0], f2_mul(h[1], Cv[i][1])));
+            v3[i] = x.x + x.y;
+          }
         }
         float v1[kK], v2[kK];
         f2_t dA[2] = {dup(0.f), dup(0.f)};
@@ -452,13 +556,13 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_kernel(const Params p) {
           f2_t gB = dup(0.f), wA = dup(0.f);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const f2_t g = f2_fma(Cv[i][j], dup(e[i]), k[j]);
+            const f2_t g = fma1(Cv[i][j], e[i], k[j]);
             k[j] = f2_mul(a[i][j], g);
-            accB[i][j] = f2_fma(g, dup(dtu[i]), accB[i][j]);
+            accB[i][j] = fma1(g, dtu[i], accB[i][j]);
             gB = f2_fma(g, Bv[i][j], gB);
             const f2_t w = f2_mul(g, ah[i][j]);
             wA = f2_fma(w, A2[j], wA);
-            dA[j] = f2_fma(w, dup(dt[i]), dA[j]);
+            dA[j] = fma1(w, dt[i], dA[j]);
           }
           const float2 x = f2_unpack(gB), y = f2_unpack(wA);
           v1[i] = x.x + x.y;
@@ -494,18 +598,14 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_kernel(const Params p) {
       }
       if (pass == p.passes - 1) {
         __syncthreads();
-        for (int i = threadIdx.x; i < kCh * kT / kK; i += kGradThreads) {
+#pragma unroll
+        for (int i = threadIdx.x; i < kGCh * kT / kK; i += kGradThreads) {
           int ch, seg;
-          unit_of(i, p.by_channel, ch, seg);
+          unit_of<kGCh>(i, p.by_channel, ch, seg);
           if (ch >= width) continue;
           const int d = d0 + ch, t = t0 + seg * kK, n = min(kK, p.seqlen - t);
-          float u[kK], raw[kK], g[kK], z[kK];
-          load_steps(static_cast<const T*>(p.u) + b * p.us[0] + d * p.us[1] + t * p.us[2], p.us[2], p.vec, n, u);
-          load_steps(static_cast<const T*>(p.delta) + b * p.ds[0] + d * p.ds[1] + t * p.ds[2], p.ds[2], p.vec, n, raw);
-          if (HAS_Z) {
-            load_steps(static_cast<const T*>(p.dy) + b * p.ys[0] + d * p.ys[1] + t * p.ys[2], p.ys[2], p.vec, n, g);
-            load_steps(static_cast<const T*>(p.z) + b * p.zs[0] + d * p.zs[1] + t * p.zs[2], p.zs[2], p.vec, n, z);
-          }
+          Raw r;
+          load_unit<T, HAS_Z>(p, b, d, t, r, now, ch, seg);
           const float bias = p.bias ? p.bias[d] : 0.f, D = p.D ? p.D[d] : 0.f;
           float du[kK], dd[kK], sumD = 0.f, sumb = 0.f;
 #pragma unroll
@@ -513,25 +613,25 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_kernel(const Params p) {
             const int at = ch * kPitch + at_step(seg, k >> 2) + (k & 3);
             const float e = se[at], gB = s1[at];
             du[k] = fmaf(sd[at], gB, D * e);
-            dd[k] = fmaf(u[k], gB, s2[at] * kLn2) * step_slope(raw[k] + bias, p.softplus);
-            sumD = fmaf(e, u[k], sumD);
+            dd[k] = fmaf(r.u[k], gB, s2[at] * kLn2) * step_slope(r.dt[k] + bias, p.softplus);
+            sumD = fmaf(e, r.u[k], sumD);
             sumb += k < n ? dd[k] : 0.f;
-            if (HAS_Z) z[k] = g[k] * fmaf(D, u[k], s3[at]) * gate_of(z[k]).slope;
+            if (HAS_Z) r.g[k] = r.e[k] * fmaf(D, r.u[k], s3[at]) * gate_of(r.g[k]).slope;
           }
           store_steps(static_cast<T*>(p.du) + b * p.dus[0] + d * p.dus[1] + t * p.dus[2], p.dus[2], p.vec, n, du);
           store_steps(static_cast<T*>(p.ddelta) + b * p.dds[0] + d * p.dds[1] + t * p.dds[2], p.dds[2], p.vec, n, dd);
           if (HAS_Z)
-            store_steps(static_cast<T*>(p.dz) + b * p.dzs[0] + d * p.dzs[1] + t * p.dzs[2], p.dzs[2], p.vec, n, z);
-          sdu[ch * kPitch + seg] = sumD;  // d u has been used
-          sdu[ch * kPitch + kT / kK + seg] = sumb;
+            store_steps(static_cast<T*>(p.dz) + b * p.dzs[0] + d * p.dzs[1] + t * p.dzs[2], p.dzs[2], p.vec, n, r.g);
+          sums[0][ch][seg] = sumD;
+          sums[1][ch][seg] = sumb;
         }
         __syncthreads();
         for (int ch = threadIdx.x; ch < width; ch += kGradThreads) {
           float x = 0.f, y = 0.f;
 #pragma unroll
           for (int seg = 0; seg < kT / kK; ++seg) {
-            x += sdu[ch * kPitch + seg];
-            y += sdu[ch * kPitch + kT / kK + seg];
+            x += sums[0][ch][seg];
+            y += sums[1][ch][seg];
           }
           p.pD[bc * p.dim + d0 + ch] = x;
           p.pbias[bc * p.dim + d0 + ch] = y;
@@ -541,8 +641,8 @@ __global__ void __launch_bounds__(kGradThreads, 2) grad_kernel(const Params p) {
     // dB and dC of this group's channels: the warps' sums, in order, as [state][step]
     __syncthreads();
     float* all = sd;  // [warp][B or C][state][step]; the staged rows that a later pass reads are restored below
-    static_assert(kGradWarps * 2 * kNB * kT <= 3 * kCh * kPitch, "the warps' sums fit the free rows");
-    all = p.passes > 1 ? s3 + kCh * kPitch : sd;
+    static_assert(kGradWarps * 2 * kNB * kT <= (5 * kGCh * kPitch), "the warps' sums fit the free rows");
+    all = once ? sd : more + 2 * kGCh * kPitch;
     float* mine = all + warp * 2 * kNB * kT;
 #pragma unroll
     for (int i = 0; i < kK; ++i)
@@ -643,9 +743,9 @@ int make_layout(const MMScanBwdArgs* a, Layout* l) {
   // tile over the passes, so there one tile is the most.
   const long long rows = f.batch * (l->chunks > 0 ? l->chunks : 1);
   long long want = f.dim * rows / (4 * 2 * 148);
-  l->width = want >= kCh ? kCh : want >= 32 ? 32 : 16;
-  long long tiles = want / kCh;
-  l->tiles = (int)(l->passes > 1 || tiles < 1 ? 1 : tiles > 8 ? 8 : tiles);
+  l->width = want >= kGCh ? kGCh : 16;
+  long long tiles = want / kGCh;
+  l->tiles = (int)(l->passes > 1 || tiles < 1 ? 1 : tiles > 512 / kGCh ? 512 / kGCh : tiles);
   const long long per = (long long)l->width * l->tiles;
   l->groups = (int)((f.dim + per - 1) / per);
   size_t at = 0;
@@ -675,7 +775,8 @@ inline void copy3(long long (&to)[3], const int64_t* from) {
 template <typename T, bool HAS_Z> int launch(const Params& p, cudaStream_t s) {
   const long long rows = (long long)p.batch * p.chunks;
   const int carry_smem = 3 * kT * kCarryPitch * (int)sizeof(float);
-  const int grad_smem = kGradSmem + (p.passes > 1 ? kGradWarps * 2 * kNB * kT * (int)sizeof(float) : 0);
+  const int grad_smem = kGradSmem + 2 * kRaw * (int)sizeof(T) +
+                        (p.passes > 1 ? (2 * kGCh * kPitch + kGradWarps * 2 * kNB * kT) * (int)sizeof(float) : 0);
   const long long dtiles = (p.dim + kCh - 1) / kCh;
   if (rows * dtiles > 0x7fffffffLL || rows * p.groups > 0x7fffffffLL) return MM_ERR_SHAPE;
   if (p.chunks > 1) {
@@ -706,6 +807,11 @@ template <typename T> int launch_z(const Params& p, cudaStream_t s) {
 bool rows_aligned(const void* q, const int64_t* st, const MMScanArgs& f) {
   const int es = dtype_size(f.dtype);
   return aligned16(q) && st[2] == 1 && (f.batch <= 1 || st[0] * es % 16 == 0) && (f.dim <= 1 || st[1] * es % 16 == 0);
+}
+
+bool columns_aligned(const void* q, const int64_t* st, const MMScanArgs& f) {
+  const int es = dtype_size(f.dtype);
+  return aligned16(q) && st[1] == 1 && (f.batch <= 1 || st[0] * es % 16 == 0) && st[2] * es % 16 == 0;
 }
 
 }  // namespace bwd
@@ -782,6 +888,11 @@ extern "C" int mm_selective_scan_bwd(const MMScanBwdArgs* a, void* workspace, si
           rows_aligned(a->ddelta, a->ddelta_stride, f) &&
           (!f.z || (rows_aligned(f.z, f.z_stride, f) && rows_aligned(a->dz, a->dz_stride, f)));
   p.by_channel = !p.vec && f.u_stride[1] == 1 && f.u_stride[2] != 1;
+  const void* act[4] = {f.u, f.delta, a->dy, f.z};
+  const int64_t* act_stride[4] = {f.u_stride, f.delta_stride, a->dy_stride, f.z_stride};
+  p.ahead = 1;
+  for (int i = 0; i < (f.z ? 4 : 3); ++i)
+    if (!(p.by_channel ? columns_aligned(act[i], act_stride[i], f) : rows_aligned(act[i], act_stride[i], f))) p.ahead = 0;
   p.chunks = l.chunks;
   p.np = l.np;
   p.passes = l.passes;
