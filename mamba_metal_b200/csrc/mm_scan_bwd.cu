@@ -18,8 +18,9 @@
 namespace mm {
 namespace bwd {
 
-constexpr int kT = 64;        // steps of a chunk
+constexpr int kT = 32;        // steps of a chunk
 constexpr int kK = 8;         // steps of a lane
+constexpr int kSegs = kT / kK;
 constexpr int kCh = 64;       // channels staged at a time
 constexpr int kPitch = kT + 4;  // floats of a staged row; rows stay 16-byte aligned, neighbours in other banks
 constexpr int kNB = 16;       // states of a pass
@@ -46,34 +47,52 @@ struct Params {
 
 MM_DEV float4 f4(float a, float b, float c, float d) { return make_float4(a, b, c, d); }
 
-// ---- elementwise parts -----------------------------------------------------------------------------
-struct Gate {
-  float silu, slope;  // silu(z), silu'(z)
-};
-MM_DEV Gate gate_of(float z) {
-  const float s = rcp(1.f + ex2(-z * kLog2e));
-  return Gate{z * s, s * fmaf(z, 1.f - s, 1.f)};
+// ---- elementwise parts, on pairs of steps -------------------------------------------------------------
+MM_DEV f2_t dup(float x) { return f2_pack(x, x); }
+MM_DEV f2_t ex2_pair(f2_t x) {
+  const float2 v = f2_unpack(x);
+  return f2_pack(ex2(v.x), ex2(v.y));
+}
+MM_DEV f2_t rcp_pair(f2_t x) {
+  const float2 v = f2_unpack(x);
+  return f2_pack(rcp(v.x), rcp(v.y));
+}
+MM_DEV f2_t sigmoid(f2_t z) { return rcp_pair(f2_add(ex2_pair(f2_mul(z, dup(-kLog2e))), dup(1.f))); }
+MM_DEV f2_t silu_of(f2_t z) { return f2_mul(z, sigmoid(z)); }
+// silu'(z) = s (1 + z (1 - s))
+MM_DEV f2_t silu_slope(f2_t z) {
+  const f2_t s = sigmoid(z);
+  return f2_mul(s, f2_fma(z, f2_sub(dup(1.f), s), dup(1.f)));
 }
 // exp(x) for x <= 20: 2^(x log2 e) with the product's rounding error carried along
-MM_DEV float exp_of(float x) {
-  const float y = x * kLog2e;
-  const float rest = fmaf(x, 1.925963033e-8f, fmaf(x, kLog2e, -y));  // the second word of log2 e
-  const float e = ex2(y);
-  return fmaf(e, rest * kLn2, e);
+MM_DEV f2_t exp_of(f2_t x) {
+  const f2_t y = f2_mul(x, dup(kLog2e));
+  const f2_t rest = f2_fma(x, dup(1.925963033e-8f), f2_fma(x, dup(kLog2e), f2_mul(y, dup(-1.f))));  // log2 e's second word
+  const f2_t e = ex2_pair(y);
+  return f2_fma(e, f2_mul(rest, dup(kLn2)), e);
 }
-// softplus with the forward's cutoff at 20, without a branch (eight of them run side by side). log(1 + e): below
+MM_DEV f2_t below20(f2_t x) {
+  const float2 v = f2_unpack(x);
+  return f2_pack(fminf(v.x, 20.f), fminf(v.y, 20.f));
+}
+// softplus with the forward's cutoff at 20, without a branch (several run side by side). log(1 + e): below
 // e = 0.4 as 2 artanh(e / (2 + e)), whose series keeps the relative accuracy of small steps (truncated below
 // 1e-7); above, where the result is no longer small against 1, as lg2(1 + e).
-MM_DEV float step_of(float raw, int softplus) {
-  const float e = exp_of(fminf(raw, 20.f));
-  const float s = e * rcp(2.f + e), z = s * s;
-  const float small = s * fmaf(z, fmaf(z, fmaf(z, 0.285714286f, 0.4f), 0.666666667f), 2.f);
-  const float r = e < 0.4f ? small : lg2(1.f + e) * kLn2;
-  return softplus && raw <= 20.f ? r : raw;
+MM_DEV f2_t step_of(f2_t raw, int softplus) {
+  const f2_t e = exp_of(below20(raw));
+  const f2_t s = f2_mul(e, rcp_pair(f2_add(e, dup(2.f)))), z = f2_mul(s, s);
+  const f2_t small =
+      f2_mul(s, f2_fma(z, f2_fma(z, f2_fma(z, dup(0.285714286f), dup(0.4f)), dup(0.666666667f)), dup(2.f)));
+  const float2 w = f2_unpack(f2_add(e, dup(1.f)));
+  const float2 large = f2_unpack(f2_mul(f2_pack(lg2(w.x), lg2(w.y)), dup(kLn2)));
+  const float2 ev = f2_unpack(e), sv = f2_unpack(small), rv = f2_unpack(raw);
+  return f2_pack(softplus && rv.x <= 20.f ? (ev.x < 0.4f ? sv.x : large.x) : rv.x,
+                 softplus && rv.y <= 20.f ? (ev.y < 0.4f ? sv.y : large.y) : rv.y);
 }
-MM_DEV float step_slope(float raw, int softplus) {
-  const float e = exp_of(fminf(raw, 20.f));
-  return softplus && raw <= 20.f ? e * rcp(1.f + e) : 1.f;
+MM_DEV f2_t step_slope(f2_t raw, int softplus) {
+  const f2_t e = exp_of(below20(raw));
+  const float2 v = f2_unpack(f2_mul(e, rcp_pair(f2_add(e, dup(1.f))))), rv = f2_unpack(raw);
+  return f2_pack(softplus && rv.x <= 20.f ? v.x : 1.f, softplus && rv.y <= 20.f ? v.y : 1.f);
 }
 
 // Eight consecutive steps of one channel; n of them exist
@@ -119,8 +138,8 @@ template <int CH> MM_DEV void unit_of(int i, int by_channel, int& ch, int& seg) 
     ch = i % CH;
     seg = i / CH;
   } else {
-    seg = i % (kT / kK);
-    ch = i / (kT / kK);
+    seg = i % (kSegs);
+    ch = i / (kSegs);
   }
 }
 
@@ -140,20 +159,23 @@ template <typename T, bool HAS_Z> MM_DEV void load_unit(const Params& p, int b, 
 template <bool HAS_Z>
 MM_DEV void stage_unit(const Params& p, int d, int t, const Raw& r, float (&dt)[kK], float (&dtu)[kK], float (&e)[kK]) {
   const int n = min(kK, p.seqlen - t);
-  const float bias = p.bias ? p.bias[d] : 0.f;
+  const f2_t bias = dup(p.bias ? p.bias[d] : 0.f);
 #pragma unroll
-  for (int k = 0; k < kK; ++k) {
-    dt[k] = k < n ? step_of(r.dt[k] + bias, p.softplus) : 0.f;
-    dtu[k] = dt[k] * r.u[k];
-    e[k] = HAS_Z ? r.e[k] * gate_of(r.g[k]).silu : r.e[k];
+  for (int k = 0; k < kK; k += 2) {
+    const float2 x = f2_unpack(step_of(f2_add(f2_pack(r.dt[k], r.dt[k + 1]), bias), p.softplus));
+    dt[k] = k < n ? x.x : 0.f;
+    dt[k + 1] = k + 1 < n ? x.y : 0.f;
+    const float2 y = f2_unpack(f2_mul(f2_pack(dt[k], dt[k + 1]), f2_pack(r.u[k], r.u[k + 1])));
+    dtu[k] = y.x;
+    dtu[k + 1] = y.y;
+    f2_t g = f2_pack(r.e[k], r.e[k + 1]);
+    if (HAS_Z) g = f2_mul(g, silu_of(f2_pack(r.g[k], r.g[k + 1])));
+    const float2 w = f2_unpack(g);
+    e[k] = w.x;
+    e[k + 1] = w.y;
   }
 }
 
-MM_DEV f2_t ex2_pair(f2_t x) {
-  const float2 v = f2_unpack(x);
-  return f2_pack(ex2(v.x), ex2(v.y));
-}
-MM_DEV f2_t dup(float x) { return f2_pack(x, x); }
 #ifdef V_DUP
 MM_DEV f2_t mul1(f2_t a, float x) { return f2_mul(a, dup(x)); }
 MM_DEV f2_t fma1(f2_t a, float x, f2_t c) { return f2_fma(a, dup(x), c); }
@@ -199,7 +221,7 @@ __global__ void __launch_bounds__(kCarryThreads) carry_kernel(const Params p) {
   const int d0 = (int)(blockIdx.x % dtiles) * kCh;
   const long long bc = blockIdx.x / dtiles;
   const int c = (int)(bc % p.chunks), b = (int)(bc / p.chunks), t0 = c * kT;
-  for (int i = threadIdx.x; i < kCh * kT / kK; i += kCarryThreads) {
+  for (int i = threadIdx.x; i < kCh * kSegs; i += kCarryThreads) {
     int ch, seg;
     unit_of<kCh>(i, p.by_channel, ch, seg);
     float dt[kK], dtu[kK], e[kK];
@@ -295,66 +317,21 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
 // runs its steps from zero, a scan over the eight segments gives its true start, and a second run the values;
 // the same backwards. B, C and the sums for dB and dC stay in registers over all channels, so the sum over
 // channels costs nothing but the final one over warps; sums over states go across the four quads.
-#ifndef V_GCH
-#define V_GCH 32
-#endif
-#ifndef V_OCC
-#define V_OCC 2
-#endif
-constexpr int kGCh = V_GCH;      // channels staged at a time
-constexpr int kGradWarps = 4;
-constexpr int kGradThreads = kGradWarps * 32;
-constexpr int kGradSmem = 5 * kGCh * kPitch * (int)sizeof(float);  // and the raw buffers
-static_assert(kGradThreads == kGCh * kNB / 4, "a thread per channel and four states");
-
-// The raw tile of one array in shared memory, [channel][step] or, contiguous along channels, [step][channel]
-constexpr int kRawOne = kGCh * kT;
-constexpr int kRaw = 4 * kRawOne;
-
-MM_DEV void cp_async16_part(void* dst, const void* src, int bytes) {  // zeros after the first `bytes`
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
-}
-// Starts copying a tile's raw inputs; one commit group. Channels and steps that do not exist arrive as zeros.
-template <typename T>
-MM_DEV void copy_one(const void* base, const long long (&st)[3], const Params& p, int b, int t0, int d0, T* raw) {
-  const T* x = static_cast<const T*>(base) + b * st[0] + d0 * st[1] + t0 * st[2];
-  constexpr int per = 16 / (int)sizeof(T);
-  const int width = min(p.width, p.dim - d0), steps = min(kT, p.seqlen - t0);
-#pragma unroll
-  for (int i = threadIdx.x; i < kRawOne / per; i += kGradThreads) {
-    const int row = p.by_channel ? i / (kGCh / per) : i / (kT / per);
-    const int col = (p.by_channel ? i % (kGCh / per) : i % (kT / per)) * per;
-    const int n = p.by_channel ? (row < steps ? width - col : 0) : (row < width ? steps - col : 0);
-    const T* src = n > 0 ? x + row * (p.by_channel ? st[2] : st[1]) + col : x;
-    cp_async16_part(raw + i * per, src, min(max(n, 0), per) * (int)sizeof(T));
-  }
-}
-template <typename T, bool HAS_Z> MM_DEV void copy_ahead(const Params& p, int b, int t0, int d0, T* raw) {
-  if (d0 < p.dim) {
-    copy_one(p.delta, p.ds, p, b, t0, d0, raw);
-    copy_one(p.u, p.us, p, b, t0, d0, raw + kRawOne);
-    copy_one(p.dy, p.ys, p, b, t0, d0, raw + 2 * kRawOne);
-    if (HAS_Z) copy_one(p.z, p.zs, p, b, t0, d0, raw + 3 * kRawOne);
-  }
-  cp_async_commit();
-}
-template <typename T, bool HAS_Z>
-MM_DEV void load_unit(const Params& p, int b, int d, int t, Raw& r, const T* raw, int ch, int seg) {
-  if (!p.ahead) {
-    load_unit<T, HAS_Z>(p, b, d, t, r);
-    return;
-  }
-  const T* x = raw + (p.by_channel ? seg * kK * kGCh + ch : ch * kT + seg * kK);
-  const int st = p.by_channel ? kGCh : 1;
-  load_steps(x, st, !p.by_channel, kK, r.dt);
-  load_steps(x + kRawOne, st, !p.by_channel, kK, r.u);
-  load_steps(x + 2 * kRawOne, st, !p.by_channel, kK, r.e);
-  if (HAS_Z) load_steps(x + 3 * kRawOne, st, !p.by_channel, kK, r.g);
-}
 
 // Position of step t in a staged row: quarter rows of every segment lie side by side, so that the eight
 // segments' 16-byte reads fall into different banks.
-MM_DEV int at_step(int seg, int half) { return (half * (kT / kK) + seg) * 4; }
+MM_DEV int at_step(int seg, int half) { return (half * kSegs + seg) * 4; }
+MM_DEV void fetch_half(const float* row, int seg, int half, float (&v)[4]) {
+  const float4 x = *reinterpret_cast<const float4*>(row + at_step(seg, half));
+  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+}
+MM_DEV void fetch_steps(const float* row, int seg, float (&v)[kK]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float4 x = *reinterpret_cast<const float4*>(row + at_step(seg, h));
+    v[4 * h] = x.x, v[4 * h + 1] = x.y, v[4 * h + 2] = x.z, v[4 * h + 3] = x.w;
+  }
+}
 
 MM_DEV f2_t shfl_up2(f2_t v, int by) {
   const float2 x = f2_unpack(v);
@@ -365,308 +342,476 @@ MM_DEV f2_t shfl_down2(f2_t v, int by) {
   return f2_pack(__shfl_down_sync(0xffffffffu, x.x, by), __shfl_down_sync(0xffffffffu, x.y, by));
 }
 
-// Sums v[0..7] over the four quads; quad q is left with the sums of steps 4 (q & 1) + 2 (q >> 1) + {0, 1}
-MM_DEV float2 sum_quads(const float (&v)[kK], int q) {
-  float w[4];
+// A staged channel's record: rows of d, d u, e; A, the incoming state and k of 16 states; rows of the sums over
+// states sum_n g B, A w, C h. The pitch puts neighbouring channels' 16-byte words into different banks.
+struct Once {  // all states in one pass: sums replace what the same warp has read
+  static constexpr int d = 0, du = kPitch, e = 2 * kPitch, s1 = du, s2 = 3 * kPitch, s3 = 4 * kPitch, in = s2, size = 5 * kPitch;
+};
+struct Passes {
+  static constexpr int d = 0, du = kPitch, e = 2 * kPitch, s1 = 3 * kPitch, s2 = 4 * kPitch, s3 = 5 * kPitch, in = 6 * kPitch,
+                       size = 6 * kPitch + 3 * kNB + 4;
+};
+static_assert(2 * kPitch >= 3 * kNB && Once::size / 4 % 2 == 1 && Passes::size / 4 % 2 == 1, "the records' layout");
+
+// One channel of a chunk, by one warp: lane = 8 * segment + pair. The sums go to the channel's record (added to
+// what is there if `more`), dA's partial sum to pA. temp: this warp's.
+constexpr int kTempRow = 7;  // 16-byte words of a lane: six, and one for the banks' sake
+constexpr int kTemp = 32 * kTempRow;
+
+template <typename R, bool HAS_Z>
+MM_DEV void work_channel(int lane, float* rec, bool more, float4* temp, const f2_t (&Bv)[kK], const f2_t (&Cv)[kK],
+                         f2_t (&accB)[kK], f2_t (&accC)[kK], float* pA, int np) {
+  const int q = lane & 7, s = lane >> 3;
+  const float *sd = rec + R::d, *sdu = rec + R::du, *se = rec + R::e;
+  const f2_t* in2 = reinterpret_cast<const f2_t*>(rec + R::in);
+  const f2_t A2 = f2_mul(in2[q], dup(kLog2e)), first = in2[kNB / 2 + q], last = in2[kNB + q];
+  float4* mine = temp + lane * kTempRow;
+  f2_t a[kK], ah[kK], P, Q, h, k;
+  {
+    float dt[kK], dtu[kK], e[kK];
+    fetch_steps(sd, s, dt);
+    fetch_steps(sdu, s, dtu);
+    fetch_steps(se, s, e);
+    float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float keep = (q & 1) ? v[4 + i] : v[i], give = (q & 1) ? v[i] : v[4 + i];
-    w[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+    for (int i = 0; i < kK; ++i) sum += dt[i];
+    const f2_t span = ex2_pair(mul1(A2, sum));
+    // The first segment has its true start, and nothing comes into it: its span counts as 0, which also makes
+    // what the shuffles give lanes that have no partner count for nothing
+    P = s == 0 ? dup(0.f) : span;
+    Q = s == kSegs - 1 ? dup(0.f) : span;
+    h = s == 0 ? first : dup(0.f);
+    k = s == kSegs - 1 ? last : dup(0.f);
+    // both directions from zero (neither needs the other), then across segments
+#pragma unroll
+    for (int i = 0; i < kK; ++i) a[i] = ex2_pair(mul1(A2, dt[i]));
+#pragma unroll
+    for (int i = 0; i < kK; ++i) {
+      h = f2_fma(a[i], h, mul1(Bv[i], dtu[i]));
+      k = f2_mul(a[kK - 1 - i], fma1(Cv[kK - 1 - i], e[kK - 1 - i], k));
+    }
   }
-  float2 r;
-  {
-    const float keep = (q & 2) ? w[2] : w[0], give = (q & 2) ? w[0] : w[2];
-    r.x = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+#pragma unroll
+  for (int by = 1; by < kSegs; by *= 2) {
+    h = f2_fma(P, shfl_up2(h, 8 * by), h);
+    k = f2_fma(Q, shfl_down2(k, 8 * by), k);
+    if (by < kSegs / 2) {
+      P = f2_mul(P, shfl_up2(P, 8 * by));
+      Q = f2_mul(Q, shfl_down2(Q, 8 * by));
+    }
   }
   {
-    const float keep = (q & 2) ? w[3] : w[1], give = (q & 2) ? w[1] : w[3];
-    r.y = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+    const f2_t hb = shfl_up2(h, 8), kb = shfl_down2(k, 8);
+    h = s == 0 ? first : hb;
+    k = s == kSegs - 1 ? last : kb;
+  }
+  {
+    float dtu[kK], e[kK], v[kK];
+    fetch_steps(sdu, s, dtu);
+    fetch_steps(se, s, e);
+#pragma unroll
+    for (int i = 0; i < kK; ++i) {
+      ah[i] = f2_mul(a[i], h);
+      h = fma1(Bv[i], dtu[i], ah[i]);
+      accC[i] = fma1(h, e[i], accC[i]);
+      const float2 x = f2_unpack(f2_mul(h, Cv[i]));
+      v[i] = x.x + x.y;
+    }
+    if (HAS_Z) {
+      mine[4] = f4(v[0], v[1], v[2], v[3]);
+      mine[5] = f4(v[4], v[5], v[6], v[7]);
+    }
+  }
+  f2_t dA = dup(0.f);
+#pragma unroll
+  for (int half = 1; half >= 0; --half) {
+    float dt[4], dtu[4], e[4], v1[4], v2[4];
+    fetch_half(sd, s, half, dt);
+    fetch_half(sdu, s, half, dtu);
+    fetch_half(se, s, half, e);
+#pragma unroll
+    for (int j = 3; j >= 0; --j) {
+      const int i = 4 * half + j;
+      const f2_t g = fma1(Cv[i], e[j], k);
+      k = f2_mul(a[i], g);
+      accB[i] = fma1(g, dtu[j], accB[i]);
+      const f2_t w = f2_mul(g, ah[i]);
+      dA = fma1(w, dt[j], dA);
+      const float2 x = f2_unpack(f2_mul(g, Bv[i])), y = f2_unpack(f2_mul(w, A2));
+      v1[j] = x.x + x.y;
+      v2[j] = y.x + y.y;
+    }
+    mine[half] = f4(v1[0], v1[1], v1[2], v1[3]);
+    mine[2 + half] = f4(v2[0], v2[1], v2[2], v2[3]);
+  }
+  __syncwarp();
+  // sums over states: of a segment's eight lanes two each add sum_n g B, A w, C h, four steps each
+  if (q < (HAS_Z ? 6 : 4)) {
+    float* out = rec + (q < 2 ? R::s1 : q < 4 ? R::s2 : R::s3) + at_step(s, q & 1);
+    float4 sum = more ? *reinterpret_cast<float4*>(out) : f4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 x = temp[(8 * s + i) * kTempRow + q];
+      sum = f4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+    }
+    *reinterpret_cast<float4*>(out) = sum;
+  }
+  __syncwarp();
+  // dA over the segments: lanes are left with one state each (twice)
+  {
+    const float2 x = f2_unpack(dA);
+    const bool hi = s & 2;
+    float v = (hi ? x.y : x.x) + __shfl_xor_sync(0xffffffffu, hi ? x.x : x.y, 16);
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    const int n = 2 * q + (hi ? 1 : 0);
+    if (!(s & 1) && n < np) pA[n] = v;
+  }
+}
+
+// B and C of a lane's steps and its two states
+template <typename T>
+MM_DEV void load_BC_lane(const Params& p, int b, int n, int t, f2_t (&Bv)[kK], f2_t (&Cv)[kK]) {
+  const T* x = static_cast<const T*>(p.B) + b * p.Bs[0] + n * p.Bs[1] + t * p.Bs[2];
+  const T* y = static_cast<const T*>(p.C) + b * p.Cs[0] + n * p.Cs[1] + t * p.Cs[2];
+#pragma unroll
+  for (int i = 0; i < kK; ++i) {
+    const bool one = t + i < p.seqlen && n < p.dstate_n, two = t + i < p.seqlen && n + 1 < p.dstate_n;
+    Bv[i] = f2_pack(one ? ld_f32(x + i * p.Bs[2]) : 0.f, two ? ld_f32(x + i * p.Bs[2] + p.Bs[1]) : 0.f);
+    Cv[i] = f2_pack(one ? ld_f32(y + i * p.Cs[2]) : 0.f, two ? ld_f32(y + i * p.Cs[2] + p.Cs[1]) : 0.f);
+  }
+}
+
+// What work_channel wants of a channel besides its row: A, the incoming state and the incoming k of four states
+struct Incoming {
+  float4 A, h, k;
+};
+MM_DEV Incoming load_incoming(const Params& p, long long bc, int b, int d, int n0) {
+  Incoming r;
+  r.A = load_A(p, d, n0);
+  r.h = r.k = f4(0.f, 0.f, 0.f, 0.f);
+  if (p.chunks > 1) {
+    const long long at = (bc * p.dim + d) * p.np + n0;
+    if (n0 < p.np) {
+      r.h = *reinterpret_cast<const float4*>(p.hst + at);
+      r.k = *reinterpret_cast<const float4*>(p.kst + at);
+    }
+  } else if (p.dstate) {
+    const float* x = p.dstate + ((long long)b * p.dim + d) * p.dstate_n + n0;
+    const int m = p.dstate_n - n0;
+    r.k = f4(m > 0 ? x[0] : 0.f, m > 1 ? x[1] : 0.f, m > 2 ? x[2] : 0.f, m > 3 ? x[3] : 0.f);
   }
   return r;
 }
+MM_DEV void store_incoming(float* row, int quad, const Incoming& v) {
+  float4* x = reinterpret_cast<float4*>(row);
+  x[quad] = v.A;
+  x[kNB / 4 + quad] = v.h;
+  x[2 * kNB / 4 + quad] = v.k;
+}
+
+MM_DEV void store_unit(float* row, int seg, const float (&v)[kK]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    *reinterpret_cast<float4*>(row + at_step(seg, h)) = f4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+}
+MM_DEV void fetch_unit(const float* row, int seg, f2_t (&v)[kK / 2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(row + at_step(seg, h));
+    v[2 * h] = x.x;
+    v[2 * h + 1] = x.y;
+  }
+}
+
+// From the sums over states to the gradients of a unit's steps, and the unit's sums for dD and of ddelta
+template <typename T, typename R, bool HAS_Z>
+MM_DEV void finish_unit(const Params& p, int b, int d, int t, int seg, const Raw& r, const float* rec, float& sumD,
+                        float& sumb) {
+  const int n = min(kK, p.seqlen - t);
+  const f2_t bias = dup(p.bias ? p.bias[d] : 0.f), D = dup(p.D ? p.D[d] : 0.f);
+  f2_t e[kK / 2], gB[kK / 2], x[kK / 2], sum = dup(0.f);
+  float out[kK];
+  auto put = [&](int k, f2_t v) {
+    const float2 w = f2_unpack(v);
+    out[2 * k] = w.x;
+    out[2 * k + 1] = w.y;
+  };
+  fetch_unit(rec + R::e, seg, e);
+  fetch_unit(rec + R::s1, seg, gB);
+  fetch_unit(rec + R::d, seg, x);
+#pragma unroll
+  for (int k = 0; k < kK / 2; ++k) {
+    put(k, f2_fma(x[k], gB[k], f2_mul(D, e[k])));
+    sum = f2_fma(e[k], f2_pack(r.u[2 * k], r.u[2 * k + 1]), sum);
+  }
+  sumD = f2_unpack(sum).x + f2_unpack(sum).y;
+  store_steps(static_cast<T*>(p.du) + b * p.dus[0] + d * p.dus[1] + t * p.dus[2], p.dus[2], p.vec, n, out);
+  fetch_unit(rec + R::s2, seg, x);
+#pragma unroll
+  for (int k = 0; k < kK / 2; ++k)
+    put(k, f2_mul(f2_fma(f2_pack(r.u[2 * k], r.u[2 * k + 1]), gB[k], f2_mul(x[k], dup(kLn2))),
+                  step_slope(f2_add(f2_pack(r.dt[2 * k], r.dt[2 * k + 1]), bias), p.softplus)));
+  sumb = 0.f;
+#pragma unroll
+  for (int k = 0; k < kK; ++k) sumb += k < n ? out[k] : 0.f;
+  store_steps(static_cast<T*>(p.ddelta) + b * p.dds[0] + d * p.dds[1] + t * p.dds[2], p.dds[2], p.vec, n, out);
+  if (HAS_Z) {
+    fetch_unit(rec + R::s3, seg, x);
+#pragma unroll
+    for (int k = 0; k < kK / 2; ++k)
+      put(k, f2_mul(f2_mul(f2_pack(r.e[2 * k], r.e[2 * k + 1]), f2_fma(D, f2_pack(r.u[2 * k], r.u[2 * k + 1]), x[k])),
+                    silu_slope(f2_pack(r.g[2 * k], r.g[2 * k + 1]))));
+    store_steps(static_cast<T*>(p.dz) + b * p.dzs[0] + d * p.dzs[1] + t * p.dzs[2], p.dzs[2], p.vec, n, out);
+  }
+}
+
+// Offset of a chunk's [state][step] block in the partial sums of dB and dC
+MM_DEV long long block_of(const Params& p, int b, int group, int c, int pass) {
+  return ((((long long)b * p.groups + group) * p.chunks + c) * p.passes + pass) * kNB * kT;
+}
+// Register pair i of a lane holds, of accB or accC, its two states at its step i
+MM_DEV int lane_place(int state, int step) { return ((step % kK) * 2 + state % 2) * 32 + (step / kK) * 8 + state / 2; }
+template <bool ADD> MM_DEV void put_sums(float* at, int lane, const f2_t (&acc)[kK]) {
+#pragma unroll
+  for (int i = 0; i < kK; ++i) {
+    float2 x = f2_unpack(acc[i]);
+    float* q = at + i * 2 * 32 + lane;
+    if (ADD) {
+      x.x += q[0];
+      x.y += q[32];
+    }
+    q[0] = x.x;
+    q[32] = x.y;
+  }
+}
+
+// ---- 3a. up to 16 states ----
+// Two CTAs of four warps per SM (the registers' limit: B, C and the sums alone are 128 a thread) take (chunk, group
+// of channels) items tile by tile: one is in its elementwise parts while the other works. The raw inputs of the
+// next tile arrive by cp.async meanwhile.
+constexpr int kGradThreads = 128;
+// float32's raw inputs take twice the room, and a tile of half the channels keeps two CTAs on an SM
+template <typename T> constexpr int kTile = sizeof(T) == 4 ? 16 : 32;
+template <typename T> constexpr int kRawOne = kTile<T> * kT;  // [channel][step] or, contiguous along channels, [step][channel]
+template <typename T> constexpr int kRaw = 4 * kRawOne<T>;
+template <typename T> constexpr int kGradSmem = kTile<T> * Once::size * 4 + 2 * kRaw<T> * (int)sizeof(T) + 4 * kTemp * 16;
+
+MM_DEV void cp_async16_part(void* dst, const void* src, int bytes) {  // zeros after the first `bytes`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+// Starts copying a tile's raw inputs; one commit group. Channels and steps that do not exist arrive as zeros.
+template <typename T>
+MM_DEV void copy_one(const void* base, const long long (&st)[3], const Params& p, int b, int t0, int d0, T* raw) {
+  const T* x = static_cast<const T*>(base) + b * st[0] + d0 * st[1] + t0 * st[2];
+  constexpr int per = 16 / (int)sizeof(T), CH = kTile<T>;
+  const int width = min(CH, p.dim - d0), steps = min(kT, p.seqlen - t0);
+#pragma unroll
+  for (int j = 0; j < kRawOne<T> / per / kGradThreads; ++j) {
+    const int i = threadIdx.x + j * kGradThreads;
+    const int row = p.by_channel ? i / (CH / per) : i / (kT / per);
+    const int col = (p.by_channel ? i % (CH / per) : i % (kT / per)) * per;
+    const int n = p.by_channel ? (row < steps ? width - col : 0) : (row < width ? steps - col : 0);
+    const T* src = n > 0 ? x + row * (p.by_channel ? st[2] : st[1]) + col : x;
+    cp_async16_part(raw + i * per, src, min(max(n, 0), per) * (int)sizeof(T));
+  }
+}
+template <typename T, bool HAS_Z> MM_DEV void copy_tile(const Params& p, int b, int t0, int d0, T* raw) {
+  if (d0 < p.dim) {
+    copy_one(p.delta, p.ds, p, b, t0, d0, raw);
+    copy_one(p.u, p.us, p, b, t0, d0, raw + kRawOne<T>);
+    copy_one(p.dy, p.ys, p, b, t0, d0, raw + 2 * kRawOne<T>);
+    if (HAS_Z) copy_one(p.z, p.zs, p, b, t0, d0, raw + 3 * kRawOne<T>);
+  }
+  cp_async_commit();
+}
+template <typename T, bool HAS_Z>
+MM_DEV void load_unit(const Params& p, int b, int d, int t, Raw& r, const T* raw, int ch, int seg) {
+  if (!p.ahead) {
+    load_unit<T, HAS_Z>(p, b, d, t, r);
+    return;
+  }
+  const T* x = raw + (p.by_channel ? seg * kK * kTile<T> + ch : ch * kT + seg * kK);
+  const int st = p.by_channel ? kTile<T> : 1;
+  load_steps(x, st, !p.by_channel, kK, r.dt);
+  load_steps(x + kRawOne<T>, st, !p.by_channel, kK, r.u);
+  load_steps(x + 2 * kRawOne<T>, st, !p.by_channel, kK, r.e);
+  if (HAS_Z) load_steps(x + 3 * kRawOne<T>, st, !p.by_channel, kK, r.g);
+}
 
 template <typename T, bool HAS_Z>
+#ifndef V_OCC
+#define V_OCC 4
+#endif
 __global__ void __launch_bounds__(kGradThreads, V_OCC) grad_kernel(const Params p) {
+  constexpr int CH = kTile<T>, units = (CH * kSegs + kGradThreads - 1) / kGradThreads;
   extern __shared__ float4 smem4[];
-  float* sd = reinterpret_cast<float*>(smem4);  // [channel][step] each
-  float* sdu = sd + kGCh * kPitch;
-  float* se = sdu + kGCh * kPitch;
-  float* s2 = se + kGCh * kPitch;  // sum_n A w
-  float* s3 = s2 + kGCh * kPitch;  // sum_n C h
-  T* raw = reinterpret_cast<T*>(s3 + kGCh * kPitch);  // two buffers of the raw delta, u, dy, z
-  float* more = reinterpret_cast<float*>(raw + 2 * kRaw);
-  // sum_n g B, and rows of [A, state, k][16 states]: where one pass takes all states, in the place of the d u
-  // that the same lanes have read, and of the sums that the same warp has yet to write
-  const bool once = p.passes == 1;
-  float* s1 = once ? sdu : more;
-  float* in = once ? s2 : more + kGCh * kPitch;
-  __shared__ float sums[2][kGCh][kT / kK];  // of dD and ddelta, per segment
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane & 3, s = lane >> 2;
+  float* recs = reinterpret_cast<float*>(smem4);
+  T* raw = reinterpret_cast<T*>(recs + CH * Once::size);  // two buffers of the raw delta, u, dy, z
+  float4* temp = reinterpret_cast<float4*>(raw + 2 * kRaw<T>);
+  __shared__ float sums[2][CH][kSegs];  // of dD and ddelta, per segment
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = (int)(blockIdx.x % p.groups);
   const long long bc = blockIdx.x / p.groups;
   const int c = (int)(bc % p.chunks), b = (int)(bc / p.chunks), t0 = c * kT;
+  const int begin = group * p.tiles * p.width, end = min(p.dim, begin + p.tiles * p.width);
 
-  for (int pass = 0; pass < p.passes; ++pass) {
-    const int n0 = pass * kNB + 4 * q;
-    f2_t Bv[kK][2], Cv[kK][2], accB[kK][2], accC[kK][2];
+  if (p.ahead) copy_tile<T, HAS_Z>(p, b, t0, begin, raw);
+  f2_t Bv[kK], Cv[kK], accB[kK], accC[kK];
+  load_BC_lane<T>(p, b, 2 * (lane & 7), t0 + (lane >> 3) * kK, Bv, Cv);
 #pragma unroll
-    for (int i = 0; i < kK; ++i) {
-      const float4 x = load_BC(static_cast<const T*>(p.B), p.Bs, b, n0, t0 + s * kK + i, p);
-      const float4 y = load_BC(static_cast<const T*>(p.C), p.Cs, b, n0, t0 + s * kK + i, p);
-      Bv[i][0] = f2_pack(x.x, x.y);
-      Bv[i][1] = f2_pack(x.z, x.w);
-      Cv[i][0] = f2_pack(y.x, y.y);
-      Cv[i][1] = f2_pack(y.z, y.w);
-      accB[i][0] = accB[i][1] = accC[i][0] = accC[i][1] = dup(0.f);
-    }
-    if (pass == 0 && p.ahead) copy_ahead<T, HAS_Z>(p, b, t0, group * p.tiles * p.width, raw);
-    for (int tile = 0; tile < p.tiles; ++tile) {
-      const int d0 = (group * p.tiles + tile) * p.width;
-      const int width = min(p.width, p.dim - d0);  // channels of this tile; none past the last
-      if (width <= 0) break;
-      T* now = raw + (tile & 1) * kRaw;
-      __syncthreads();  // the tile before has been read
-      // of this pass's states, for every channel: A, the incoming state and k (one of each per thread)
-      const int jc = threadIdx.x / 4, jn = pass * kNB + 4 * (threadIdx.x % 4);
-      float4 jA = f4(0.f, 0.f, 0.f, 0.f), jh = jA, jk = jA;
-      if (jc < width) {
-        jA = load_A(p, d0 + jc, jn);
-        if (p.chunks > 1) {
-          const long long at = (bc * p.dim + d0 + jc) * p.np + jn;
-          if (jn < p.np) {
-            jh = *reinterpret_cast<const float4*>(p.hst + at);
-            jk = *reinterpret_cast<const float4*>(p.kst + at);
-          }
-        } else if (p.dstate) {
-          const float* x = p.dstate + ((long long)b * p.dim + d0 + jc) * p.dstate_n + jn;
-          const int m = p.dstate_n - jn;
-          jk = f4(m > 0 ? x[0] : 0.f, m > 1 ? x[1] : 0.f, m > 2 ? x[2] : 0.f, m > 3 ? x[3] : 0.f);
-        }
-      }
-      if (pass == 0) {
-        if (p.ahead) {
-          if (tile + 1 < p.tiles) copy_ahead<T, HAS_Z>(p, b, t0, d0 + p.width, raw + ((tile + 1) & 1) * kRaw);
-          else cp_async_commit();
-          cp_async_wait<1>();
-          __syncthreads();
-        }
-#pragma unroll
-        for (int i = threadIdx.x; i < kGCh * kT / kK; i += kGradThreads) {
-          int ch, seg;
-          unit_of<kGCh>(i, p.by_channel, ch, seg);
-          if (ch >= width) continue;
-          float dt[kK], dtu[kK], e[kK];
-          Raw r;
-          load_unit<T, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, r, now, ch, seg);
-          stage_unit<HAS_Z>(p, d0 + ch, t0 + seg * kK, r, dt, dtu, e);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int at = ch * kPitch + at_step(seg, h);
-            *reinterpret_cast<float4*>(sd + at) = f4(dt[4 * h], dt[4 * h + 1], dt[4 * h + 2], dt[4 * h + 3]);
-            *reinterpret_cast<float4*>(sdu + at) = f4(dtu[4 * h], dtu[4 * h + 1], dtu[4 * h + 2], dtu[4 * h + 3]);
-            *reinterpret_cast<float4*>(se + at) = f4(e[4 * h], e[4 * h + 1], e[4 * h + 2], e[4 * h + 3]);
-          }
-        }
-      }
-      float* j = in + jc * kPitch + 4 * (threadIdx.x % 4);
-      *reinterpret_cast<float4*>(j) = jA;
-      *reinterpret_cast<float4*>(j + kNB) = jh;
-      *reinterpret_cast<float4*>(j + 2 * kNB) = jk;
+  for (int k = 0; k < kK; ++k) accB[k] = accC[k] = dup(0.f);
+
+  for (int d0 = begin, i = 0; d0 < end; d0 += p.width, ++i) {
+    const int width = min(p.width, end - d0);
+    T* now = raw + (i & 1) * kRaw<T>;
+    Incoming x = {};
+    if (tid / 4 < width) x = load_incoming(p, bc, b, d0 + tid / 4, 4 * (tid % 4));
+    __syncthreads();  // the tile before has been read
+    if (p.ahead) {
+      copy_tile<T, HAS_Z>(p, b, t0, d0 + p.width < end ? d0 + p.width : p.dim, raw + (~i & 1) * kRaw<T>);
+      cp_async_wait<1>();
       __syncthreads();
-      for (int ch = warp; ch < width; ch += kGradWarps) {
-        const int d = d0 + ch;
-        const float4* row = reinterpret_cast<const float4*>(in + ch * kPitch);
-        const float4 xA = row[q], xh = row[kNB / 4 + q], xk = row[2 * kNB / 4 + q];
-        const f2_t A2[2] = {f2_mul(f2_pack(xA.x, xA.y), dup(kLog2e)), f2_mul(f2_pack(xA.z, xA.w), dup(kLog2e))};
-        const f2_t first[2] = {f2_pack(xh.x, xh.y), f2_pack(xh.z, xh.w)}, last[2] = {f2_pack(xk.x, xk.y), f2_pack(xk.z, xk.w)};
-        float dt[kK], dtu[kK], e[kK];
+    }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int at = ch * kPitch + at_step(s, h);
-          const float4 x = *reinterpret_cast<const float4*>(sd + at);
-          const float4 y = *reinterpret_cast<const float4*>(sdu + at);
-          const float4 w = *reinterpret_cast<const float4*>(se + at);
-          dt[4 * h] = x.x, dt[4 * h + 1] = x.y, dt[4 * h + 2] = x.z, dt[4 * h + 3] = x.w;
-          dtu[4 * h] = y.x, dtu[4 * h + 1] = y.y, dtu[4 * h + 2] = y.z, dtu[4 * h + 3] = y.w;
-          e[4 * h] = w.x, e[4 * h + 1] = w.y, e[4 * h + 2] = w.z, e[4 * h + 3] = w.w;
-        }
-        float sum = 0.f;
+    for (int j = 0; j < units; ++j) {
+      int ch, seg;
+      unit_of<CH>(tid + j * kGradThreads, p.by_channel, ch, seg);
+      if (ch >= width || seg >= kSegs) continue;
+      Raw r;
+      float dt[kK], dtu[kK], e[kK];
+      load_unit<T, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, r, now, ch, seg);
+      stage_unit<HAS_Z>(p, d0 + ch, t0 + seg * kK, r, dt, dtu, e);
+      float* rec = recs + ch * Once::size;
+      store_unit(rec + Once::d, seg, dt);
+      store_unit(rec + Once::du, seg, dtu);
+      store_unit(rec + Once::e, seg, e);
+    }
+    if (tid / 4 < CH) store_incoming(recs + tid / 4 * Once::size + Once::in, tid % 4, x);
+    __syncthreads();
+    for (int ch = warp; ch < width; ch += kGradThreads / 32)
+      work_channel<Once, HAS_Z>(lane, recs + ch * Once::size, false, temp + warp * kTemp, Bv, Cv, accB, accC,
+                                p.pA + (bc * p.dim + d0 + ch) * p.np, p.np);
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kK; ++i) sum += dt[i];
-        f2_t a[kK][2], ah[kK][2], P[2], Q[2], h[2];
+    for (int j = 0; j < units; ++j) {
+      int ch, seg;
+      unit_of<CH>(tid + j * kGradThreads, p.by_channel, ch, seg);
+      if (ch >= width || seg >= kSegs) continue;
+      Raw r;
+      load_unit<T, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, r, now, ch, seg);
+      finish_unit<T, Once, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, seg, r, recs + ch * Once::size, sums[0][ch][seg],
+                                  sums[1][ch][seg]);
+    }
+    __syncthreads();
+    if (tid < 2 * width) {
+      float v = 0.f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          Q[j] = P[j] = ex2_pair(mul1(A2[j], sum));
-          h[j] = s == 0 ? first[j] : dup(0.f);
-        }
-        // both directions from zero (neither needs the other), then across segments
-        f2_t k[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) k[j] = s == 7 ? last[j] : dup(0.f);
-#pragma unroll
-        for (int i = 0; i < kK; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) a[i][j] = ex2_pair(mul1(A2[j], dt[i]));
-#pragma unroll
-        for (int i = 0; i < kK; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            h[j] = f2_fma(a[i][j], h[j], mul1(Bv[i][j], dtu[i]));
-            k[j] = f2_mul(a[kK - 1 - i][j], fma1(Cv[kK - 1 - i][j], e[kK - 1 - i], k[j]));
-          }
-#pragma unroll
-        for (int by = 1; by < 8; by *= 2)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const f2_t hb = shfl_up2(h[j], 4 * by), kb = shfl_down2(k[j], 4 * by);
-            const f2_t Pb = shfl_up2(P[j], 4 * by), Qb = shfl_down2(Q[j], 4 * by);
-            if (s >= by) {
-              h[j] = f2_fma(P[j], hb, h[j]);
-              P[j] = f2_mul(P[j], Pb);
-            }
-            if (s + by < 8) {
-              k[j] = f2_fma(Q[j], kb, k[j]);
-              Q[j] = f2_mul(Q[j], Qb);
-            }
-          }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const f2_t hb = shfl_up2(h[j], 4), kb = shfl_down2(k[j], 4);
-          h[j] = s == 0 ? first[j] : hb;
-          k[j] = s == 7 ? last[j] : kb;
-        }
-        float v3[kK];
-#pragma unroll
-        for (int i = 0; i < kK; ++i) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            ah[i][j] = f2_mul(a[i][j], h[j]);
-            h[j] = fma1(Bv[i][j], dtu[i], ah[i][j]);
-            accC[i][j] = fma1(h[j], e[i], accC[i][j]);
-          }
-          if (HAS_Z) {
-            const float2 x = f2_unpack(f2_fma(h[0], Cv[i][0], f2_mul(h[1], Cv[i][1])));
-            v3[i] = x.x + x.y;
-          }
-        }
-        float v1[kK], v2[kK];
-        f2_t dA[2] = {dup(0.f), dup(0.f)};
-#pragma unroll
-        for (int i = kK - 1; i >= 0; --i) {
-          f2_t gB = dup(0.f), wA = dup(0.f);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const f2_t g = fma1(Cv[i][j], e[i], k[j]);
-            k[j] = f2_mul(a[i][j], g);
-            accB[i][j] = fma1(g, dtu[i], accB[i][j]);
-            gB = f2_fma(g, Bv[i][j], gB);
-            const f2_t w = f2_mul(g, ah[i][j]);
-            wA = f2_fma(w, A2[j], wA);
-            dA[j] = fma1(w, dt[i], dA[j]);
-          }
-          const float2 x = f2_unpack(gB), y = f2_unpack(wA);
-          v1[i] = x.x + x.y;
-          v2[i] = y.x + y.y;
-        }
-        // sums over states, for the two steps that this quad keeps
-        const int at = ch * kPitch + at_step(s, q & 1) + 2 * (q >> 1);
-        float2 r1 = sum_quads(v1, q), r2 = sum_quads(v2, q), r3 = make_float2(0.f, 0.f);
-        if (HAS_Z) r3 = sum_quads(v3, q);
-        if (pass > 0) {
-          const float2 x = *reinterpret_cast<float2*>(s1 + at), y = *reinterpret_cast<float2*>(s2 + at);
-          r1 = make_float2(r1.x + x.x, r1.y + x.y);
-          r2 = make_float2(r2.x + y.x, r2.y + y.y);
-          if (HAS_Z) {
-            const float2 w = *reinterpret_cast<float2*>(s3 + at);
-            r3 = make_float2(r3.x + w.x, r3.y + w.y);
-          }
-        }
-        *reinterpret_cast<float2*>(s1 + at) = r1;
-        *reinterpret_cast<float2*>(s2 + at) = r2;
-        if (HAS_Z) *reinterpret_cast<float2*>(s3 + at) = r3;
-        // dA over the segments: lanes are left with one state each (twice)
-        {
-          const float2 x = f2_unpack(dA[0]), y = f2_unpack(dA[1]);
-          const bool hi = s & 4, mid = s & 2;
-          const float k0 = hi ? y.x : x.x, k1 = hi ? y.y : x.y, g0 = hi ? x.x : y.x, g1 = hi ? x.y : y.y;
-          const float m0 = k0 + __shfl_xor_sync(0xffffffffu, g0, 16), m1 = k1 + __shfl_xor_sync(0xffffffffu, g1, 16);
-          float v = (mid ? m1 : m0) + __shfl_xor_sync(0xffffffffu, mid ? m0 : m1, 8);
-          v += __shfl_xor_sync(0xffffffffu, v, 4);
-          const int n = n0 + (hi ? 2 : 0) + (mid ? 1 : 0);
-          if (!(s & 1) && n < p.np) p.pA[(bc * p.dim + d) * p.np + n] = v;
-        }
-      }
-      if (pass == p.passes - 1) {
-        __syncthreads();
-#pragma unroll
-        for (int i = threadIdx.x; i < kGCh * kT / kK; i += kGradThreads) {
-          int ch, seg;
-          unit_of<kGCh>(i, p.by_channel, ch, seg);
-          if (ch >= width) continue;
-          const int d = d0 + ch, t = t0 + seg * kK, n = min(kK, p.seqlen - t);
-          Raw r;
-          load_unit<T, HAS_Z>(p, b, d, t, r, now, ch, seg);
-          const float bias = p.bias ? p.bias[d] : 0.f, D = p.D ? p.D[d] : 0.f;
-          float du[kK], dd[kK], sumD = 0.f, sumb = 0.f;
-#pragma unroll
-          for (int k = 0; k < kK; ++k) {
-            const int at = ch * kPitch + at_step(seg, k >> 2) + (k & 3);
-            const float e = se[at], gB = s1[at];
-            du[k] = fmaf(sd[at], gB, D * e);
-            dd[k] = fmaf(r.u[k], gB, s2[at] * kLn2) * step_slope(r.dt[k] + bias, p.softplus);
-            sumD = fmaf(e, r.u[k], sumD);
-            sumb += k < n ? dd[k] : 0.f;
-            if (HAS_Z) r.g[k] = r.e[k] * fmaf(D, r.u[k], s3[at]) * gate_of(r.g[k]).slope;
-          }
-          store_steps(static_cast<T*>(p.du) + b * p.dus[0] + d * p.dus[1] + t * p.dus[2], p.dus[2], p.vec, n, du);
-          store_steps(static_cast<T*>(p.ddelta) + b * p.dds[0] + d * p.dds[1] + t * p.dds[2], p.dds[2], p.vec, n, dd);
-          if (HAS_Z)
-            store_steps(static_cast<T*>(p.dz) + b * p.dzs[0] + d * p.dzs[1] + t * p.dzs[2], p.dzs[2], p.vec, n, r.g);
-          sums[0][ch][seg] = sumD;
-          sums[1][ch][seg] = sumb;
-        }
-        __syncthreads();
-        for (int ch = threadIdx.x; ch < width; ch += kGradThreads) {
-          float x = 0.f, y = 0.f;
-#pragma unroll
-          for (int seg = 0; seg < kT / kK; ++seg) {
-            x += sums[0][ch][seg];
-            y += sums[1][ch][seg];
-          }
-          p.pD[bc * p.dim + d0 + ch] = x;
-          p.pbias[bc * p.dim + d0 + ch] = y;
-        }
+      for (int seg = 0; seg < kSegs; ++seg) v += sums[tid & 1][tid >> 1][seg];
+      ((tid & 1) ? p.pbias : p.pD)[bc * p.dim + d0 + (tid >> 1)] = v;
+    }
+  }
+  // dB and dC of this group's channels: the warps' sums, in order
+  float* all = reinterpret_cast<float*>(temp);  // [B or C][lane place]
+  static_assert(2 * kNB * kT * 4 <= 4 * kTemp * 16, "the sums fit");
+  for (int k = 0; k < kGradThreads / 32; ++k) {
+    if (k == warp) {
+      if (k == 0) {
+        put_sums<false>(all, lane, accB);
+        put_sums<false>(all + kNB * kT, lane, accC);
+      } else {
+        put_sums<true>(all, lane, accB);
+        put_sums<true>(all + kNB * kT, lane, accC);
       }
     }
-    // dB and dC of this group's channels: the warps' sums, in order, as [state][step]
     __syncthreads();
-    float* all = sd;  // [warp][B or C][state][step]; the staged rows that a later pass reads are restored below
-    static_assert(kGradWarps * 2 * kNB * kT <= (5 * kGCh * kPitch), "the warps' sums fit the free rows");
-    all = once ? sd : more + 2 * kGCh * kPitch;
+  }
+  const long long out = block_of(p, b, group, c, 0);
+  for (int k = tid; k < kNB * kT; k += kGradThreads) {
+    const int place = lane_place(k / kT, k % kT);
+    p.pB[out + k] = all[place];
+    p.pC[out + k] = all[kNB * kT + place];
+  }
+}
+
+// ---- 3b. more than 16 states ----
+// The same in passes of 16 states over one staged tile of channels per CTA; every warp does all of it.
+constexpr int kWideThreads = 128;
+constexpr int kWideCh = 32;
+constexpr int kWideSmem = kWideCh * Passes::size * 4 + 4 * kTemp * 16 + 4 * 2 * kNB * kT * 4;
+
+template <typename T, bool HAS_Z>
+__global__ void __launch_bounds__(kWideThreads, 1) grad_wide_kernel(const Params p) {
+  extern __shared__ float4 smem4[];
+  float* recs = reinterpret_cast<float*>(smem4);
+  float4* temp = reinterpret_cast<float4*>(recs + kWideCh * Passes::size);
+  float* all = reinterpret_cast<float*>(temp + 4 * kTemp);  // [warp][B or C][lane place]
+  __shared__ float sums[2][kWideCh][kSegs];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int group = (int)(blockIdx.x % p.groups);
+  const long long bc = blockIdx.x / p.groups;
+  const int c = (int)(bc % p.chunks), b = (int)(bc / p.chunks), t0 = c * kT;
+  const int d0 = group * p.width, width = min(p.width, p.dim - d0);
+  for (int k = tid; k < kWideCh * kSegs; k += kWideThreads) {
+    int ch, seg;
+    unit_of<kWideCh>(k, p.by_channel, ch, seg);
+    if (ch >= width) continue;
+    Raw r;
+    float dt[kK], dtu[kK], e[kK];
+    load_unit<T, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, r);
+    stage_unit<HAS_Z>(p, d0 + ch, t0 + seg * kK, r, dt, dtu, e);
+    float* rec = recs + ch * Passes::size;
+    store_unit(rec + Passes::d, seg, dt);
+    store_unit(rec + Passes::du, seg, dtu);
+    store_unit(rec + Passes::e, seg, e);
+  }
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const int n0 = pass * kNB;
+    f2_t Bv[kK], Cv[kK], accB[kK], accC[kK];
+    load_BC_lane<T>(p, b, n0 + 2 * (lane & 7), t0 + (lane >> 3) * kK, Bv, Cv);
+#pragma unroll
+    for (int k = 0; k < kK; ++k) accB[k] = accC[k] = dup(0.f);
+    if (tid / 4 < width)
+      store_incoming(recs + tid / 4 * Passes::size + Passes::in, tid % 4, load_incoming(p, bc, b, d0 + tid / 4, n0 + 4 * (tid % 4)));
+    __syncthreads();
+    for (int ch = warp; ch < width; ch += 4)
+      work_channel<Passes, HAS_Z>(lane, recs + ch * Passes::size, pass > 0, temp + warp * kTemp, Bv, Cv, accB, accC,
+                                  p.pA + (bc * p.dim + d0 + ch) * p.np + n0, p.np - n0);
     float* mine = all + warp * 2 * kNB * kT;
-#pragma unroll
-    for (int i = 0; i < kK; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float2 x = f2_unpack(accB[i][j]), y = f2_unpack(accC[i][j]);
-        const int at = (4 * q + 2 * j) * kT + s * kK + i;
-        mine[at] = x.x;
-        mine[at + kT] = x.y;
-        mine[kNB * kT + at] = y.x;
-        mine[kNB * kT + at + kT] = y.y;
-      }
+    put_sums<false>(mine, lane, accB);
+    put_sums<false>(mine + kNB * kT, lane, accC);
     __syncthreads();
-    const long long out = ((((long long)b * p.groups + group) * p.chunks + c) * p.passes + pass) * kNB * kT;
-    for (int i = threadIdx.x; i < kNB * kT; i += kGradThreads) {
+    const long long out = block_of(p, b, group, c, pass);
+    for (int k = tid; k < kNB * kT; k += kWideThreads) {
+      const int place = lane_place(k / kT, k % kT);
       float x = 0.f, y = 0.f;
 #pragma unroll
-      for (int w = 0; w < kGradWarps; ++w) {
-        x += all[w * 2 * kNB * kT + i];
-        y += all[w * 2 * kNB * kT + kNB * kT + i];
+      for (int v = 0; v < 4; ++v) {
+        x += all[v * 2 * kNB * kT + place];
+        y += all[v * 2 * kNB * kT + kNB * kT + place];
       }
-      p.pB[out + i] = x;
-      p.pC[out + i] = y;
+      p.pB[out + k] = x;
+      p.pC[out + k] = y;
     }
+  }
+  for (int k = tid; k < kWideCh * kSegs; k += kWideThreads) {
+    int ch, seg;
+    unit_of<kWideCh>(k, p.by_channel, ch, seg);
+    if (ch >= width) continue;
+    Raw r;
+    load_unit<T, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, r);
+    finish_unit<T, Passes, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, seg, r, recs + ch * Passes::size, sums[0][ch][seg],
+                                  sums[1][ch][seg]);
+  }
+  __syncthreads();
+  if (tid < width) {
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int seg = 0; seg < kSegs; ++seg) {
+      x += sums[0][tid][seg];
+      y += sums[1][tid][seg];
+    }
+    p.pD[bc * p.dim + d0 + tid] = x;
+    p.pbias[bc * p.dim + d0 + tid] = y;
   }
 }
 
@@ -738,14 +883,13 @@ int make_layout(const MMScanBwdArgs* a, Layout* l) {
   l->chunks = (int)((f.seqlen + kT - 1) / kT);
   l->np = (int)(f.dstate + 3) / 4 * 4;
   l->passes = (int)((f.dstate + kNB - 1) / kNB);
-  // Channels of a CTA: as many as leave four CTAs to every one of the 2 x 148 places (fewer partial sums of dB
-  // and dC), in tiles of 64; down to 16 channels where there are few chunks. States above 16 keep their staged
-  // tile over the passes, so there one tile is the most.
+  // Channels of a CTA of the third kernel: as many (fewer partial sums of dB and dC) as leave every one of the
+  // 2 x 148 places four CTAs, at most 512, in tiles of 32 (16 for float32, and where 32 would leave places empty).
   const long long rows = f.batch * (l->chunks > 0 ? l->chunks : 1);
-  long long want = f.dim * rows / (4 * 2 * 148);
-  l->width = want >= kGCh ? kGCh : 16;
-  long long tiles = want / kGCh;
-  l->tiles = (int)(l->passes > 1 || tiles < 1 ? 1 : tiles > 512 / kGCh ? 512 / kGCh : tiles);
+  const long long want = f.dim * rows / (4 * 2 * 148);
+  l->width = (f.dtype == MM_F32 && l->passes == 1) || f.dim * rows < 2 * 148 * 32 ? 16 : 32;
+  const long long tiles = want / l->width;
+  l->tiles = (int)(l->passes > 1 || tiles < 1 ? 1 : tiles > 512 / l->width ? 512 / l->width : tiles);
   const long long per = (long long)l->width * l->tiles;
   l->groups = (int)((f.dim + per - 1) / per);
   size_t at = 0;
@@ -775,8 +919,6 @@ inline void copy3(long long (&to)[3], const int64_t* from) {
 template <typename T, bool HAS_Z> int launch(const Params& p, cudaStream_t s) {
   const long long rows = (long long)p.batch * p.chunks;
   const int carry_smem = 3 * kT * kCarryPitch * (int)sizeof(float);
-  const int grad_smem = kGradSmem + 2 * kRaw * (int)sizeof(T) +
-                        (p.passes > 1 ? (2 * kGCh * kPitch + kGradWarps * 2 * kNB * kT) * (int)sizeof(float) : 0);
   const long long dtiles = (p.dim + kCh - 1) / kCh;
   if (rows * dtiles > 0x7fffffffLL || rows * p.groups > 0x7fffffffLL) return MM_ERR_SHAPE;
   if (p.chunks > 1) {
@@ -789,9 +931,15 @@ template <typename T, bool HAS_Z> int launch(const Params& p, cudaStream_t s) {
     join_kernel<<<dim3((unsigned)((states + 255) / 256), 2), 256, 0, s>>>(p);
     if (cudaGetLastError() != cudaSuccess) return MM_ERR_LAUNCH;
   }
-  if (cudaFuncSetAttribute(grad_kernel<T, HAS_Z>, cudaFuncAttributeMaxDynamicSharedMemorySize, grad_smem) != cudaSuccess)
-    return MM_ERR_LAUNCH;
-  grad_kernel<T, HAS_Z><<<(unsigned)(rows * p.groups), kGradThreads, grad_smem, s>>>(p);
+  if (p.passes > 1) {
+    if (cudaFuncSetAttribute(grad_wide_kernel<T, HAS_Z>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem) != cudaSuccess)
+      return MM_ERR_LAUNCH;
+    grad_wide_kernel<T, HAS_Z><<<(unsigned)(rows * p.groups), kWideThreads, kWideSmem, s>>>(p);
+  } else {
+    if (cudaFuncSetAttribute(grad_kernel<T, HAS_Z>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGradSmem<T>) != cudaSuccess)
+      return MM_ERR_LAUNCH;
+    grad_kernel<T, HAS_Z><<<(unsigned)(rows * p.groups), kGradThreads, kGradSmem<T>, s>>>(p);
+  }
   if (cudaGetLastError() != cudaSuccess) return MM_ERR_LAUNCH;
   const long long bc = (rows * p.passes * kNB * kT + 255) / 256;
   const long long rest = ((long long)p.dim * (p.np + 2) + 31) / 32;
