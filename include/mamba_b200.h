@@ -451,14 +451,24 @@ int mm_preference_loss_fwd(const MMPreferenceArgs* args, void* workspace, size_t
                            mm_stream_t stream);
 int mm_preference_loss_bwd(const MMPreferenceArgs* args, mm_stream_t stream);
 
-/* Gradient of mm_selective_scan_fwd. `fwd` holds the forward call's inputs (its y, state_out, piece_tiles and
- * options are not read); nothing else is kept from the forward pass.
+/* mm_selective_scan_fwd for training: the same function, in kernels whose sums do not depend on timing, with
+ * softplus at full relative accuracy for small steps, and with the states that the gradient starts from:
+ * states (fp32, size from mm_selective_scan_states_size, 16-byte aligned) receives h before every 32nd step. y
+ * may be NULL: only states (and state_out) are computed. piece_tiles and options are not read. */
+int mm_selective_scan_states_size(const MMScanArgs* args, size_t* bytes);
+int mm_selective_scan_train_workspace_size(const MMScanArgs* args, size_t* bytes);
+int mm_selective_scan_train_fwd(const MMScanArgs* args, float* states, void* workspace, size_t workspace_bytes,
+                                mm_stream_t stream);
+
+/* Gradient of mm_selective_scan_train_fwd (and of mm_selective_scan_fwd). `fwd` holds the forward call's inputs
+ * (its y, state_out, piece_tiles and options are not read), `states` what the forward call left.
  *   dy: (batch, dim, seqlen) of the forward's dtype; dstate: gradient of the last state, fp32 (batch, dim, dstate)
  *   contiguous, or NULL; du, ddelta, dz alike (dz when z is given); dB, dC: (batch, dstate, seqlen) of the dtype;
  *   dA (dim, dstate), dD (dim,), ddelta_bias (dim,): fp32 contiguous; dD / ddelta_bias may be NULL.
  * All strides free. Sums are taken in a fixed order: equal calls give equal bits. */
 typedef struct MMScanBwdArgs {
   MMScanArgs fwd;
+  const float* states;
   const void* dy;
   const float* dstate; /* may be NULL */
   void* du;

@@ -136,7 +136,7 @@ class MMPreferenceArgs(ctypes.Structure):
 
 class MMScanBwdArgs(ctypes.Structure):
     _fields_ = [
-        ("fwd", MMScanArgs), ("dy", _p), ("dstate", _p), ("du", _p), ("ddelta", _p), ("dA", _p), ("dB", _p),
+        ("fwd", MMScanArgs), ("states", _p), ("dy", _p), ("dstate", _p), ("du", _p), ("ddelta", _p), ("dA", _p), ("dB", _p),
         ("dC", _p), ("dD", _p), ("dz", _p), ("ddelta_bias", _p), ("dy_stride", _i64 * 3), ("du_stride", _i64 * 3),
         ("ddelta_stride", _i64 * 3), ("dz_stride", _i64 * 3), ("dB_stride", _i64 * 3), ("dC_stride", _i64 * 3),
     ]
@@ -168,6 +168,10 @@ _SIGNATURES = {
                                           ctypes.c_int),
     "mm_preference_loss_fwd": ([ctypes.POINTER(MMPreferenceArgs), _p, ctypes.c_size_t, _p], ctypes.c_int),
     "mm_preference_loss_bwd": ([ctypes.POINTER(MMPreferenceArgs), _p], ctypes.c_int),
+    "mm_selective_scan_states_size": ([ctypes.POINTER(MMScanArgs), ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "mm_selective_scan_train_workspace_size": ([ctypes.POINTER(MMScanArgs), ctypes.POINTER(ctypes.c_size_t)],
+                                               ctypes.c_int),
+    "mm_selective_scan_train_fwd": ([ctypes.POINTER(MMScanArgs), _p, _p, ctypes.c_size_t, _p], ctypes.c_int),
     "mm_selective_scan_bwd_workspace_size": ([ctypes.POINTER(MMScanBwdArgs), ctypes.POINTER(ctypes.c_size_t)],
                                              ctypes.c_int),
     "mm_selective_scan_bwd": ([ctypes.POINTER(MMScanBwdArgs), _p, ctypes.c_size_t, _p], ctypes.c_int),

@@ -5,143 +5,17 @@
 //   g_t = C_t e_t + k_t,  k_t = a_{t+1} g_{t+1}  (k at the end: the last state's gradient)
 //   dC_t = sum_d h e     dB_t = sum_d g d u     du = d sum_n g B + D e     w = g a h_{t-1}
 //   dd = u sum_n g B + sum_n A w     dA = sum_{b,t} d w     dz = dy p silu'(z)     dD = sum e u
-// Nothing is kept from the forward pass: time is cut into chunks of 64 steps, and three kernels make the chunks
-// independent of one another:
-//   1. carry_kernel: of every chunk, the state it ends with from zero, the k it hands to the chunk before from
-//      zero, and the sum of d (the chunk's decay is exp(A sum d), so no products are kept);
-//   2. join_kernel: those in order, forwards for the states and backwards for k;
-//   3. grad_kernel: every chunk from its true incoming state and k.
+// Time is cut into chunks of 32 steps. The forward pass leaves the state that every chunk starts from; walk_back
+// (mm_scan_walk.cu) finds the k that comes into every chunk; then grad_kernel takes all chunks side by side.
 // Sums over channels and over chunks leave as partials that reduce_kernel adds in a fixed order, so the results
 // do not depend on timing. All state and all sums are float32 (the last sums over partials float64).
-#include "mm_common.cuh"
+#include "mm_scan_train.cuh"
 
 namespace mm {
-namespace bwd {
+namespace train {
 
-constexpr int kT = 32;        // steps of a chunk
-constexpr int kK = 8;         // steps of a lane
-constexpr int kSegs = kT / kK;
-constexpr int kCh = 64;       // channels staged at a time
 constexpr int kPitch = kT + 4;  // floats of a staged row; rows stay 16-byte aligned, neighbours in other banks
-constexpr int kNB = 16;       // states of a pass
-
-struct Params {
-  const void *u, *delta, *z, *B, *C, *dy;
-  const float *A, *D, *bias, *dstate;
-  void *du, *ddelta, *dz, *dB, *dC;
-  float *dA, *dD, *dbias;
-  long long us[3], ds[3], zs[3], Bs[3], Cs[3], ys[3], As[2];
-  long long dus[3], dds[3], dzs[3], dBs[3], dCs[3];
-  int batch, dim, dstate_n, seqlen;
-  int softplus;
-  int vec;        // every activation's rows are contiguous in time and 16-byte aligned
-  int by_channel; // u is contiguous along channels
-  int ahead;      // grad_kernel copies its raw inputs ahead: all contiguous along one axis, rows 16-byte aligned
-  // workspace
-  float *hst, *kst, *sum_d;  // (batch, chunks, dim, np): states and k; (batch, chunks, dim)
-  float *pB, *pC;            // (batch, groups, chunks, passes, 16, 64)
-  float *pA, *pD, *pbias;    // (batch, chunks, dim, np), (batch, chunks, dim)
-  int chunks, np, passes, groups, tiles;  // tiles of `width` channels that one CTA works off
-  int width;
-};
-
-MM_DEV float4 f4(float a, float b, float c, float d) { return make_float4(a, b, c, d); }
-
-// ---- elementwise parts, on pairs of steps -------------------------------------------------------------
-MM_DEV f2_t dup(float x) { return f2_pack(x, x); }
-MM_DEV f2_t ex2_pair(f2_t x) {
-  const float2 v = f2_unpack(x);
-  return f2_pack(ex2(v.x), ex2(v.y));
-}
-MM_DEV f2_t rcp_pair(f2_t x) {
-  const float2 v = f2_unpack(x);
-  return f2_pack(rcp(v.x), rcp(v.y));
-}
-MM_DEV f2_t sigmoid(f2_t z) { return rcp_pair(f2_add(ex2_pair(f2_mul(z, dup(-kLog2e))), dup(1.f))); }
-MM_DEV f2_t silu_of(f2_t z) { return f2_mul(z, sigmoid(z)); }
-// silu'(z) = s (1 + z (1 - s))
-MM_DEV f2_t silu_slope(f2_t z) {
-  const f2_t s = sigmoid(z);
-  return f2_mul(s, f2_fma(z, f2_sub(dup(1.f), s), dup(1.f)));
-}
-// exp(x) for x <= 20: 2^(x log2 e) with the product's rounding error carried along
-MM_DEV f2_t exp_of(f2_t x) {
-  const f2_t y = f2_mul(x, dup(kLog2e));
-  const f2_t rest = f2_fma(x, dup(1.925963033e-8f), f2_fma(x, dup(kLog2e), f2_mul(y, dup(-1.f))));  // log2 e's second word
-  const f2_t e = ex2_pair(y);
-  return f2_fma(e, f2_mul(rest, dup(kLn2)), e);
-}
-MM_DEV f2_t below20(f2_t x) {
-  const float2 v = f2_unpack(x);
-  return f2_pack(fminf(v.x, 20.f), fminf(v.y, 20.f));
-}
-// softplus with the forward's cutoff at 20, without a branch (several run side by side). log(1 + e): below
-// e = 0.4 as 2 artanh(e / (2 + e)), whose series keeps the relative accuracy of small steps (truncated below
-// 1e-7); above, where the result is no longer small against 1, as lg2(1 + e).
-MM_DEV f2_t step_of(f2_t raw, int softplus) {
-  const f2_t e = exp_of(below20(raw));
-  const f2_t s = f2_mul(e, rcp_pair(f2_add(e, dup(2.f)))), z = f2_mul(s, s);
-  const f2_t small =
-      f2_mul(s, f2_fma(z, f2_fma(z, f2_fma(z, dup(0.285714286f), dup(0.4f)), dup(0.666666667f)), dup(2.f)));
-  const float2 w = f2_unpack(f2_add(e, dup(1.f)));
-  const float2 large = f2_unpack(f2_mul(f2_pack(lg2(w.x), lg2(w.y)), dup(kLn2)));
-  const float2 ev = f2_unpack(e), sv = f2_unpack(small), rv = f2_unpack(raw);
-  return f2_pack(softplus && rv.x <= 20.f ? (ev.x < 0.4f ? sv.x : large.x) : rv.x,
-                 softplus && rv.y <= 20.f ? (ev.y < 0.4f ? sv.y : large.y) : rv.y);
-}
-MM_DEV f2_t step_slope(f2_t raw, int softplus) {
-  const f2_t e = exp_of(below20(raw));
-  const float2 v = f2_unpack(f2_mul(e, rcp_pair(f2_add(e, dup(1.f))))), rv = f2_unpack(raw);
-  return f2_pack(softplus && rv.x <= 20.f ? v.x : 1.f, softplus && rv.y <= 20.f ? v.y : 1.f);
-}
-
-// Eight consecutive steps of one channel; n of them exist
-template <typename T> MM_DEV void load_steps(const T* p, long long s, bool vec, int n, float (&v)[kK]) {
-  if (vec && n == kK) {
-#pragma unroll
-    for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
-      const uint4 a = *(reinterpret_cast<const uint4*>(p) + h);
-      constexpr int pairs = 8 / (int)sizeof(T);
-#pragma unroll
-      for (int k = 0; k < pairs; ++k) {
-        const float2 q = vec_pair<T>(a, k);
-        v[2 * (h * pairs + k)] = q.x;
-        v[2 * (h * pairs + k) + 1] = q.y;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < kK; ++k) v[k] = k < n ? ld_f32(p + k * s) : 0.f;
-  }
-}
-template <typename T> MM_DEV void store_steps(T* p, long long s, bool vec, int n, const float (&v)[kK]) {
-  if (vec && n == kK) {
-#pragma unroll
-    for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
-      uint4 a;
-      constexpr int pairs = 8 / (int)sizeof(T);
-#pragma unroll
-      for (int k = 0; k < pairs; ++k) vec_set_pair<T>(a, k, v[2 * (h * pairs + k)], v[2 * (h * pairs + k) + 1]);
-      __stcs(reinterpret_cast<uint4*>(p) + h, a);
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < kK; ++k)
-      if (k < n) st_f32(p + k * s, v[k]);
-  }
-}
-
-// Where a thread's unit (eight steps of a channel) of a staged tile lies. Lanes run along whichever of time and
-// channels is contiguous in memory.
-template <int CH> MM_DEV void unit_of(int i, int by_channel, int& ch, int& seg) {
-  if (by_channel) {
-    ch = i % CH;
-    seg = i / CH;
-  } else {
-    seg = i % (kSegs);
-    ch = i / (kSegs);
-  }
-}
+constexpr int kNB = 16;         // states of a pass
 
 // The raw values of a unit, so that several units' loads can be in flight before the first is worked on
 struct Raw {
@@ -176,155 +50,15 @@ MM_DEV void stage_unit(const Params& p, int d, int t, const Raw& r, float (&dt)[
   }
 }
 
-#ifdef V_DUP
-MM_DEV f2_t mul1(f2_t a, float x) { return f2_mul(a, dup(x)); }
-MM_DEV f2_t fma1(f2_t a, float x, f2_t c) { return f2_fma(a, dup(x), c); }
-#else
-MM_DEV f2_t mul1(f2_t a, float x) {
-  const float2 v = f2_unpack(a);
-  return f2_pack(v.x * x, v.y * x);
-}
-MM_DEV f2_t fma1(f2_t a, float x, f2_t c) {
-  const float2 v = f2_unpack(a), w = f2_unpack(c);
-  return f2_pack(fmaf(v.x, x, w.x), fmaf(v.y, x, w.y));
-}
-#endif
-
-// Four consecutive states' entries of a (dim, dstate)-shaped row; zeros past the last state
-MM_DEV float4 load_A(const Params& p, int d, int n0) {
-  const float* a = p.A + d * p.As[0] + n0 * p.As[1];
-  const int n = p.dstate_n - n0;
-  return f4(n > 0 ? a[0] : 0.f, n > 1 ? a[p.As[1]] : 0.f, n > 2 ? a[2 * p.As[1]] : 0.f, n > 3 ? a[3 * p.As[1]] : 0.f);
-}
-template <typename T>
-MM_DEV float4 load_BC(const T* base, const long long (&st)[3], int b, int n0, int t, const Params& p) {
-  const T* q = base + b * st[0] + n0 * st[1] + t * st[2];
-  const int n = t < p.seqlen ? p.dstate_n - n0 : 0;
-  return f4(n > 0 ? ld_f32(q) : 0.f, n > 1 ? ld_f32(q + st[1]) : 0.f, n > 2 ? ld_f32(q + 2 * st[1]) : 0.f,
-            n > 3 ? ld_f32(q + 3 * st[1]) : 0.f);
-}
-
-// ---- 1. what every chunk contributes -----------------------------------------------------------------
-// A CTA takes 64 channels of one chunk. Lanes are channels, warps pairs of a channel half and four states; each
-// thread walks the chunk's 64 steps: h = a h + d u B,  P = a P,  k += P C e.
-constexpr int kCarryThreads = 256;
-constexpr int kCarryPitch = kCh + 1;
-
-template <typename T, bool HAS_Z>
-__global__ void __launch_bounds__(kCarryThreads) carry_kernel(const Params p) {
-  extern __shared__ float4 smem4[];
-  float* sd = reinterpret_cast<float*>(smem4);  // [t][channel] each
-  float* sdu = sd + kT * kCarryPitch;
-  float* se = sdu + kT * kCarryPitch;
-  __shared__ float4 sB[kT][kNB / 4], sC[kT][kNB / 4];
-  const int dtiles = (p.dim + kCh - 1) / kCh;
-  const int d0 = (int)(blockIdx.x % dtiles) * kCh;
-  const long long bc = blockIdx.x / dtiles;
-  const int c = (int)(bc % p.chunks), b = (int)(bc / p.chunks), t0 = c * kT;
-  for (int i = threadIdx.x; i < kCh * kSegs; i += kCarryThreads) {
-    int ch, seg;
-    unit_of<kCh>(i, p.by_channel, ch, seg);
-    float dt[kK], dtu[kK], e[kK];
-    if (d0 + ch < p.dim) {
-      Raw r;
-      load_unit<T, HAS_Z>(p, b, d0 + ch, t0 + seg * kK, r);
-      stage_unit<HAS_Z>(p, d0 + ch, t0 + seg * kK, r, dt, dtu, e);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kK; ++k) dt[k] = dtu[k] = e[k] = 0.f;
-    }
-#pragma unroll
-    for (int k = 0; k < kK; ++k) {
-      const int at = (seg * kK + k) * kCarryPitch + ch;
-      sd[at] = dt[k];
-      sdu[at] = dtu[k];
-      se[at] = e[k];
-    }
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int ch = (warp & 1) * 32 + lane, q = warp >> 1, d = d0 + ch;
-  for (int pass = 0; pass < p.passes; ++pass) {
-    const int n0 = pass * kNB;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kT * kNB / 4; i += kCarryThreads) {
-      const int t = i % kT, j = i / kT;
-      sB[t][j] = load_BC(static_cast<const T*>(p.B), p.Bs, b, n0 + 4 * j, t0 + t, p);
-      sC[t][j] = load_BC(static_cast<const T*>(p.C), p.Cs, b, n0 + 4 * j, t0 + t, p);
-    }
-    __syncthreads();
-    if (n0 + 4 * q >= p.np || d >= p.dim) continue;
-    const float4 A = load_A(p, d, n0 + 4 * q);
-    const f2_t A0 = f2_mul(f2_pack(A.x, A.y), dup(kLog2e)), A1 = f2_mul(f2_pack(A.z, A.w), dup(kLog2e));
-    f2_t h0 = dup(0.f), h1 = h0, k0 = h0, k1 = h0, P0 = dup(1.f), P1 = P0;
-    float sum = 0.f;
-#pragma unroll 4
-    for (int t = 0; t < kT; ++t) {
-      const float dt = sd[t * kCarryPitch + ch];
-      const f2_t dd = dup(dt), du = dup(sdu[t * kCarryPitch + ch]), e = dup(se[t * kCarryPitch + ch]);
-      const float4 Bv = sB[t][q], Cv = sC[t][q];
-      const f2_t a0 = ex2_pair(f2_mul(dd, A0)), a1 = ex2_pair(f2_mul(dd, A1));
-      h0 = f2_fma(a0, h0, f2_mul(du, f2_pack(Bv.x, Bv.y)));
-      h1 = f2_fma(a1, h1, f2_mul(du, f2_pack(Bv.z, Bv.w)));
-      P0 = f2_mul(P0, a0);
-      P1 = f2_mul(P1, a1);
-      k0 = f2_fma(P0, f2_mul(e, f2_pack(Cv.x, Cv.y)), k0);
-      k1 = f2_fma(P1, f2_mul(e, f2_pack(Cv.z, Cv.w)), k1);
-      sum += dt;
-    }
-    const long long at = (bc * p.dim + d) * p.np + n0 + 4 * q;
-    const float2 x = f2_unpack(h0), y = f2_unpack(h1), v = f2_unpack(k0), w = f2_unpack(k1);
-    *reinterpret_cast<float4*>(p.hst + at) = f4(x.x, x.y, y.x, y.y);
-    *reinterpret_cast<float4*>(p.kst + at) = f4(v.x, v.y, w.x, w.y);
-    if (n0 + 4 * q == 0) p.sum_d[bc * p.dim + d] = sum;
-  }
-}
-
-// ---- 2. the chunks in order ---------------------------------------------------------------------------
-// A thread per state and direction replaces, chunk by chunk, what the chunk contributes by what comes into it.
-__global__ void __launch_bounds__(256) join_kernel(const Params p) {
-  const long long per = (long long)p.dim * p.np;
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= p.batch * per) return;
-  const long long b = i / per, dn = i % per;
-  const int d = (int)(dn / p.np), n = (int)(dn % p.np);
-  const bool back = blockIdx.y != 0;
-  const float A = n < p.dstate_n ? p.A[d * p.As[0] + n * p.As[1]] * kLog2e : 0.f;
-  float* st = (back ? p.kst : p.hst) + b * p.chunks * per + dn;
-  const float* sum = p.sum_d + b * p.chunks * p.dim + d;
-  float v = back && p.dstate && n < p.dstate_n ? p.dstate[(b * p.dim + d) * p.dstate_n + n] : 0.f;
-  constexpr int kU = 8;
-  for (int c0 = 0; c0 < p.chunks; c0 += kU) {
-    float own[kU], s[kU];
-#pragma unroll
-    for (int j = 0; j < kU; ++j) {
-      if (c0 + j >= p.chunks) break;
-      const long long c = back ? p.chunks - 1 - (c0 + j) : c0 + j;
-      own[j] = st[c * per];
-      s[j] = sum[c * p.dim];
-    }
-#pragma unroll
-    for (int j = 0; j < kU; ++j) {
-      if (c0 + j >= p.chunks) break;
-      const long long c = back ? p.chunks - 1 - (c0 + j) : c0 + j;
-      st[c * per] = v;
-      v = fmaf(ex2(s[j] * A), v, own[j]);
-    }
-  }
-}
-
-// ---- 3. the gradient of every chunk -----------------------------------------------------------------
-// A warp works off channels one by one: lane = 4 * segment + quad holds eight steps of four states. Each segment
-// runs its steps from zero, a scan over the eight segments gives its true start, and a second run the values;
+// ---- the gradient of every chunk ------------------------------------------------------------------------
+// A warp works off channels one by one: lane = 8 * segment + pair holds eight steps of two states. Each segment
+// runs its steps from zero, a scan over the four segments gives its true start, and a second run the values;
 // the same backwards. B, C and the sums for dB and dC stay in registers over all channels, so the sum over
-// channels costs nothing but the final one over warps; sums over states go across the four quads.
+// channels costs nothing but the final one over warps; sums over states go across the eight lanes of a segment.
 
-// Position of step t in a staged row: quarter rows of every segment lie side by side, so that the eight
-// segments' 16-byte reads fall into different banks.
+// Position of a segment's half in a staged row: the first halves of the segments lie side by side, so that their
+// 16-byte reads fall into different banks.
 MM_DEV int at_step(int seg, int half) { return (half * kSegs + seg) * 4; }
-MM_DEV void fetch_half(const float* row, int seg, int half, float (&v)[4]) {
-  const float4 x = *reinterpret_cast<const float4*>(row + at_step(seg, half));
-  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-}
 MM_DEV void fetch_steps(const float* row, int seg, float (&v)[kK]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -367,8 +101,8 @@ MM_DEV void work_channel(int lane, float* rec, bool more, float4* temp, const f2
   const f2_t A2 = f2_mul(in2[q], dup(kLog2e)), first = in2[kNB / 2 + q], last = in2[kNB + q];
   float4* mine = temp + lane * kTempRow;
   f2_t a[kK], ah[kK], P, Q, h, k;
+  float dt[kK], dtu[kK], e[kK];
   {
-    float dt[kK], dtu[kK], e[kK];
     fetch_steps(sd, s, dt);
     fetch_steps(sdu, s, dtu);
     fetch_steps(se, s, e);
@@ -406,9 +140,7 @@ MM_DEV void work_channel(int lane, float* rec, bool more, float4* temp, const f2
     k = s == kSegs - 1 ? last : kb;
   }
   {
-    float dtu[kK], e[kK], v[kK];
-    fetch_steps(sdu, s, dtu);
-    fetch_steps(se, s, e);
+    float v[kK];
 #pragma unroll
     for (int i = 0; i < kK; ++i) {
       ah[i] = f2_mul(a[i], h);
@@ -425,18 +157,15 @@ MM_DEV void work_channel(int lane, float* rec, bool more, float4* temp, const f2
   f2_t dA = dup(0.f);
 #pragma unroll
   for (int half = 1; half >= 0; --half) {
-    float dt[4], dtu[4], e[4], v1[4], v2[4];
-    fetch_half(sd, s, half, dt);
-    fetch_half(sdu, s, half, dtu);
-    fetch_half(se, s, half, e);
+    float v1[4], v2[4];
 #pragma unroll
     for (int j = 3; j >= 0; --j) {
       const int i = 4 * half + j;
-      const f2_t g = fma1(Cv[i], e[j], k);
+      const f2_t g = fma1(Cv[i], e[i], k);
       k = f2_mul(a[i], g);
-      accB[i] = fma1(g, dtu[j], accB[i]);
+      accB[i] = fma1(g, dtu[i], accB[i]);
       const f2_t w = f2_mul(g, ah[i]);
-      dA = fma1(w, dt[j], dA);
+      dA = fma1(w, dt[i], dA);
       const float2 x = f2_unpack(f2_mul(g, Bv[i])), y = f2_unpack(f2_mul(w, A2));
       v1[j] = x.x + x.y;
       v2[j] = y.x + y.y;
@@ -489,16 +218,23 @@ MM_DEV Incoming load_incoming(const Params& p, long long bc, int b, int d, int n
   Incoming r;
   r.A = load_A(p, d, n0);
   r.h = r.k = f4(0.f, 0.f, 0.f, 0.f);
-  if (p.chunks > 1) {
-    const long long at = (bc * p.dim + d) * p.np + n0;
+  const long long at = (bc * p.dim + d) * p.np + n0;
+  if (p.longs > 1) {
     if (n0 < p.np) {
-      r.h = *reinterpret_cast<const float4*>(p.hst + at);
-      r.k = *reinterpret_cast<const float4*>(p.kst + at);
+      const long long bl = (long long)b * p.longs + (int)(bc % p.chunks) / kLong;
+      r.k = *reinterpret_cast<const float4*>(p.klong + (bl * p.dim + d) * p.np + n0);
     }
   } else if (p.dstate) {
     const float* x = p.dstate + ((long long)b * p.dim + d) * p.dstate_n + n0;
     const int m = p.dstate_n - n0;
     r.k = f4(m > 0 ? x[0] : 0.f, m > 1 ? x[1] : 0.f, m > 2 ? x[2] : 0.f, m > 3 ? x[3] : 0.f);
+  }
+  if (p.chunks > 1 && n0 < p.np) {
+    r.h = *reinterpret_cast<const float4*>(p.hst + at);
+    const float4 x = *reinterpret_cast<const float4*>(p.kst + at);
+    const float span = p.later[bc * p.dim + d] * kLog2e;
+    r.k = f4(fmaf(ex2(span * r.A.x), r.k.x, x.x), fmaf(ex2(span * r.A.y), r.k.y, x.y), fmaf(ex2(span * r.A.z), r.k.z, x.z),
+             fmaf(ex2(span * r.A.w), r.k.w, x.w));
   }
   return r;
 }
@@ -585,12 +321,12 @@ template <bool ADD> MM_DEV void put_sums(float* at, int lane, const f2_t (&acc)[
   }
 }
 
-// ---- 3a. up to 16 states ----
-// Two CTAs of four warps per SM (the registers' limit: B, C and the sums alone are 128 a thread) take (chunk, group
-// of channels) items tile by tile: one is in its elementwise parts while the other works. The raw inputs of the
+// ---- up to 16 states ----
+// Three CTAs of four warps per SM (the registers' limit) take (chunk, group of channels) items tile by tile: some are
+// in their elementwise parts while others work. The raw inputs of the
 // next tile arrive by cp.async meanwhile.
 constexpr int kGradThreads = 128;
-// float32's raw inputs take twice the room, and a tile of half the channels keeps two CTAs on an SM
+// float32's raw inputs take twice the room, and a tile of half the channels keeps three CTAs on an SM
 template <typename T> constexpr int kTile = sizeof(T) == 4 ? 16 : 32;
 template <typename T> constexpr int kRawOne = kTile<T> * kT;  // [channel][step] or, contiguous along channels, [step][channel]
 template <typename T> constexpr int kRaw = 4 * kRawOne<T>;
@@ -639,10 +375,7 @@ MM_DEV void load_unit(const Params& p, int b, int d, int t, Raw& r, const T* raw
 }
 
 template <typename T, bool HAS_Z>
-#ifndef V_OCC
-#define V_OCC 4
-#endif
-__global__ void __launch_bounds__(kGradThreads, V_OCC) grad_kernel(const Params p) {
+__global__ void __launch_bounds__(kGradThreads, 3) grad_kernel(const Params p) {
   constexpr int CH = kTile<T>, units = (CH * kSegs + kGradThreads - 1) / kGradThreads;
   extern __shared__ float4 smem4[];
   float* recs = reinterpret_cast<float*>(smem4);
@@ -733,7 +466,7 @@ __global__ void __launch_bounds__(kGradThreads, V_OCC) grad_kernel(const Params 
   }
 }
 
-// ---- 3b. more than 16 states ----
+// ---- more than 16 states ----
 // The same in passes of 16 states over one staged tile of channels per CTA; every warp does all of it.
 constexpr int kWideThreads = 128;
 constexpr int kWideCh = 32;
@@ -870,66 +603,47 @@ template <typename T> __global__ void __launch_bounds__(256) reduce_kernel(const
 
 // ---- host ---------------------------------------------------------------------------------------------
 struct Layout {
-  int chunks, np, passes, groups, tiles, width;
-  size_t hst, kst, sum_d, pB, pC, pA, pD, pbias, bytes;
+  int passes, groups, tiles, width;
+  size_t kst, later, klong, slong, pB, pC, pA, pD, pbias, bytes;
 };
 
 int make_layout(const MMScanBwdArgs* a, Layout* l) {
   const MMScanArgs& f = a->fwd;
-  if (!dtype_size(f.dtype)) return MM_ERR_DTYPE;
-  if (f.batch < 0 || f.dim < 0 || f.seqlen < 0 || f.dstate < 1 || f.dstate > MM_MAX_DSTATE || f.batch > 0x7fffffffLL ||
-      f.dim > 0x7fffffffLL / (2 * MM_MAX_DSTATE) || f.seqlen > 0x7fffffffLL - kT)
-    return MM_ERR_SHAPE;
-  l->chunks = (int)((f.seqlen + kT - 1) / kT);
-  l->np = (int)(f.dstate + 3) / 4 * 4;
+  const int rc = check_sizes(f);
+  if (rc != MM_OK) return rc;
+  const int chunks = chunks_of(f), longs = longs_of(f), np = (int)(f.dstate + 3) / 4 * 4;
   l->passes = (int)((f.dstate + kNB - 1) / kNB);
-  // Channels of a CTA of the third kernel: as many (fewer partial sums of dB and dC) as leave every one of the
-  // 2 x 148 places four CTAs, at most 512, in tiles of 32 (16 for float32, and where 32 would leave places empty).
-  const long long rows = f.batch * (l->chunks > 0 ? l->chunks : 1);
-  const long long want = f.dim * rows / (4 * 2 * 148);
-  l->width = (f.dtype == MM_F32 && l->passes == 1) || f.dim * rows < 2 * 148 * 32 ? 16 : 32;
+  // Channels of a CTA: as many (fewer partial sums of dB and dC) as leave every one of the 3 x 148 places four CTAs,
+  // at most 512, in tiles of 32 (16 for float32, and where 32 would leave places empty).
+  const long long rows = f.batch * (chunks > 0 ? chunks : 1), lrows = f.batch * (longs > 0 ? longs : 1);
+  const long long want = f.dim * rows / (4 * 3 * 148);
+  l->width = (f.dtype == MM_F32 && l->passes == 1) || f.dim * rows < 3 * 148 * 32 ? 16 : 32;
   const long long tiles = want / l->width;
   l->tiles = (int)(l->passes > 1 || tiles < 1 ? 1 : tiles > 512 / l->width ? 512 / l->width : tiles);
   const long long per = (long long)l->width * l->tiles;
   l->groups = (int)((f.dim + per - 1) / per);
-  size_t at = 0;
-  auto take = [&](size_t n) {
-    const size_t r = at;
-    at += (n * sizeof(float) + 255) / 256 * 256;
-    return r;
-  };
-  const size_t rowd = (size_t)rows * f.dim, st = rowd * l->np;
+  const size_t rowd = (size_t)rows * f.dim, st = rowd * np, lrowd = (size_t)lrows * f.dim;
   const size_t bc = (size_t)rows * l->groups * l->passes * kNB * kT;
-  l->hst = take(l->chunks > 1 ? st : 0);
-  l->kst = take(l->chunks > 1 ? st : 0);
-  l->sum_d = take(l->chunks > 1 ? rowd : 0);
-  l->pB = take(bc);
-  l->pC = take(bc);
-  l->pA = take(st);
-  l->pD = take(rowd);
-  l->pbias = take(rowd);
-  l->bytes = at + 256;
+  Offsets o;
+  l->kst = o.take(chunks > 1 ? st : 0);
+  l->later = o.take(chunks > 1 ? rowd : 0);
+  l->klong = o.take(chunks > 1 ? lrowd * np : 0);
+  l->slong = o.take(chunks > 1 ? lrowd : 0);
+  l->pB = o.take(bc);
+  l->pC = o.take(bc);
+  l->pA = o.take(st);
+  l->pD = o.take(rowd);
+  l->pbias = o.take(rowd);
+  l->bytes = o.at + 256;
   return MM_OK;
 }
 
-inline void copy3(long long (&to)[3], const int64_t* from) {
-  for (int i = 0; i < 3; ++i) to[i] = from[i];
-}
-
-template <typename T, bool HAS_Z> int launch(const Params& p, cudaStream_t s) {
+template <typename T, bool HAS_Z> int launch(const Params& p, int64_t dtype, cudaStream_t s) {
   const long long rows = (long long)p.batch * p.chunks;
-  const int carry_smem = 3 * kT * kCarryPitch * (int)sizeof(float);
-  const long long dtiles = (p.dim + kCh - 1) / kCh;
-  if (rows * dtiles > 0x7fffffffLL || rows * p.groups > 0x7fffffffLL) return MM_ERR_SHAPE;
+  if (rows * p.groups > 0x7fffffffLL) return MM_ERR_SHAPE;
   if (p.chunks > 1) {
-    if (cudaFuncSetAttribute(carry_kernel<T, HAS_Z>, cudaFuncAttributeMaxDynamicSharedMemorySize, carry_smem) != cudaSuccess)
-      return MM_ERR_LAUNCH;
-    carry_kernel<T, HAS_Z><<<(unsigned)(rows * dtiles), kCarryThreads, carry_smem, s>>>(p);
-    if (cudaGetLastError() != cudaSuccess) return MM_ERR_LAUNCH;
-    const long long states = (long long)p.batch * p.dim * p.np;
-    if ((states + 255) / 256 > 0x7fffffffLL) return MM_ERR_SHAPE;
-    join_kernel<<<dim3((unsigned)((states + 255) / 256), 2), 256, 0, s>>>(p);
-    if (cudaGetLastError() != cudaSuccess) return MM_ERR_LAUNCH;
+    const int rc = walk_back(p, dtype, s);
+    if (rc != MM_OK) return rc;
   }
   if (p.passes > 1) {
     if (cudaFuncSetAttribute(grad_wide_kernel<T, HAS_Z>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem) != cudaSuccess)
@@ -948,13 +662,8 @@ template <typename T, bool HAS_Z> int launch(const Params& p, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
 }
 
-template <typename T> int launch_z(const Params& p, cudaStream_t s) {
-  return p.z ? launch<T, true>(p, s) : launch<T, false>(p, s);
-}
-
-bool rows_aligned(const void* q, const int64_t* st, const MMScanArgs& f) {
-  const int es = dtype_size(f.dtype);
-  return aligned16(q) && st[2] == 1 && (f.batch <= 1 || st[0] * es % 16 == 0) && (f.dim <= 1 || st[1] * es % 16 == 0);
+template <typename T> int launch_z(const Params& p, int64_t dtype, cudaStream_t s) {
+  return p.z ? launch<T, true>(p, dtype, s) : launch<T, false>(p, dtype, s);
 }
 
 bool columns_aligned(const void* q, const int64_t* st, const MMScanArgs& f) {
@@ -962,11 +671,11 @@ bool columns_aligned(const void* q, const int64_t* st, const MMScanArgs& f) {
   return aligned16(q) && st[1] == 1 && (f.batch <= 1 || st[0] * es % 16 == 0) && st[2] * es % 16 == 0;
 }
 
-}  // namespace bwd
+}  // namespace train
 }  // namespace mm
 
 using namespace mm;
-using namespace mm::bwd;
+using namespace mm::train;
 
 extern "C" int mm_selective_scan_bwd_workspace_size(const MMScanBwdArgs* a, size_t* bytes) {
   if (!a || !bytes) return MM_ERR_ARG;
@@ -994,16 +703,10 @@ extern "C" int mm_selective_scan_bwd(const MMScanBwdArgs* a, void* workspace, si
   if (!f.u || !f.delta || !f.A || !f.B || !f.C || !a->dy || !a->du || !a->ddelta || !a->dB || !a->dC || (f.z && !a->dz))
     return MM_ERR_ARG;
   if (!workspace || workspace_bytes < l.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return MM_ERR_WORKSPACE;
+  if (chunks_of(f) > 1 && (!a->states || reinterpret_cast<uintptr_t>(a->states) % 16)) return MM_ERR_ARG;
   Params p = {};
-  p.u = f.u;
-  p.delta = f.delta;
-  p.z = f.z;
-  p.B = f.B;
-  p.C = f.C;
+  set_inputs(p, f);
   p.dy = a->dy;
-  p.A = f.A;
-  p.D = f.D;
-  p.bias = f.delta_bias;
   p.dstate = a->dstate;
   p.du = a->du;
   p.ddelta = a->ddelta;
@@ -1013,24 +716,12 @@ extern "C" int mm_selective_scan_bwd(const MMScanBwdArgs* a, void* workspace, si
   p.dA = a->dA;
   p.dD = a->dD;
   p.dbias = a->ddelta_bias;
-  copy3(p.us, f.u_stride);
-  copy3(p.ds, f.delta_stride);
-  copy3(p.zs, f.z_stride);
-  copy3(p.Bs, f.B_stride);
-  copy3(p.Cs, f.C_stride);
   copy3(p.ys, a->dy_stride);
   copy3(p.dus, a->du_stride);
   copy3(p.dds, a->ddelta_stride);
   copy3(p.dzs, a->dz_stride);
   copy3(p.dBs, a->dB_stride);
   copy3(p.dCs, a->dC_stride);
-  p.As[0] = f.A_stride[0];
-  p.As[1] = f.A_stride[1];
-  p.batch = (int)f.batch;
-  p.dim = (int)f.dim;
-  p.dstate_n = (int)f.dstate;
-  p.seqlen = (int)f.seqlen;
-  p.softplus = f.delta_softplus != 0;
   p.vec = rows_aligned(f.u, f.u_stride, f) && rows_aligned(f.delta, f.delta_stride, f) &&
           rows_aligned(a->dy, a->dy_stride, f) && rows_aligned(a->du, a->du_stride, f) &&
           rows_aligned(a->ddelta, a->ddelta_stride, f) &&
@@ -1041,24 +732,24 @@ extern "C" int mm_selective_scan_bwd(const MMScanBwdArgs* a, void* workspace, si
   p.ahead = 1;
   for (int i = 0; i < (f.z ? 4 : 3); ++i)
     if (!(p.by_channel ? columns_aligned(act[i], act_stride[i], f) : rows_aligned(act[i], act_stride[i], f))) p.ahead = 0;
-  p.chunks = l.chunks;
-  p.np = l.np;
   p.passes = l.passes;
   p.groups = l.groups;
   p.tiles = l.tiles;
   p.width = l.width;
   char* w = static_cast<char*>(workspace);
-  p.hst = reinterpret_cast<float*>(w + l.hst);
+  p.hst = const_cast<float*>(a->states);
   p.kst = reinterpret_cast<float*>(w + l.kst);
-  p.sum_d = reinterpret_cast<float*>(w + l.sum_d);
+  p.later = reinterpret_cast<float*>(w + l.later);
+  p.klong = reinterpret_cast<float*>(w + l.klong);
+  p.slong = reinterpret_cast<float*>(w + l.slong);
   p.pB = reinterpret_cast<float*>(w + l.pB);
   p.pC = reinterpret_cast<float*>(w + l.pC);
   p.pA = reinterpret_cast<float*>(w + l.pA);
   p.pD = reinterpret_cast<float*>(w + l.pD);
   p.pbias = reinterpret_cast<float*>(w + l.pbias);
   switch (f.dtype) {
-    case MM_F32: return launch_z<float>(p, s);
-    case MM_F16: return launch_z<__half>(p, s);
-    default: return launch_z<__nv_bfloat16>(p, s);
+    case MM_F32: return launch_z<float>(p, f.dtype, s);
+    case MM_F16: return launch_z<__half>(p, f.dtype, s);
+    default: return launch_z<__nv_bfloat16>(p, f.dtype, s);
   }
 }

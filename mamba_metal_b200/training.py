@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from mamba_metal_b200 import _lib, ops
-from mamba_metal_b200.selective_scan import MAX_DSTATE, _scan_dtype, selective_scan_into
+from mamba_metal_b200.selective_scan import MAX_DSTATE, _scan_dtype
 
 CHECKPOINT8_BLOCK = 32  # values of a row that share an exponent (MM_CHECKPOINT8_BLOCK)
 
@@ -246,10 +246,13 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
 
 
 def selective_scan_backward(dy: torch.Tensor, u, delta, A, B, C, *, D=None, z=None, delta_bias=None,
-                            delta_softplus: bool = False, dstate: torch.Tensor | None = None) -> dict:
+                            delta_softplus: bool = False, dstate: torch.Tensor | None = None,
+                            states: torch.Tensor | None = None) -> dict:
     """Gradient of ``selective_scan`` for given dy (batch, dim, seqlen) and, optionally, dstate (batch, dim, dstate) of
-    the last state. All activations share one dtype; A, D and delta_bias are float32. Returns a dict of "u", "delta",
-    "B", "C", "z" (that dtype; "z" None without z) and "A", "D", "delta_bias" (float32; None where not given)."""
+    the last state. All activations share one dtype; A, D and delta_bias are float32. ``states`` is what
+    ``selective_scan_states`` returned for the same inputs; without it they are computed again. Returns a dict of
+    "u", "delta", "B", "C", "z" (that dtype; "z" None without z) and "A", "D", "delta_bias" (float32; None where
+    not given)."""
     dev = _lib.require_cuda(dy, u, delta, A, B, C, D, z, delta_bias, dstate)
     batch, dim, seqlen = u.shape
     n = A.shape[1]
@@ -262,6 +265,10 @@ def selective_scan_backward(dy: torch.Tensor, u, delta, A, B, C, *, D=None, z=No
     assert A.dtype == torch.float32
     if u.dtype not in _lib.DTYPE_CODE:
         raise TypeError(f"unsupported dtype {u.dtype}")
+    if states is None:
+        states = selective_scan_states(u, delta, A, B, C, D=D, z=z, delta_bias=delta_bias, delta_softplus=delta_softplus,
+                                       outputs=False)[2]
+    assert states.dtype == torch.float32 and states.is_contiguous() and states.is_cuda
     by_channel = _by_channel(u)
     dy = _laid_out(dy, by_channel)
     act = lambda: _empty(u.shape, u.dtype, dev, by_channel)
@@ -270,20 +277,18 @@ def selective_scan_backward(dy: torch.Tensor, u, delta, A, B, C, *, D=None, z=No
          "B": _empty(B.shape, u.dtype, dev, _by_channel(B)), "C": _empty(C.shape, u.dtype, dev, _by_channel(C)),
          "D": None if D is None else f32(dim), "delta_bias": None if delta_bias is None else f32(dim)}
     a = _lib.MMScanBwdArgs()
-    f = a.fwd
-    f.u, f.delta, f.A, f.B, f.C, f.D, f.z, f.delta_bias = (_lib.ptr(t) for t in (u, delta, A, B, C, D, z, delta_bias))
-    f.dtype = _lib.DTYPE_CODE[u.dtype]
-    f.batch, f.dim, f.dstate, f.seqlen = batch, dim, n, seqlen
-    f.u_stride, f.delta_stride, f.z_stride, f.B_stride, f.C_stride = (_lib.strides3(t) for t in (u, delta, z, B, C))
-    f.A_stride = (ctypes.c_int64 * 2)(*A.stride())
-    f.delta_softplus = int(bool(delta_softplus))
+    _scan_args(u, delta, A, B, C, D, z, delta_bias, delta_softplus, a.fwd)
+    nbytes = ctypes.c_size_t(0)
+    lib = _lib.lib()
+    _lib.check(lib.mm_selective_scan_states_size(ctypes.byref(a.fwd), ctypes.byref(nbytes)),
+               "mm_selective_scan_states_size")
+    assert states.numel() * 4 == nbytes.value, "states of another call"
+    a.states = states.data_ptr()
     a.dy, a.dstate = dy.data_ptr(), _lib.ptr(dstate)
     a.du, a.ddelta, a.dA, a.dB, a.dC = (g[k].data_ptr() for k in ("u", "delta", "A", "B", "C"))
     a.dD, a.dz, a.ddelta_bias = (_lib.ptr(g[k]) for k in ("D", "z", "delta_bias"))
     a.dy_stride, a.du_stride, a.ddelta_stride, a.dz_stride, a.dB_stride, a.dC_stride = \
         (_lib.strides3(t) for t in (dy, g["u"], g["delta"], g["z"], g["B"], g["C"]))
-    lib = _lib.lib()
-    nbytes = ctypes.c_size_t(0)
     _lib.check(lib.mm_selective_scan_bwd_workspace_size(ctypes.byref(a), ctypes.byref(nbytes)),
                "mm_selective_scan_bwd_workspace_size")
     ws = torch.empty(int(nbytes.value), dtype=torch.uint8, device=dev)
@@ -291,6 +296,54 @@ def selective_scan_backward(dy: torch.Tensor, u, delta, A, B, C, *, D=None, z=No
         rc = lib.mm_selective_scan_bwd(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
     _lib.check(rc, "mm_selective_scan_bwd")
     return g
+
+
+def selective_scan_states(u, delta, A, B, C, *, D=None, z=None, delta_bias=None, delta_softplus: bool = False,
+                          outputs: bool = True):
+    """The training forward pass: (y, last state, states), without a graph. All activations share one dtype; A, D and
+    delta_bias are float32. ``states`` (a flat float32 tensor: h before every 32nd step) is what
+    ``selective_scan_backward`` starts from. With ``outputs=False`` only states is computed, y and the last state
+    are None."""
+    dev = _lib.require_cuda(u, delta, A, B, C, D, z, delta_bias)
+    batch, dim, seqlen = u.shape
+    n = A.shape[1]
+    assert delta.shape == u.shape and tuple(B.shape) == (batch, n, seqlen) == tuple(C.shape)
+    assert (z is None or z.shape == u.shape) and tuple(A.shape) == (dim, n) and n <= MAX_DSTATE
+    for t in (delta, B, C, z):
+        assert t is None or t.dtype == u.dtype
+    for t in (D, delta_bias):
+        assert t is None or (t.dtype == torch.float32 and tuple(t.shape) == (dim,) and t.is_contiguous())
+    assert A.dtype == torch.float32
+    if u.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {u.dtype}")
+    y = _empty(u.shape, u.dtype, dev, _by_channel(u)) if outputs else None
+    state = torch.empty((batch, dim, n), dtype=torch.float32, device=dev) if outputs else None
+    a = _scan_args(u, delta, A, B, C, D, z, delta_bias, delta_softplus)
+    a.y, a.y_stride, a.state_out = _lib.ptr(y), _lib.strides3(y), _lib.ptr(state)
+    lib = _lib.lib()
+    nbytes, wbytes = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    _lib.check(lib.mm_selective_scan_states_size(ctypes.byref(a), ctypes.byref(nbytes)), "mm_selective_scan_states_size")
+    _lib.check(lib.mm_selective_scan_train_workspace_size(ctypes.byref(a), ctypes.byref(wbytes)),
+               "mm_selective_scan_train_workspace_size")
+    states = torch.empty(nbytes.value // 4, dtype=torch.float32, device=dev)
+    ws = torch.empty(wbytes.value, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        rc = lib.mm_selective_scan_train_fwd(ctypes.byref(a), states.data_ptr(), ws.data_ptr(), ws.numel(),
+                                             _lib.stream_handle(dev))
+    _lib.check(rc, "mm_selective_scan_train_fwd")
+    return y, state, states
+
+
+def _scan_args(u, delta, A, B, C, D, z, delta_bias, softplus, f=None):
+    f = _lib.MMScanArgs() if f is None else f
+    f.u, f.delta, f.A, f.B, f.C, f.D, f.z, f.delta_bias = (_lib.ptr(t) for t in (u, delta, A, B, C, D, z, delta_bias))
+    f.dtype = _lib.DTYPE_CODE[u.dtype]
+    f.batch, f.dim, f.seqlen = u.shape
+    f.dstate = A.shape[1]
+    f.u_stride, f.delta_stride, f.z_stride, f.B_stride, f.C_stride = (_lib.strides3(t) for t in (u, delta, z, B, C))
+    f.A_stride = (ctypes.c_int64 * 2)(*A.stride())
+    f.delta_softplus = int(bool(softplus))
+    return f
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -301,26 +354,21 @@ class _SelectiveScan(torch.autograd.Function):
         cast = lambda t: None if t is None else t.detach().to(dtype)
         uc, dc, Bc, Cc, zc = map(cast, (u, delta, B, C, z))
         Af, Df, bf = A.detach().float(), _f32(D), _f32(delta_bias)
-        batch, dim, seqlen = u.shape
-        y = _empty(u.shape, dtype, u.device, _by_channel(u))
-        state = torch.zeros if u.numel() == 0 else torch.empty  # a scan over nothing leaves the state at zero
-        state = state((batch, dim, A.shape[1]), dtype=torch.float32, device=u.device)
-        if u.numel():
-            selective_scan_into(uc, dc, Af, Bc, Cc, Df, zc, y, state, softplus, delta_bias=bf)
+        y, state, states = selective_scan_states(uc, dc, Af, Bc, Cc, D=Df, z=zc, delta_bias=bf, delta_softplus=softplus)
         ctx.softplus = softplus
         ctx.dtypes = tuple(None if t is None else t.dtype for t in (u, delta, A, B, C, D, z, delta_bias))
-        ctx.save_for_backward(uc, dc, Af, Bc, Cc, Df, zc, bf)
+        ctx.save_for_backward(uc, dc, Af, Bc, Cc, Df, zc, bf, states)
         return y.to(u.dtype), state
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dstate):
-        u, delta, A, B, C, D, z, bias = ctx.saved_tensors
+        u, delta, A, B, C, D, z, bias, states = ctx.saved_tensors
         if dy is None and dstate is None:
             return (None,) * 9
         dy = torch.zeros_like(u) if dy is None else dy.to(u.dtype)
         g = selective_scan_backward(dy, u, delta, A, B, C, D=D, z=z, delta_bias=bias, delta_softplus=ctx.softplus,
-                                    dstate=_f32(dstate))
+                                    dstate=_f32(dstate), states=states)
         names = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")
         return (*(None if t is None else g[k].to(t) for k, t in zip(names, ctx.dtypes)), None)
 
@@ -330,7 +378,7 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
                    delta_bias: torch.Tensor | None = None, delta_softplus: bool = False, return_state: bool = False):
     """Differentiable ``mamba_metal_b200.selective_scan``: shapes, dtypes and results as there, and ``delta_bias``
     (dim,), added to delta before softplus. The last state is differentiable too. y and the gradients of u, delta
-    and z are laid out like u. The backward pass keeps the inputs and nothing else: it recomputes the states."""
+    and z are laid out like u. Kept for the backward pass: the inputs and the state before every 32nd step."""
     batch, dim, seqlen = u.shape
     _, dstate = A.shape
     assert delta.shape == u.shape

@@ -17,7 +17,7 @@ def test_struct_layouts_are_padding_free():
     scan = 9 + 5 + 6 * 3 + 2 + 3 + 1
     for s, n in ((_lib.MMCheckpoint8Args, 3 + 4 + 9), (_lib.MMConvCheckpointArgs, 6 + 5 + 12 + 1),
                  (_lib.MMConvBwdArgs, 9 + 5 + 15 + 1), (_lib.MMPreferenceArgs, 10 + 4 + 4 + 1 + 2),
-                 (_lib.MMScanBwdArgs, scan + 10 + 18)):
+                 (_lib.MMScanBwdArgs, scan + 11 + 18)):
         assert ctypes.sizeof(s) == 8 * n, s.__name__
 
 
