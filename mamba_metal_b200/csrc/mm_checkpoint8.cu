@@ -15,61 +15,75 @@ struct Params {
 };
 
 // Time contiguous: a lane takes 8 consecutive values, so four lanes share a block and agree on its maximum by
-// two shuffles. VEC: 16-byte loads of x and 8-byte stores of codes. A warp covers 256 values of one row.
-template <typename T, bool PACK, bool VEC>
+// two shuffles. VEC: 16-byte accesses of x and 8-byte ones of codes. A warp covers CPT * 256 values of one row, with
+// all its loads in flight before the first is used (bf16 10240 x 32768: CPT 4 against 1).
+template <typename T, bool PACK, bool VEC, int CPT>
 __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per_row) {
   const int lane = threadIdx.x & 31;
   const long long gw = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (gw >= p.rows * warps_per_row) return;
   const long long row = gw / warps_per_row;
-  const int t0 = ((int)(gw % warps_per_row) * 32 + lane) * 8;
+  const int begin = (int)(gw % warps_per_row) * CPT * 256 + lane * 8;
   const long long b = row / p.dim, d = row % p.dim;
-  T* x = static_cast<T*>(p.x) + b * p.xs[0] + d * p.xs[1] + (long long)t0 * p.xs[2];
-  int8_t* codes = p.codes + b * p.cs[0] + d * p.cs[1] + (long long)t0 * p.cs[2];
-  uint8_t* exps = p.exps + b * p.es[0] + d * p.es[1] + (long long)(t0 / kCkBlock) * p.es[2];
-  const int n = min(8, p.length - t0);  // values of this lane; none or fewer than none past the row's end
-  float v[8];
+  T* x = static_cast<T*>(p.x) + b * p.xs[0] + d * p.xs[1];
+  int8_t* codes = p.codes + b * p.cs[0] + d * p.cs[1];
+  uint8_t* exps = p.exps + b * p.es[0] + d * p.es[1];
   if (PACK) {
-    if (VEC && n == 8) {
-      ck_load8<T>(x, v);
-    } else {
+    Raw8<T> raw[CPT];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = k < n ? ld_f32(x + k * p.xs[2]) : 0.f;
+    for (int j = 0; j < CPT; ++j) {
+      const int t = begin + j * 256;
+      raw[j] = raw_load(x + t * p.xs[2], p.xs[2], VEC, min(8, p.length - t));
     }
-    unsigned m = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, ck_abs_bits(v[k]));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    if (n <= 0) return;
-    const unsigned byte = ck_exponent(m);
-    const float inv = ck_inverse_scale(byte);
-    if ((lane & 3) == 0) *exps = (uint8_t)byte;
-    if (VEC && n == 8) {
-      uint2 w;
-      w.x = ck_pack4(ck_code(v[0], inv), ck_code(v[1], inv), ck_code(v[2], inv), ck_code(v[3], inv));
-      w.y = ck_pack4(ck_code(v[4], inv), ck_code(v[5], inv), ck_code(v[6], inv), ck_code(v[7], inv));
-      __stcs(reinterpret_cast<uint2*>(codes), w);
-    } else {
+    for (int j = 0; j < CPT; ++j) {
+      const int t = begin + j * 256, n = min(8, p.length - t);  // values of this lane; none past the row's end
+      unsigned m = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < n) codes[k * p.cs[2]] = (int8_t)ck_code(v[k], inv);
+      for (int k = 0; k < 8; ++k) m = max(m, ck_abs_bits(raw_at(raw[j], k)));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      if (n <= 0) continue;
+      const unsigned byte = ck_exponent(m);
+      const float inv = ck_inverse_scale(byte);
+      if ((lane & 3) == 0) exps[(long long)(t / kCkBlock) * p.es[2]] = (uint8_t)byte;
+      int c[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) c[k] = ck_code(raw_at(raw[j], k), inv);
+      if (VEC && n == 8) {
+        __stcs(reinterpret_cast<uint2*>(codes + t), make_uint2(ck_pack4(c[0], c[1], c[2], c[3]), ck_pack4(c[4], c[5], c[6], c[7])));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < n) codes[(t + k) * p.cs[2]] = (int8_t)c[k];
+      }
     }
   } else {
-    if (n <= 0) return;
-    const float scale = ck_scale(*exps);
-    if (VEC && n == 8) {
-      const uint2 w = __ldcs(reinterpret_cast<const uint2*>(codes));
+    uint2 raw[CPT];
+    float scale[CPT];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[k] = ck_restore<T>(ck_byte(w.x, k), scale);
-        v[k + 4] = ck_restore<T>(ck_byte(w.y, k), scale);
+    for (int j = 0; j < CPT; ++j) {
+      const int t = begin + j * 256;
+      if (t >= p.length) continue;
+      scale[j] = ck_scale(exps[(long long)(t / kCkBlock) * p.es[2]]);
+      if (VEC && t + 8 <= p.length) raw[j] = __ldcs(reinterpret_cast<const uint2*>(codes + t));
+    }
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) {
+      const int t = begin + j * 256, n = min(8, p.length - t);
+      if (VEC && n == 8) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[k] = ck_restore<T>(ck_byte(raw[j].x, k), scale[j]);
+          v[k + 4] = ck_restore<T>(ck_byte(raw[j].y, k), scale[j]);
+        }
+        ck_store8<T>(x + t, v);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < n) st_f32(x + (t + k) * p.xs[2], ck_restore<T>(codes[(t + k) * p.cs[2]], scale[j]));
       }
-      ck_store8<T>(x, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < n) st_f32(x + k * p.xs[2], ck_restore<T>(codes[k * p.cs[2]], scale));
     }
   }
 }
@@ -126,16 +140,19 @@ template <typename T, bool PACK> int launch(const MMCheckpoint8Args* a, cudaStre
     if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
     columns_kernel<T, PACK><<<(unsigned)grid, 256, 0, s>>>(p, blocks);
   } else {
-    const int wpr = (int)((a->length + 255) / 256);
+    const bool few = a->length <= 512;  // a warp per row, or half of one, where rows are short
+    const int wpr = (int)((a->length + (few ? 255 : 1023)) / (few ? 256 : 1024));
     const long long grid = (p.rows * wpr + 7) / 8;
     if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
     const bool vec = (p.xs[2] == 1 && p.cs[2] == 1) &&
                      ck_rows_aligned(a->x, a->x_stride, a->batch, a->dim, (int)sizeof(T), 16) &&
                      ck_rows_aligned(a->codes, a->codes_stride, a->batch, a->dim, 1, 8);
     if (vec)
-      rows_kernel<T, PACK, true><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
+      few ? rows_kernel<T, PACK, true, 1><<<(unsigned)grid, 256, 0, s>>>(p, wpr)
+          : rows_kernel<T, PACK, true, 4><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
     else
-      rows_kernel<T, PACK, false><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
+      few ? rows_kernel<T, PACK, false, 1><<<(unsigned)grid, 256, 0, s>>>(p, wpr)
+          : rows_kernel<T, PACK, false, 4><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
   }
   return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
 }
@@ -143,7 +160,7 @@ template <typename T, bool PACK> int launch(const MMCheckpoint8Args* a, cudaStre
 template <bool PACK> int dispatch(const MMCheckpoint8Args* a, mm_stream_t stream) {
   if (!a) return MM_ERR_ARG;
   if (!dtype_size(a->dtype)) return MM_ERR_DTYPE;
-  if (a->batch < 0 || a->dim < 0 || a->length < 0 || a->dim > 0x7fffffffLL || a->length > 0x7fffffffLL - 512)
+  if (a->batch < 0 || a->dim < 0 || a->length < 0 || a->dim > 0x7fffffffLL || a->length > 0x7fffffffLL - 2048)
     return MM_ERR_SHAPE;
   if (a->batch == 0 || a->dim == 0 || a->length == 0) return MM_OK;
   if (!a->x || !a->codes || !a->exponents) return MM_ERR_ARG;

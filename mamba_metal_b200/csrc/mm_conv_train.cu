@@ -38,66 +38,92 @@ MM_DEV float dact(float v, int silu_on) {
   return silu_on ? s * fmaf(v, 1.f - s, 1.f) : 1.f;
 }
 
+// The same on pairs
+MM_DEV f2_t both(float x) { return f2_pack(x, x); }
+MM_DEV f2_t sigmoid2(f2_t v) {
+  const float2 x = f2_unpack(f2_mul(v, both(-kLog2e)));
+  const float2 y = f2_unpack(f2_add(f2_pack(ex2(x.x), ex2(x.y)), both(1.f)));
+  return f2_pack(rcp(y.x), rcp(y.y));
+}
+MM_DEV f2_t act2(f2_t v, int silu_on) { return silu_on ? f2_mul(v, sigmoid2(v)) : v; }
+MM_DEV f2_t dact2(f2_t v, int silu_on) {
+  if (!silu_on) return both(1.f);
+  const f2_t s = sigmoid2(v);
+  return f2_mul(s, f2_fma(v, f2_sub(both(1.f), s), both(1.f)));
+}
+MM_DEV f2_t taps(const f2_t (&w)[kW], f2_t bias, f2_t a, f2_t b, f2_t c, f2_t d) {
+  return f2_fma(w[3], d, f2_fma(w[2], c, f2_fma(w[1], b, f2_fma(w[0], a, bias))));
+}
+
 // ---- time contiguous --------------------------------------------------------------------------------
-// A warp covers 256 consecutive steps of one row, 8 per lane; halos come from the neighbouring lanes, and for
-// the warp's first and last lane from memory.
-template <typename T, bool VEC>
+// A warp covers CPT * 256 consecutive steps of one row: chunk j of lane l are the 8 steps from 256 j + 8 l. All
+// its loads are in flight before the first is used (8 KB a warp at CPT 4, which the memory needs: 84 -> 46 us for
+// 8x1536x4096 f16 against CPT 1). Halos come from the neighbouring lanes, and for the warp's first and last lane
+// from memory.
+
+template <typename T, bool VEC, int CPT>
 __global__ void __launch_bounds__(256) fwd_rows_kernel(const Params p, int warps_per_row) {
   const int lane = threadIdx.x & 31;
   const long long gw = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long long rows = (long long)p.batch * p.dim;
   if (gw >= rows * warps_per_row) return;
   const long long row = gw / warps_per_row;
-  const int t0 = ((int)(gw % warps_per_row) * 32 + lane) * kE;
+  const int begin = (int)(gw % warps_per_row) * CPT * 256;
   const int b = (int)(row / p.dim), d = (int)(row % p.dim);
   const T* xr = static_cast<const T*>(p.x) + b * p.xs[0] + d * p.xs[1];
-  const int n = min(kE, p.seqlen - t0);
-  float win[kE + 3];
-  float v[kE];
-  if (VEC && n == kE) {
-    ck_load8<T>(xr + t0, v);
-  } else {
+  Raw8<T> x[CPT];
 #pragma unroll
-    for (int k = 0; k < kE; ++k) v[k] = k < n ? ld_f32(xr + (long long)(t0 + k) * p.xs[2]) : 0.f;
+  for (int j = 0; j < CPT; ++j) {
+    const int t = begin + j * 256 + lane * kE;
+    x[j] = raw_load(xr + (long long)t * p.xs[2], p.xs[2], VEC, min(kE, p.seqlen - t));
   }
+  float before[3];  // the three steps before the warp's chunk
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    win[k] = __shfl_up_sync(0xffffffffu, v[kE - 3 + k], 1);
-    if (lane == 0) win[k] = t0 > 0 ? ld_f32(xr + (long long)(t0 - 3 + k) * p.xs[2]) : 0.f;
-  }
-  unsigned m = 0;
-#pragma unroll
-  for (int k = 0; k < kE; ++k) {
-    win[k + 3] = v[k];
-    m = max(m, ck_abs_bits(v[k]));
-  }
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  if (n <= 0) return;
+  for (int k = 0; k < 3; ++k) before[k] = begin > 0 ? ld_f32(xr + (long long)(begin - 3 + k) * p.xs[2]) : 0.f;
   const float4 w = *reinterpret_cast<const float4*>(p.w + (long long)d * kW);
   const float bb = p.bias ? p.bias[d] : 0.f;
-  float o[kE];
-#pragma unroll
-  for (int k = 0; k < kE; ++k)
-    o[k] = act(fmaf(w.w, win[k + 3], fmaf(w.z, win[k + 2], fmaf(w.y, win[k + 1], fmaf(w.x, win[k], bb)))), p.silu);
-  const unsigned byte = ck_exponent(m);
-  const float inv = ck_inverse_scale(byte);
   T* orow = static_cast<T*>(p.out) + b * p.os[0] + d * p.os[1];
   int8_t* crow = p.codes_out + b * p.cs[0] + d * p.cs[1];
-  if ((lane & 3) == 0) p.exps_out[b * p.es[0] + d * p.es[1] + (long long)(t0 / kCkBlock) * p.es[2]] = (uint8_t)byte;
-  if (VEC && n == kE) {
-    ck_store8<T>(orow + t0, o);
-    uint2 c;
-    c.x = ck_pack4(ck_code(v[0], inv), ck_code(v[1], inv), ck_code(v[2], inv), ck_code(v[3], inv));
-    c.y = ck_pack4(ck_code(v[4], inv), ck_code(v[5], inv), ck_code(v[6], inv), ck_code(v[7], inv));
-    __stcs(reinterpret_cast<uint2*>(crow + t0), c);
-  } else {
+#pragma unroll
+  for (int j = 0; j < CPT; ++j) {
+    const int t0 = begin + j * 256 + lane * kE, n = min(kE, p.seqlen - t0);
+    float win[kE + 3];
+    unsigned m = 0;
+#pragma unroll
+    for (int k = 0; k < kE; ++k) {
+      win[k + 3] = raw_at(x[j], k);
+      m = max(m, ck_abs_bits(win[k + 3]));
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const float v = __shfl_sync(0xffffffffu, win[kE + k], (lane + 31) & 31);  // lane 0 takes lane 31's for the next chunk
+      win[k] = lane == 0 ? before[k] : v;
+      before[k] = v;
+    }
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    if (n <= 0) continue;
+    float o[kE];
 #pragma unroll
     for (int k = 0; k < kE; ++k)
-      if (k < n) {
-        st_f32(orow + (long long)(t0 + k) * p.os[2], o[k]);
-        crow[(long long)(t0 + k) * p.cs[2]] = (int8_t)ck_code(v[k], inv);
-      }
+      o[k] = act(fmaf(w.w, win[k + 3], fmaf(w.z, win[k + 2], fmaf(w.y, win[k + 1], fmaf(w.x, win[k], bb)))), p.silu);
+    const unsigned byte = ck_exponent(m);
+    const float inv = ck_inverse_scale(byte);
+    if ((lane & 3) == 0) p.exps_out[b * p.es[0] + d * p.es[1] + (long long)(t0 / kCkBlock) * p.es[2]] = (uint8_t)byte;
+    if (VEC && n == kE) {
+      ck_store8<T>(orow + t0, o);
+      uint2 c;
+      c.x = ck_pack4(ck_code(win[3], inv), ck_code(win[4], inv), ck_code(win[5], inv), ck_code(win[6], inv));
+      c.y = ck_pack4(ck_code(win[7], inv), ck_code(win[8], inv), ck_code(win[9], inv), ck_code(win[10], inv));
+      __stcs(reinterpret_cast<uint2*>(crow + t0), c);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kE; ++k)
+        if (k < n) {
+          st_f32(orow + (long long)(t0 + k) * p.os[2], o[k]);
+          crow[(long long)(t0 + k) * p.cs[2]] = (int8_t)ck_code(win[k + 3], inv);
+        }
+    }
   }
 }
 
@@ -121,95 +147,106 @@ template <typename T, bool CK> struct Source {
   MM_DEV float at(int t) const {
     return CK ? (float)codes[t * cs] * ck_scale(exps[(long long)(t / kCkBlock) * es]) : ld_f32(x + t * xs);
   }
-  MM_DEV void load8(int t0, float (&v)[kE]) const {
-    if (CK) {
-      const uint2 c = __ldcs(reinterpret_cast<const uint2*>(codes + t0));
-      const float scale = ck_scale(exps[(long long)(t0 / kCkBlock) * es]);
+  // eight steps as they lie in memory, their scale (1 for the input itself), and a value of them
+  struct Eight {
+    Raw8<T> x;
+    uint2 c;
+    float scale;
+    MM_DEV float at(int k) const { return CK ? (float)ck_byte(k < 4 ? c.x : c.y, k & 3) * scale : raw_at(x, k); }
+  };
+  MM_DEV Eight load(int t0, bool vec, int n) const {
+    Eight r = {};
+    if (!CK) {
+      r.x = raw_load(x + (long long)t0 * xs, xs, vec, n);
+    } else if (n > 0) {
+      if (vec && n == kE) {
+        r.c = __ldcs(reinterpret_cast<const uint2*>(codes + t0));
+      } else {
+        int v[kE];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[k] = (float)ck_byte(c.x, k) * scale;
-        v[k + 4] = (float)ck_byte(c.y, k) * scale;
+        for (int k = 0; k < kE; ++k) v[k] = k < n ? codes[(t0 + k) * cs] : 0;
+        r.c = make_uint2(ck_pack4(v[0], v[1], v[2], v[3]), ck_pack4(v[4], v[5], v[6], v[7]));
       }
-    } else {
-      ck_load8<T>(x + t0, v);
+      r.scale = ck_scale(exps[(long long)(t0 / kCkBlock) * es]);
     }
+    return r;
   }
 };
 
-template <typename T, bool CK, bool VEC>
+// The chunks from the last to the first, so that the three dpre after a chunk are known
+template <typename T, bool CK, bool VEC, int CPT>
 __global__ void __launch_bounds__(256) bwd_rows_kernel(const Params p, int warps_per_row) {
   const int lane = threadIdx.x & 31;
   const long long gw = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long long rows = (long long)p.batch * p.dim;
   if (gw >= rows * warps_per_row) return;
   const long long row = gw / warps_per_row;
-  const int part = (int)(gw % warps_per_row);
-  const int t0 = (part * 32 + lane) * kE;
+  const int part = (int)(gw % warps_per_row), begin = part * CPT * 256, end = begin + CPT * 256;
   const int b = (int)(row / p.dim), d = (int)(row % p.dim);
   const Source<T, CK> src(p, b, d);
   const T* grow = static_cast<const T*>(p.dout) + b * p.gs[0] + d * p.gs[1];
-  const int n = min(kE, p.seqlen - t0);
-  float v[kE], dp[kE + 3], win[kE + 3];
-  if (VEC && n == kE) {
-    src.load8(t0, v);
-    float g[kE];
-    ck_load8<T>(grow + t0, g);
+  typename Source<T, CK>::Eight x[CPT];
+  Raw8<T> g[CPT];
 #pragma unroll
-    for (int k = 0; k < kE; ++k) dp[k] = g[k];
-  } else {
-#pragma unroll
-    for (int k = 0; k < kE; ++k) {
-      v[k] = k < n ? src.at(t0 + k) : 0.f;
-      dp[k] = k < n ? ld_f32(grow + (long long)(t0 + k) * p.gs[2]) : 0.f;
-    }
+  for (int j = 0; j < CPT; ++j) {
+    const int t = begin + j * 256 + lane * kE, n = min(kE, p.seqlen - t);
+    x[j] = src.load(t, VEC, n);
+    g[j] = raw_load(grow + (long long)t * p.gs[2], p.gs[2], VEC, n);
   }
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    win[k] = __shfl_up_sync(0xffffffffu, v[kE - 3 + k], 1);
-    if (lane == 0) win[k] = t0 > 0 ? src.at(t0 - 3 + k) : 0.f;
-  }
-#pragma unroll
-  for (int k = 0; k < kE; ++k) win[k + 3] = v[k];
+  float before[3], after[3];  // x before the warp's steps; dpre of the three steps that follow the chunk at hand
   const float4 w = *reinterpret_cast<const float4*>(p.w + (long long)d * kW);
   const float bb = p.bias ? p.bias[d] : 0.f;
   auto pre = [&](float a, float c, float e, float f) { return fmaf(w.w, f, fmaf(w.z, e, fmaf(w.y, c, fmaf(w.x, a, bb)))); };
+#pragma unroll
+  for (int k = 0; k < 3; ++k) before[k] = begin > 0 ? src.at(begin - 3 + k) : 0.f;
+  {
+    float v[6];
+#pragma unroll
+    for (int k = 0; k < 6; ++k) v[k] = end - 3 + k < p.seqlen ? src.at(end - 3 + k) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      after[k] = end + k < p.seqlen ? ld_f32(grow + (long long)(end + k) * p.gs[2]) *
+                                          dact(pre(v[k], v[k + 1], v[k + 2], v[k + 3]), p.silu)
+                                    : 0.f;
+  }
+  T* orow = static_cast<T*>(p.out) + b * p.os[0] + d * p.os[1];
   float sum[kSums] = {0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int k = 0; k < kE; ++k) {
-    dp[k] *= dact(pre(win[k], win[k + 1], win[k + 2], win[k + 3]), p.silu);
+  for (int j = CPT - 1; j >= 0; --j) {
+    const int t0 = begin + j * 256 + lane * kE, n = min(kE, p.seqlen - t0);
+    float win[kE + 3], dp[kE + 3];
 #pragma unroll
-    for (int j = 0; j < kW; ++j) sum[j] = fmaf(dp[k], win[k + j], sum[j]);
-    sum[4] += dp[k];
-  }
-#pragma unroll
-  for (int k = 0; k < 3; ++k) dp[kE + k] = __shfl_down_sync(0xffffffffu, dp[k], 1);
-  if (lane == 31) {  // the three steps that the next warp owns
-    float a = win[kE], c = win[kE + 1], e = win[kE + 2];
+    for (int k = 0; k < kE; ++k) win[k + 3] = x[j].at(k);
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-      const int t = t0 + kE + k;
-      float f = 0.f, g = 0.f;
-      if (t < p.seqlen) {
-        f = src.at(t);
-        g = ld_f32(grow + (long long)t * p.gs[2]);
-      }
-      dp[kE + k] = t < p.seqlen ? g * dact(pre(a, c, e, f), p.silu) : 0.f;
-      a = c;
-      c = e;
-      e = f;
+      win[k] = __shfl_up_sync(0xffffffffu, win[kE + k], 1);
+      const float last = j > 0 ? __shfl_sync(0xffffffffu, x[j > 0 ? j - 1 : 0].at(kE - 3 + k), 31) : before[k];
+      if (lane == 0) win[k] = last;
     }
-  }
-  float o[kE];
 #pragma unroll
-  for (int k = 0; k < kE; ++k)
-    o[k] = fmaf(w.w, dp[k], fmaf(w.z, dp[k + 1], fmaf(w.y, dp[k + 2], w.x * dp[k + 3])));
-  T* orow = static_cast<T*>(p.out) + b * p.os[0] + d * p.os[1];
-  if (VEC && n == kE) {
-    ck_store8<T>(orow + t0, o);
-  } else {
+    for (int k = 0; k < kE; ++k) {
+      dp[k] = raw_at(g[j], k) * dact(pre(win[k], win[k + 1], win[k + 2], win[k + 3]), p.silu);
+#pragma unroll
+      for (int i = 0; i < kW; ++i) sum[i] = fmaf(dp[k], win[k + i], sum[i]);
+      sum[4] += dp[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      dp[kE + k] = __shfl_down_sync(0xffffffffu, dp[k], 1);
+      if (lane == 31) dp[kE + k] = after[k];
+      after[k] = __shfl_sync(0xffffffffu, dp[k], 0);
+    }
+    float o[kE];
 #pragma unroll
     for (int k = 0; k < kE; ++k)
-      if (k < n) st_f32(orow + (long long)(t0 + k) * p.os[2], o[k]);
+      o[k] = fmaf(w.w, dp[k], fmaf(w.z, dp[k + 1], fmaf(w.y, dp[k + 2], w.x * dp[k + 3])));
+    if (VEC && n == kE) {
+      ck_store8<T>(orow + t0, o);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kE; ++k)
+        if (k < n) st_f32(orow + (long long)(t0 + k) * p.os[2], o[k]);
+    }
   }
 #pragma unroll
   for (int j = 0; j < kSums; ++j)
@@ -223,213 +260,287 @@ __global__ void __launch_bounds__(256) bwd_rows_kernel(const Params p, int warps
 }
 
 // ---- channels contiguous ------------------------------------------------------------------------------
-// A thread walks `run` steps (a multiple of the checkpoint block) of two neighbouring channels, so a warp's
-// accesses run along 64 channels.
-constexpr int kC = 2;
+// A thread walks `run` steps (a multiple of the checkpoint block) of C neighbouring channels (8 bytes of them), so a
+// warp's accesses run along 128 channels of a 16-bit type, 64 of float32.
+template <typename T> constexpr int kC = 8 / (int)sizeof(T);
 
-template <typename T, bool VEC> MM_DEV void load_pair(const T* p, long long s, bool two, float (&v)[kC]) {
-  if (VEC && sizeof(T) == 2) {
-    const unsigned u = *reinterpret_cast<const unsigned*>(p);
-    uint4 q;
-    q.x = u;
-    const float2 f = vec_pair<T>(q, 0);
-    v[0] = f.x;
-    v[1] = f.y;
-  } else if (VEC) {
-    const float2 f = *reinterpret_cast<const float2*>(p);
-    v[0] = f.x;
-    v[1] = f.y;
-  } else {
-    v[0] = ld_f32(p);
-    v[1] = two ? ld_f32(p + s) : 0.f;
-  }
-}
-template <typename T, bool VEC> MM_DEV void store_pair(T* p, long long s, bool two, const float (&v)[kC]) {
-  if (VEC && sizeof(T) == 2) {
-    uint4 q;
-    vec_set_pair<T>(q, 0, v[0], v[1]);
-    *reinterpret_cast<unsigned*>(p) = q.x;
-  } else if (VEC) {
-    *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
-  } else {
-    st_f32(p, v[0]);
-    if (two) st_f32(p + s, v[1]);
-  }
-}
-template <bool VEC> MM_DEV void load_codes(const int8_t* p, long long s, bool two, int (&c)[kC]) {
+template <typename T, bool VEC> MM_DEV void load_few(const T* p, long long s, int n, f2_t (&v)[kC<T> / 2]) {
   if (VEC) {
-    const int u = *reinterpret_cast<const short*>(p);
-    c[0] = (int)(int8_t)u;
-    c[1] = u >> 8;
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    uint4 q;
+    q.x = u.x;
+    q.y = u.y;
+#pragma unroll
+    for (int c = 0; c < kC<T> / 2; ++c) {
+      const float2 f = vec_pair<T>(q, c);
+      v[c] = f2_pack(f.x, f.y);
+    }
   } else {
-    c[0] = *p;
-    c[1] = two ? p[s] : 0;
+#pragma unroll
+    for (int c = 0; c < kC<T> / 2; ++c)
+      v[c] = f2_pack(2 * c < n ? ld_f32(p + 2 * c * s) : 0.f, 2 * c + 1 < n ? ld_f32(p + (2 * c + 1) * s) : 0.f);
+  }
+}
+// The same as they lie in memory, to be unpacked later
+template <typename T, bool VEC> MM_DEV uint2 fetch_few(const T* p, long long s, int n) {
+  if (VEC) return __ldcs(reinterpret_cast<const uint2*>(p));
+  uint4 q = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int c = 0; c < kC<T>; ++c)
+    if (c < n) vec_set<T>(q, c, ld_f32(p + c * s));
+  return make_uint2(q.x, q.y);
+}
+template <typename T> MM_DEV f2_t unpack_few(uint2 u, int c) {
+  uint4 q;
+  q.x = u.x;
+  q.y = u.y;
+  const float2 f = vec_pair<T>(q, c);
+  return f2_pack(f.x, f.y);
+}
+template <typename T, bool VEC> MM_DEV void store_few(T* p, long long s, int n, const f2_t (&v)[kC<T> / 2]) {
+  if (VEC) {
+    uint4 q = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < kC<T> / 2; ++c) vec_set_pair<T>(q, c, f2_unpack(v[c]).x, f2_unpack(v[c]).y);
+    __stcs(reinterpret_cast<uint2*>(p), make_uint2(q.x, q.y));
+  } else {
+#pragma unroll
+    for (int c = 0; c < kC<T> / 2; ++c) {
+      if (2 * c < n) st_f32(p + 2 * c * s, f2_unpack(v[c]).x);
+      if (2 * c + 1 < n) st_f32(p + (2 * c + 1) * s, f2_unpack(v[c]).y);
+    }
+  }
+}
+// C bytes (codes or exponents)
+template <int C, bool VEC> MM_DEV unsigned load_bytes(const void* q, long long s, int n) {
+  const uint8_t* p = static_cast<const uint8_t*>(q);
+  if (VEC) return C == 4 ? *reinterpret_cast<const unsigned*>(p) : *reinterpret_cast<const unsigned short*>(p);
+  unsigned r = 0;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (c < n) r |= (unsigned)p[c * s] << (8 * c);
+  return r;
+}
+template <int C, bool VEC> MM_DEV void store_bytes(void* q, long long s, int n, unsigned v) {
+  uint8_t* p = static_cast<uint8_t*>(q);
+  if (VEC) {
+    if (C == 4)
+      *reinterpret_cast<unsigned*>(p) = v;
+    else
+      *reinterpret_cast<unsigned short*>(p) = (unsigned short)v;
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (c < n) p[c * s] = (uint8_t)(v >> (8 * c));
   }
 }
 
 struct Walk {
-  int b, d, t0, t1, run;
-  bool two;
+  int b, d, t0, t1, run, n;  // n: channels of this thread that exist
 };
-MM_DEV bool walk_of(const Params& p, int run, int runs, Walk& k) {
-  const int cg = (p.dim + kC - 1) / kC;
+template <int C> MM_DEV bool walk_of(const Params& p, int run, int runs, Walk& k) {
+  const int cg = (p.dim + C - 1) / C;
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= (long long)p.batch * runs * cg) return false;
-  k.d = (int)(i % cg) * kC;
+  k.d = (int)(i % cg) * C;
   k.run = (int)(i / cg % runs);
   k.b = (int)(i / cg / runs);
   k.t0 = k.run * run;
   k.t1 = min(p.seqlen, k.t0 + run);
-  k.two = k.d + 1 < p.dim;
+  k.n = min(C, p.dim - k.d);
   return true;
 }
-MM_DEV void load_weights(const Params& p, const Walk& k, float (&w)[kC][kW], float (&bb)[kC]) {
+template <int C> MM_DEV void load_weights(const Params& p, const Walk& k, f2_t (&w)[C / 2][kW], f2_t (&bb)[C / 2]) {
 #pragma unroll
-  for (int c = 0; c < kC; ++c) {
-    const int d = min(k.d + c, p.dim - 1);
-#pragma unroll
-    for (int j = 0; j < kW; ++j) w[c][j] = p.w[(long long)d * kW + j];
-    bb[c] = p.bias ? p.bias[d] : 0.f;
+  for (int c = 0; c < C / 2; ++c) {
+    const int d = min(k.d + 2 * c, p.dim - 1), e = min(k.d + 2 * c + 1, p.dim - 1);
+    const float4 v = *reinterpret_cast<const float4*>(p.w + (long long)d * kW);
+    const float4 u = *reinterpret_cast<const float4*>(p.w + (long long)e * kW);
+    w[c][0] = f2_pack(v.x, u.x), w[c][1] = f2_pack(v.y, u.y), w[c][2] = f2_pack(v.z, u.z), w[c][3] = f2_pack(v.w, u.w);
+    bb[c] = f2_pack(p.bias ? p.bias[d] : 0.f, p.bias ? p.bias[e] : 0.f);
   }
 }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int run, int runs) {
+  constexpr int C = kC<T>, H = C / 2;
   Walk k;
-  if (!walk_of(p, run, runs, k)) return;
+  if (!walk_of<C>(p, run, runs, k)) return;
   const T* x = static_cast<const T*>(p.x) + k.b * p.xs[0] + k.d * p.xs[1];
   T* out = static_cast<T*>(p.out) + k.b * p.os[0] + k.d * p.os[1];
   int8_t* codes = p.codes_out + k.b * p.cs[0] + k.d * p.cs[1];
   uint8_t* exps = p.exps_out + k.b * p.es[0] + k.d * p.es[1];
-  float w[kC][kW], bb[kC], win[kC][3];
-  load_weights(p, k, w, bb);
+  f2_t w[H][kW], bb[H], win[3][H];
+  load_weights<C>(p, k, w, bb);
 #pragma unroll
   for (int j = 0; j < 3; ++j) {
-    float v[kC] = {0.f, 0.f};
-    if (k.t0 > 0) load_pair<T, VEC>(x + (long long)(k.t0 - 3 + j) * p.xs[2], p.xs[1], k.two, v);
-    win[0][j] = v[0];
-    win[1][j] = v[1];
+#pragma unroll
+    for (int c = 0; c < H; ++c) win[j][c] = both(0.f);
+    if (k.t0 > 0) load_few<T, VEC>(x + (long long)(k.t0 - 3 + j) * p.xs[2], p.xs[1], k.n, win[j]);
   }
+  // Twice over each block: for its maxima, then, out of L1, for everything else. (Holding the block in registers
+  // instead leaves 8 warps an SM: bf16 4x5120x5601 255 us.)
   for (int tb = k.t0; tb < k.t1; tb += kCkBlock) {
-    T raw[kC][kCkBlock];
-    unsigned m[kC] = {0, 0};
+    const int n = min(kCkBlock, k.t1 - tb);
+    const T* xb = x + (long long)tb * p.xs[2];
+    unsigned m[C];
 #pragma unroll
-    for (int i = 0; i < kCkBlock; ++i) {
-      float v[kC] = {0.f, 0.f};
-      if (tb + i < k.t1) load_pair<T, VEC>(x + (long long)(tb + i) * p.xs[2], p.xs[1], k.two, v);
+    for (int c = 0; c < C; ++c) m[c] = 0;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      f2_t v[H];
+      load_few<T, VEC>(xb + i * p.xs[2], p.xs[1], k.n, v);
 #pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        raw[c][i] = ElemTraits<T>::from_f32(v[c]);
-        m[c] = max(m[c], ck_abs_bits(v[c]));
+      for (int c = 0; c < H; ++c) {
+        const float2 q = f2_unpack(v[c]);
+        m[2 * c] = max(m[2 * c], ck_abs_bits(q.x));
+        m[2 * c + 1] = max(m[2 * c + 1], ck_abs_bits(q.y));
       }
     }
-    float inv[kC];
+    float inv[C];
+    unsigned bytes = 0;
 #pragma unroll
-    for (int c = 0; c < kC; ++c) {
+    for (int c = 0; c < C; ++c) {
       const unsigned byte = ck_exponent(m[c]);
       inv[c] = ck_inverse_scale(byte);
-      if (c == 0 || k.two) exps[(long long)(tb / kCkBlock) * p.es[2] + c * p.es[1]] = (uint8_t)byte;
+      bytes |= byte << (8 * c);
     }
+    store_bytes<C, false>(exps + (long long)(tb / kCkBlock) * p.es[2], p.es[1], k.n, bytes);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      f2_t v[H], o[H];
+      load_few<T, VEC>(xb + i * p.xs[2], p.xs[1], k.n, v);
+      unsigned code = 0;
 #pragma unroll
-    for (int i = 0; i < kCkBlock; ++i) {
-      if (tb + i < k.t1) {
-        float o[kC];
-        int code[kC];
-#pragma unroll
-        for (int c = 0; c < kC; ++c) {
-          const float v = ElemTraits<T>::to_f32(raw[c][i]);
-          o[c] = act(fmaf(w[c][3], v, fmaf(w[c][2], win[c][2], fmaf(w[c][1], win[c][1], fmaf(w[c][0], win[c][0], bb[c])))),
-                     p.silu);
-          code[c] = ck_code(v, inv[c]);
-          win[c][0] = win[c][1];
-          win[c][1] = win[c][2];
-          win[c][2] = v;
-        }
-        store_pair<T, VEC>(out + (long long)(tb + i) * p.os[2], p.os[1], k.two, o);
-        int8_t* cp = codes + (long long)(tb + i) * p.cs[2];
-        if (VEC) {
-          *reinterpret_cast<short*>(cp) = (short)((code[0] & 0xff) | (code[1] << 8));
-        } else {
-          cp[0] = (int8_t)code[0];
-          if (k.two) cp[p.cs[1]] = (int8_t)code[1];
-        }
+      for (int c = 0; c < H; ++c) {
+        const float2 q = f2_unpack(v[c]);
+        o[c] = act2(taps(w[c], bb[c], win[0][c], win[1][c], win[2][c], v[c]), p.silu);
+        code |= (unsigned)(ck_code(q.x, inv[2 * c]) & 0xff) << (16 * c) |
+                (unsigned)(ck_code(q.y, inv[2 * c + 1]) & 0xff) << (16 * c + 8);
+        win[0][c] = win[1][c];
+        win[1][c] = win[2][c];
+        win[2][c] = v[c];
       }
+      store_few<T, VEC>(out + (long long)(tb + i) * p.os[2], p.os[1], k.n, o);
+      store_bytes<C, VEC>(codes + (long long)(tb + i) * p.cs[2], p.cs[1], k.n, code);
     }
   }
 }
 
 // Backward: step t completes dx[t-3] from the last four dpre; three steps past the run finish its end. Only the
-// run's own steps enter the sums.
+// run's own steps enter the sums. The loads of the next eight steps are in flight while eight are worked on; two
+// CTAs of an SM (128 registers) hide them best.
 template <typename T, bool CK, bool VEC>
-__global__ void __launch_bounds__(256) bwd_columns_kernel(const Params p, int run, int runs) {
+__global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int run, int runs) {
+    constexpr int C = kC<T>, H = C / 2, kU = 8;
+  static_assert(kU > 3 && kCkBlock % kU == 0, "from the second group on, step t - 3 is the run's own");
   Walk k;
-  if (!walk_of(p, run, runs, k)) return;
+  if (!walk_of<C>(p, run, runs, k)) return;
   const T* x = CK ? nullptr : static_cast<const T*>(p.x) + k.b * p.xs[0] + k.d * p.xs[1];
   const int8_t* codes = CK ? p.codes + k.b * p.cs[0] + k.d * p.cs[1] : nullptr;
   const uint8_t* exps = CK ? p.exps + k.b * p.es[0] + k.d * p.es[1] : nullptr;
   const T* dout = static_cast<const T*>(p.dout) + k.b * p.gs[0] + k.d * p.gs[1];
   T* dx = static_cast<T*>(p.out) + k.b * p.os[0] + k.d * p.os[1];
-  float w[kC][kW], bb[kC], win[kC][3], dp[kC][3], sum[kC][kSums];
-  load_weights(p, k, w, bb);
-  auto load_x = [&](int t, float (&v)[kC]) {
-    if (CK) {
-      int c[kC];
-      load_codes<VEC>(codes + (long long)t * p.cs[2], p.cs[1], k.two, c);
-      const uint8_t* e = exps + (long long)(t / kCkBlock) * p.es[2];
-      v[0] = (float)c[0] * ck_scale(e[0]);
-      v[1] = k.two ? (float)c[1] * ck_scale(e[p.es[1]]) : 0.f;
-    } else {
-      load_pair<T, VEC>(x + (long long)t * p.xs[2], p.xs[1], k.two, v);
-    }
+  f2_t w[H][kW], bb[H], win[3][H], dp[3][H], sum[kSums][H], scale[H];
+  load_weights<C>(p, k, w, bb);
+  auto scales = [&](int t) {  // of the block that holds step t
+    const unsigned e = load_bytes<C, false>(exps + (long long)(t / kCkBlock) * p.es[2], p.es[1], k.n);
+#pragma unroll
+    for (int c = 0; c < H; ++c)
+      scale[c] = f2_pack(ck_scale((e >> (16 * c)) & 0xff), ck_scale((e >> (16 * c + 8)) & 0xff));
   };
+  auto code_row = [&](int t) { return load_bytes<C, VEC>(codes + (long long)t * p.cs[2], p.cs[1], k.n); };
+  auto value = [&](unsigned v, int c) {
+    return f2_mul(f2_pack((float)ck_byte(v, 2 * c), (float)ck_byte(v, 2 * c + 1)), scale[c]);
+  };
+  if (CK && k.t0 > 0) scales(k.t0 - 1);
 #pragma unroll
   for (int j = 0; j < 3; ++j) {
-    float v[kC] = {0.f, 0.f};
-    if (k.t0 > 0) load_x(k.t0 - 3 + j, v);
 #pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      win[c][j] = v[c];
-      dp[c][j] = 0.f;
+    for (int c = 0; c < H; ++c) win[j][c] = dp[j][c] = both(0.f);
+    if (k.t0 > 0) {
+      if (CK) {
+        const unsigned v = code_row(k.t0 - 3 + j);
+#pragma unroll
+        for (int c = 0; c < H; ++c) win[j][c] = value(v, c);
+      } else {
+        load_few<T, VEC>(x + (long long)(k.t0 - 3 + j) * p.xs[2], p.xs[1], k.n, win[j]);
+      }
     }
   }
 #pragma unroll
-  for (int c = 0; c < kC; ++c)
+  for (int j = 0; j < kSums; ++j)
 #pragma unroll
-    for (int j = 0; j < kSums; ++j) sum[c][j] = 0.f;
-#pragma unroll 8
-  for (int t = k.t0; t < k.t1 + 3; ++t) {
-    float v[kC] = {0.f, 0.f}, g[kC] = {0.f, 0.f}, o[kC];
-    if (t < p.seqlen) {
-      load_x(t, v);
-      load_pair<T, VEC>(dout + (long long)t * p.gs[2], p.gs[1], k.two, g);
-    }
-    const bool mine = t < k.t1;
+    for (int c = 0; c < H; ++c) sum[j][c] = both(0.f);
+  // of the next kU steps, while these are worked on
+  uint2 v[kU], g[kU];
+  unsigned code[kU];
+  const int end = min(k.t1 + 3, p.seqlen);
+  auto fetch = [&](int i, int t) {
+    if (CK)
+      code[i] = code_row(t);
+    else
+      v[i] = fetch_few<T, VEC>(x + (long long)t * p.xs[2], p.xs[1], k.n);
+    g[i] = fetch_few<T, VEC>(dout + (long long)t * p.gs[2], p.gs[1], k.n);
+  };
+  auto fetch_some = [&](int i, int t) {
+    code[i] = 0;
+    v[i] = g[i] = make_uint2(0, 0);
+    if (t < end) fetch(i, t);
+  };
+  auto step = [&](int i, int t, bool inside, bool next) {
+    f2_t o[H], xv[H], gv[H];
 #pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      const float pre = fmaf(w[c][3], v[c], fmaf(w[c][2], win[c][2], fmaf(w[c][1], win[c][1], fmaf(w[c][0], win[c][0], bb[c]))));
-      const float q = t < p.seqlen ? g[c] * dact(pre, p.silu) : 0.f;
-      const float own = mine ? q : 0.f;
-      sum[c][0] = fmaf(own, win[c][0], sum[c][0]);
-      sum[c][1] = fmaf(own, win[c][1], sum[c][1]);
-      sum[c][2] = fmaf(own, win[c][2], sum[c][2]);
-      sum[c][3] = fmaf(own, v[c], sum[c][3]);
-      sum[c][4] += own;
-      o[c] = fmaf(w[c][3], dp[c][0], fmaf(w[c][2], dp[c][1], fmaf(w[c][1], dp[c][2], w[c][0] * q)));
-      win[c][0] = win[c][1];
-      win[c][1] = win[c][2];
-      win[c][2] = v[c];
-      dp[c][0] = dp[c][1];
-      dp[c][1] = dp[c][2];
-      dp[c][2] = q;
+    for (int c = 0; c < H; ++c) {
+      xv[c] = CK ? value(code[i], c) : unpack_few<T>(v[i], c);
+      gv[c] = unpack_few<T>(g[i], c);
     }
-    if (t - 3 >= k.t0) store_pair<T, VEC>(dx + (long long)(t - 3) * p.os[2], p.os[1], k.two, o);
+    if (next)
+      fetch(i, t + kU);
+    else
+      fetch_some(i, t + kU);
+#pragma unroll
+    for (int c = 0; c < H; ++c) {
+      // past the end dout is 0, past the run's own steps the sums are left alone
+      const f2_t q = f2_mul(gv[c], dact2(taps(w[c], bb[c], win[0][c], win[1][c], win[2][c], xv[c]), p.silu));
+      if (inside || t < k.t1) {
+        sum[0][c] = f2_fma(q, win[0][c], sum[0][c]);
+        sum[1][c] = f2_fma(q, win[1][c], sum[1][c]);
+        sum[2][c] = f2_fma(q, win[2][c], sum[2][c]);
+        sum[3][c] = f2_fma(q, xv[c], sum[3][c]);
+        sum[4][c] = f2_add(sum[4][c], q);
+      }
+      o[c] = f2_fma(w[c][3], dp[0][c], f2_fma(w[c][2], dp[1][c], f2_fma(w[c][1], dp[2][c], f2_mul(w[c][0], q))));
+      win[0][c] = win[1][c];
+      win[1][c] = win[2][c];
+      win[2][c] = xv[c];
+      dp[0][c] = dp[1][c];
+      dp[1][c] = dp[2][c];
+      dp[2][c] = q;
+    }
+    if (inside || (t - 3 >= k.t0 && t < k.t1 + 3)) store_few<T, VEC>(dx + (long long)(t - 3) * p.os[2], p.os[1], k.n, o);
+  };
+#pragma unroll
+  for (int i = 0; i < kU; ++i) fetch_some(i, k.t0 + i);
+  for (int tb = k.t0; tb < k.t1 + 3; tb += kU) {
+    if (CK && tb % kCkBlock == 0 && tb < p.seqlen) scales(tb);
+    if (tb > k.t0 && tb + 2 * kU <= k.t1) {  // nothing to check: without branches the steps overlap
+#pragma unroll
+      for (int i = 0; i < kU; ++i) step(i, tb + i, true, true);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kU; ++i) step(i, tb + i, false, false);
+    }
   }
   float* out = p.part + (((long long)k.b * runs + k.run) * p.dim + k.d) * kSums;
 #pragma unroll
-  for (int j = 0; j < kSums; ++j) {
-    out[j] = sum[0][j];
-    if (k.two) out[kSums + j] = sum[1][j];
-  }
+  for (int c = 0; c < H; ++c)
+#pragma unroll
+    for (int j = 0; j < kSums; ++j) {
+      const float2 v = f2_unpack(sum[j][c]);
+      if (2 * c < k.n) out[2 * c * kSums + j] = v.x;
+      if (2 * c + 1 < k.n) out[(2 * c + 1) * kSums + j] = v.y;
+    }
 }
 
 // Sums the partials of every channel in order, in 64 bits (a channel has up to a few thousand).
@@ -452,16 +563,17 @@ struct Plan {
 
 // Channels contiguous: runs long enough to be worth their three extra steps, short enough that the runs of all
 // rows fill the GPU twice over (148 SMs x 2048 threads).
-inline Plan make_plan(int64_t batch, int64_t dim, int64_t seqlen, bool columns) {
+inline Plan make_plan(int64_t dtype, int64_t batch, int64_t dim, int64_t seqlen, bool columns) {
   Plan pl;
+  const int C = 8 / dtype_size(dtype);
   pl.columns = columns;
   if (columns) {
-    const int64_t want = (2 * 148 * 2048 + batch * dim / kC) / (batch * dim / kC + 1);
+    const int64_t want = 2 * 148 * 2048 / (batch * dim / C + 1) + 1;
     int64_t run = (seqlen / (want > 0 ? want : 1) + kCkBlock - 1) / kCkBlock * kCkBlock;
     run = run < kCkBlock ? kCkBlock : run > 256 ? 256 : run;
     pl.run = (int)run;
   } else {
-    pl.run = 32 * kE;
+    pl.run = seqlen <= 512 ? 256 : 1024;  // CPT 1 or 4: a warp per row where a row is short
   }
   pl.parts = (int)((seqlen + pl.run - 1) / pl.run);
   return pl;
@@ -472,7 +584,7 @@ inline bool unit(const int64_t* st, int64_t n, int i) { return n <= 1 || st[i] =
 inline int check(int64_t dtype, int64_t batch, int64_t dim, int64_t seqlen, int64_t width) {
   if (width != kW) return MM_ERR_SHAPE;
   if (!dtype_size(dtype)) return MM_ERR_DTYPE;
-  if (batch < 0 || dim < 0 || seqlen < 0 || batch > 0x7fffffffLL || dim > 0x7fffffffLL / 8 || seqlen > 0x7fffffffLL - 512)
+  if (batch < 0 || dim < 0 || seqlen < 0 || batch > 0x7fffffffLL || dim > 0x7fffffffLL / 8 || seqlen > 0x7fffffffLL - 2048)
     return MM_ERR_SHAPE;
   return MM_OK;
 }
@@ -487,9 +599,9 @@ inline bool all_columns(int64_t dim, int64_t seqlen, const int64_t* const* st, i
     if (st[i][1] != 1 || st[i][2] == 1) return false;
   return true;
 }
-inline bool columns_aligned(const void* p, const int64_t* st, int64_t dim, int elem) {
-  const int a = kC * elem;
-  return dim % kC == 0 && reinterpret_cast<uintptr_t>(p) % a == 0 && (st[0] * elem) % a == 0 && (st[2] * elem) % a == 0;
+inline bool columns_aligned(const void* p, const int64_t* st, int64_t dim, int elem, int count) {
+  const int a = count * elem;
+  return dim % count == 0 && reinterpret_cast<uintptr_t>(p) % a == 0 && (st[0] * elem) % a == 0 && (st[2] * elem) % a == 0;
 }
 
 template <typename T> int launch_fwd(const MMConvCheckpointArgs* a, cudaStream_t s) {
@@ -509,13 +621,13 @@ template <typename T> int launch_fwd(const MMConvCheckpointArgs* a, cudaStream_t
   p.seqlen = (int)a->seqlen;
   p.silu = a->silu != 0;
   const int64_t* st[3] = {a->x_stride, a->out_stride, a->codes_stride};
-  const Plan pl = make_plan(a->batch, a->dim, a->seqlen, all_columns(a->dim, a->seqlen, st, 3));
+  const Plan pl = make_plan(a->dtype, a->batch, a->dim, a->seqlen, all_columns(a->dim, a->seqlen, st, 3));
   const int es = (int)sizeof(T);
   if (pl.columns) {
-    const long long threads = a->batch * pl.parts * ((a->dim + kC - 1) / kC), grid = (threads + 255) / 256;
+    const long long threads = a->batch * pl.parts * ((a->dim + kC<T> - 1) / kC<T>), grid = (threads + 255) / 256;
     if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
-    if (columns_aligned(a->x, a->x_stride, a->dim, es) && columns_aligned(a->out, a->out_stride, a->dim, es) &&
-        columns_aligned(a->codes, a->codes_stride, a->dim, 1))
+    if (columns_aligned(a->x, a->x_stride, a->dim, es, kC<T>) && columns_aligned(a->out, a->out_stride, a->dim, es, kC<T>) &&
+        columns_aligned(a->codes, a->codes_stride, a->dim, 1, kC<T>))
       fwd_columns_kernel<T, true><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts);
     else
       fwd_columns_kernel<T, false><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts);
@@ -526,16 +638,18 @@ template <typename T> int launch_fwd(const MMConvCheckpointArgs* a, cudaStream_t
         ck_rows_aligned(a->x, a->x_stride, a->batch, a->dim, es, 16) &&
         ck_rows_aligned(a->out, a->out_stride, a->batch, a->dim, es, 16) &&
         ck_rows_aligned(a->codes, a->codes_stride, a->batch, a->dim, 1, 8))
-      fwd_rows_kernel<T, true><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
+      pl.run == 256 ? fwd_rows_kernel<T, true, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
+                    : fwd_rows_kernel<T, true, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
     else
-      fwd_rows_kernel<T, false><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
+      pl.run == 256 ? fwd_rows_kernel<T, false, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
+                    : fwd_rows_kernel<T, false, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
   }
   return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
 }
 
 inline Plan bwd_plan(const MMConvBwdArgs* a) {
   const int64_t* st[3] = {a->x ? a->x_stride : a->codes_stride, a->dout_stride, a->dx_stride};
-  return make_plan(a->batch, a->dim, a->seqlen, all_columns(a->dim, a->seqlen, st, 3));
+  return make_plan(a->dtype, a->batch, a->dim, a->seqlen, all_columns(a->dim, a->seqlen, st, 3));
 }
 
 template <typename T, bool CK> int launch_bwd(const MMConvBwdArgs* a, float* part, cudaStream_t s) {
@@ -560,10 +674,10 @@ template <typename T, bool CK> int launch_bwd(const MMConvBwdArgs* a, float* par
   const Plan pl = bwd_plan(a);
   const int es = (int)sizeof(T);
   if (pl.columns) {
-    const long long threads = a->batch * pl.parts * ((a->dim + kC - 1) / kC), grid = (threads + 255) / 256;
+    const long long threads = a->batch * pl.parts * ((a->dim + kC<T> - 1) / kC<T>), grid = (threads + 255) / 256;
     if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
-    const bool src = CK ? columns_aligned(a->codes, a->codes_stride, a->dim, 1) : columns_aligned(a->x, a->x_stride, a->dim, es);
-    if (src && columns_aligned(a->dout, a->dout_stride, a->dim, es) && columns_aligned(a->dx, a->dx_stride, a->dim, es))
+    const bool src = CK ? columns_aligned(a->codes, a->codes_stride, a->dim, 1, kC<T>) : columns_aligned(a->x, a->x_stride, a->dim, es, kC<T>);
+    if (src && columns_aligned(a->dout, a->dout_stride, a->dim, es, kC<T>) && columns_aligned(a->dx, a->dx_stride, a->dim, es, kC<T>))
       bwd_columns_kernel<T, CK, true><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts);
     else
       bwd_columns_kernel<T, CK, false><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts);
@@ -576,9 +690,11 @@ template <typename T, bool CK> int launch_bwd(const MMConvBwdArgs* a, float* par
     if (src && unit(ss, a->seqlen, 2) && unit(a->dout_stride, a->seqlen, 2) && unit(a->dx_stride, a->seqlen, 2) &&
         ck_rows_aligned(a->dout, a->dout_stride, a->batch, a->dim, es, 16) &&
         ck_rows_aligned(a->dx, a->dx_stride, a->batch, a->dim, es, 16))
-      bwd_rows_kernel<T, CK, true><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
+      pl.run == 256 ? bwd_rows_kernel<T, CK, true, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
+                    : bwd_rows_kernel<T, CK, true, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
     else
-      bwd_rows_kernel<T, CK, false><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
+      pl.run == 256 ? bwd_rows_kernel<T, CK, false, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
+                    : bwd_rows_kernel<T, CK, false, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
   }
   if (cudaGetLastError() != cudaSuccess) return MM_ERR_LAUNCH;
   sum_kernel<<<(unsigned)((a->dim * kSums + 255) / 256), 256, 0, s>>>(part, a->batch * pl.parts, (int)a->dim, a->dweight,

@@ -10,6 +10,9 @@ namespace mm {
 namespace pref {
 
 constexpr int kThreads = 512;
+// Forward, so that a thread has about 24 vectors of a row of 50280: with 512 threads 189 us for 8200 rows of bf16,
+// with 256 156; for 1865 rows of float32 76 and 80.
+template <typename T> constexpr int kStatsThreads = sizeof(T) == 4 ? 512 : 256;
 
 struct Params {
   const void* logits;
@@ -19,6 +22,7 @@ struct Params {
   const float* grad_loss;
   void* dlogits;
   double* gain;  // beta (logp - ref) of every answer
+  unsigned* done;  // answers whose gain is there
   float4* part;  // of every (token, split): maximum, sum of exp(x - maximum), the label's logit
   long long ls[2], ds[2];
   long long tokens;
@@ -49,7 +53,8 @@ MM_DEV MaxSum join(MaxSum a, MaxSum b) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) stats_kernel(const Params p) {
+__global__ void __launch_bounds__(kStatsThreads<T>) stats_kernel(const Params p) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;  // for loss_kernel, which follows
   const long long token = blockIdx.x / p.splits;
   const int split = (int)(blockIdx.x % p.splits);
   const long long label = p.labels[token];
@@ -66,14 +71,14 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const Params p) {
   };
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   constexpr int kU = 4;  // vectors in flight
-  for (int i = v0 + threadIdx.x; i < v1; i += kU * kThreads) {
+  for (int i = v0 + threadIdx.x; i < v1; i += kU * kStatsThreads<T>) {
     uint4 q[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u)
-      if (i + u * kThreads < v1) q[u] = xv[i + u * kThreads];
+      if (i + u * kStatsThreads<T> < v1) q[u] = xv[i + u * kStatsThreads<T>];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      if (i + u * kThreads >= v1) break;
+      if (i + u * kStatsThreads<T> >= v1) break;
       float m = a.m;
 #pragma unroll
       for (int k = 0; k < kVec<T>; ++k) m = fmaxf(m, vec_elem<T>(q[u], k));
@@ -86,9 +91,9 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const Params p) {
     }
   }
   if (split == 0)
-    for (int i = threadIdx.x; i < head; i += kThreads) add1(ld_f32(x + i));
+    for (int i = threadIdx.x; i < head; i += kStatsThreads<T>) add1(ld_f32(x + i));
   if (split == p.splits - 1)
-    for (int i = head + nv * kVec<T> + threadIdx.x; i < p.vocab; i += kThreads) add1(ld_f32(x + i));
+    for (int i = head + nv * kVec<T> + threadIdx.x; i < p.vocab; i += kStatsThreads<T>) add1(ld_f32(x + i));
 #pragma unroll
   for (int h = 16; h > 0; h >>= 1) {
     MaxSum b;
@@ -96,11 +101,11 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const Params p) {
     b.s = __shfl_xor_sync(0xffffffffu, a.s, h);
     a = join(a, b);
   }
-  __shared__ MaxSum warp[kThreads / 32];
+  __shared__ MaxSum warp[kStatsThreads<T> / 32];
   if ((threadIdx.x & 31) == 0) warp[threadIdx.x >> 5] = a;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / 32; ++w) a = join(a, warp[w]);
+    for (int w = 1; w < kStatsThreads<T> / 32; ++w) a = join(a, warp[w]);
     const bool valid = label >= 0 && label < p.vocab;
     p.part[token * p.splits + split] = make_float4(a.m, a.s, valid ? ld_f32(x + label) : __uint_as_float(0x7fffffffu), 0.f);
   }
@@ -109,53 +114,59 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const Params p) {
 MM_DEV double softplus64(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
 MM_DEV double sigmoid64(double v) { return 1.0 / (1.0 + exp(-v)); }
 
-// One CTA: joins the splits, sums every answer's tokens (a warp per answer) and the pairs' losses.
-__global__ void __launch_bounds__(1024) loss_kernel(const Params p) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int r = warp; r < 2 * p.pairs; r += 32) {
-    double sum = 0;
-    for (int t = lane; t < p.length; t += 32) {
-      const long long token = (long long)r * p.length + t;
-      if (p.labels[token] == p.ignore) continue;
-      float4 a = p.part[token * p.splits];
-      MaxSum ms = {a.x, a.y};
-      for (int i = 1; i < p.splits; ++i) {
-        const float4 b = p.part[token * p.splits + i];
-        ms = join(ms, MaxSum{b.x, b.y});
-      }
-      p.stats[2 * token] = ms.m;
-      p.stats[2 * token + 1] = ms.s;
-      sum += (double)a.z - (double)ms.m - log((double)ms.s);
-    }
+// A CTA per answer joins the splits and sums the answer's tokens; the last one to finish takes the pairs' losses.
+constexpr int kLossThreads = 256;
+MM_DEV double block_sum(double v, double* warps) {  // in a fixed order; the result is thread 0's
 #pragma unroll
-    for (int h = 16; h > 0; h >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, h);
-    if (lane == 0) {
-      const double gain = p.beta * (sum - (double)p.ref[r]);
-      p.gain[r] = gain;
-      if (r < p.pairs)
-        p.chosen[r] = (float)gain;
-      else
-        p.rejected[r - p.pairs] = (float)gain;
+  for (int h = 16; h > 0; h >>= 1) v += __shfl_xor_sync(0xffffffffu, v, h);
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int w = 1; w < kLossThreads / 32; ++w) v += warps[w];
+  return v;
+}
+__global__ void __launch_bounds__(kLossThreads) loss_kernel(const Params p) {
+  __shared__ double warps[kLossThreads / 32];
+  __shared__ bool last;
+  const int r = blockIdx.x;
+  double sum = 0;
+  for (int t = threadIdx.x; t < p.length; t += kLossThreads) {
+    const long long token = (long long)r * p.length + t;
+    if (p.labels[token] == p.ignore) continue;
+    float4 a = p.part[token * p.splits];
+    MaxSum ms = {a.x, a.y};
+    for (int i = 1; i < p.splits; ++i) {
+      const float4 b = p.part[token * p.splits + i];
+      ms = join(ms, MaxSum{b.x, b.y});
     }
+    p.stats[2 * token] = ms.m;
+    p.stats[2 * token + 1] = ms.s;
+    sum += (double)a.z - (double)ms.m - log((double)ms.s);
   }
-  __syncthreads();  // the CTA that wrote the gains reads them
+  sum = block_sum(sum, warps);
+  if (threadIdx.x == 0) {
+    const double gain = p.beta * (sum - (double)p.ref[r]);
+    p.gain[r] = gain;
+    if (r < p.pairs)
+      p.chosen[r] = (float)gain;
+    else
+      p.rejected[r - p.pairs] = (float)gain;
+    __threadfence();  // the gain is there before the count says so
+    last = atomicAdd(p.done, 1u) == 2u * p.pairs - 1u;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
   double loss = 0;
-  for (int i = threadIdx.x; i < p.pairs; i += 1024) {
-    const double m = p.gain[i] - p.gain[p.pairs + i];
+  for (int i = threadIdx.x; i < p.pairs; i += kLossThreads) {
+    const double m = __ldcg(p.gain + i) - __ldcg(p.gain + p.pairs + i);
     loss += (1.0 - p.smoothing) * softplus64(-m) + p.smoothing * softplus64(m);
     const double dm = (p.smoothing * sigmoid64(m) - (1.0 - p.smoothing) * sigmoid64(-m)) * p.beta / p.pairs;
     p.slope[i] = (float)dm;
     p.slope[p.pairs + i] = (float)-dm;
   }
-  __shared__ double warps[32];
-#pragma unroll
-  for (int h = 16; h > 0; h >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, h);
-  if (lane == 0) warps[warp] = loss;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) loss += warps[w];
-    *p.loss = (float)(loss / p.pairs);
-  }
+  loss = block_sum(loss, warps);
+  if (threadIdx.x == 0) *p.loss = (float)(loss / p.pairs);
 }
 
 // dlogits of one (token, split of the vocabulary). Tokens run from the last to the first: the forward pass read
@@ -277,7 +288,7 @@ extern "C" int mm_preference_loss_workspace_size(const MMPreferenceArgs* a, size
   if (rc != MM_OK) return rc;
   if (!bytes) return MM_ERR_ARG;
   const long long tokens = 2 * a->pairs * a->length;
-  *bytes = (size_t)(2 * a->pairs) * 16 + (tokens ? (size_t)tokens * splits_of(a) * sizeof(float4) : 0);
+  *bytes = 16 + (size_t)(2 * a->pairs) * 16 + (tokens ? (size_t)tokens * splits_of(a) * sizeof(float4) : 0);
   return MM_OK;
 }
 
@@ -290,20 +301,23 @@ extern "C" int mm_preference_loss_fwd(const MMPreferenceArgs* a, void* workspace
   if (!a->ref || !a->loss || !a->chosen || !a->rejected || !a->slope) return MM_ERR_ARG;
   if (p.tokens && (!a->logits || !a->labels || !a->stats)) return MM_ERR_ARG;
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return MM_ERR_WORKSPACE;
-  p.gain = static_cast<double*>(workspace);
-  p.part = reinterpret_cast<float4*>(static_cast<char*>(workspace) + (size_t)(2 * a->pairs) * 16);
+  p.done = static_cast<unsigned*>(workspace);
+  p.gain = reinterpret_cast<double*>(static_cast<char*>(workspace) + 16);
+  p.part = reinterpret_cast<float4*>(static_cast<char*>(workspace) + 16 + (size_t)(2 * a->pairs) * 16);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const long long grid = p.tokens * p.splits;
   if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
   if (grid) {
     switch (a->dtype) {
-      case MM_F32: stats_kernel<float><<<(unsigned)grid, kThreads, 0, s>>>(p); break;
-      case MM_F16: stats_kernel<__half><<<(unsigned)grid, kThreads, 0, s>>>(p); break;
-      default: stats_kernel<__nv_bfloat16><<<(unsigned)grid, kThreads, 0, s>>>(p);
+      case MM_F32: stats_kernel<float><<<(unsigned)grid, kStatsThreads<float>, 0, s>>>(p); break;
+      case MM_F16: stats_kernel<__half><<<(unsigned)grid, kStatsThreads<__half>, 0, s>>>(p); break;
+      default: stats_kernel<__nv_bfloat16><<<(unsigned)grid, kStatsThreads<__nv_bfloat16>, 0, s>>>(p);
     }
     if (cudaGetLastError() != cudaSuccess) return MM_ERR_LAUNCH;
+  } else if (cudaMemsetAsync(p.done, 0, sizeof(unsigned), s) != cudaSuccess) {
+    return MM_ERR_LAUNCH;
   }
-  loss_kernel<<<1, 1024, 0, s>>>(p);
+  loss_kernel<<<(unsigned)(2 * a->pairs), kLossThreads, 0, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
 }
 

@@ -398,6 +398,7 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ref, beta, smoothing, ignore_index):
+        ctx.set_materialize_grads(False)
         rows, length, vocab = logits.shape
         dev, pairs = logits.device, rows // 2
         f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)
@@ -428,6 +429,8 @@ class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss, *_):
+        if grad_loss is None:
+            return (None,) * 6
         x, labels, stats, slope = ctx.saved_tensors
         grad = grad_loss.float().contiguous()
         dlogits = torch.empty(x.shape, dtype=x.dtype, device=x.device)
