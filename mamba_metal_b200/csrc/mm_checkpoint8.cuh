@@ -43,26 +43,6 @@ template <typename T> MM_DEV float ck_restore(int code, float scale) {
   return v > CkMax<T>::v ? CkMax<T>::v : v < -CkMax<T>::v ? -CkMax<T>::v : v;  // NaN passes both
 }
 
-// Eight values of a row as they lie in memory
-template <typename T> struct Raw8 {
-  uint4 v[sizeof(T) / 2];
-};
-template <typename T> MM_DEV Raw8<T> raw_load(const T* p, long long s, bool vec, int n) {
-  Raw8<T> r;
-  if (vec && n == 8) {
-#pragma unroll
-    for (int h = 0; h < (int)sizeof(T) / 2; ++h) r.v[h] = __ldcs(reinterpret_cast<const uint4*>(p) + h);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      vec_set<T>(r.v[k * sizeof(T) / 16], k % (16 / (int)sizeof(T)), k < n ? ld_f32(p + k * s) : 0.f);
-  }
-  return r;
-}
-template <typename T> MM_DEV float raw_at(const Raw8<T>& r, int k) {
-  return vec_elem<T>(r.v[k * sizeof(T) / 16], k % (16 / (int)sizeof(T)));
-}
-
 template <typename T> MM_DEV void ck_store8(T* p, const float (&v)[8]) {
 #pragma unroll
   for (int h = 0; h < (int)sizeof(T) / 2; ++h) {

@@ -210,6 +210,26 @@ template <> MM_DEV void vec_set<__nv_bfloat16>(uint4& v, int k, float x) {
   u4_set_word(v, k >> 1, (k & 1) ? ((w & 0xffffu) | (h << 16)) : ((w & 0xffff0000u) | h));
 }
 
+// Eight values of a row as they lie in memory
+template <typename T> struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+};
+template <typename T> MM_DEV Raw8<T> raw_load(const T* p, long long s, bool vec, int n) {
+  Raw8<T> r;
+  if (vec && n == 8) {
+#pragma unroll
+    for (int h = 0; h < (int)sizeof(T) / 2; ++h) r.v[h] = __ldcs(reinterpret_cast<const uint4*>(p) + h);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      vec_set<T>(r.v[k * sizeof(T) / 16], k % (16 / (int)sizeof(T)), k < n ? ld_f32(p + k * s) : 0.f);
+  }
+  return r;
+}
+template <typename T> MM_DEV float raw_at(const Raw8<T>& r, int k) {
+  return vec_elem<T>(r.v[k * sizeof(T) / 16], k % (16 / (int)sizeof(T)));
+}
+
 // ---- cp.async (LDGSTS) staging --------------------------------------------------------------------
 MM_DEV unsigned smem_u32(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
 MM_DEV void cp_async16(void* smem_dst, const void* gmem_src) {

@@ -543,12 +543,20 @@ __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int
     }
 }
 
-// Sums the partials of every channel in order, in 64 bits (a channel has up to a few thousand).
+// Sums the partials of every channel in a fixed order, in 64 bits: eight threads share a value.
 __global__ void __launch_bounds__(256) sum_kernel(const float* part, long long parts, int dim, float* dw, float* db) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= dim * kSums) return;
+  __shared__ double sum[8][32];
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+  const long long pitch = (long long)dim * kSums;
   double s = 0;
-  for (long long k = 0; k < parts; ++k) s += part[k * dim * kSums + i];
+  if (i < pitch) {
+#pragma unroll 4
+    for (long long k = row; k < parts; k += 8) s += part[k * pitch + i];
+  }
+  sum[row][lane] = s;
+  __syncthreads();
+  if (row != 0 || i >= pitch) return;
+  for (int k = 1; k < 8; ++k) s += sum[k][lane];
   const int d = i / kSums, j = i % kSums;
   if (j < kW)
     dw[d * kW + j] = (float)s;
@@ -697,7 +705,7 @@ template <typename T, bool CK> int launch_bwd(const MMConvBwdArgs* a, float* par
                     : bwd_rows_kernel<T, CK, false, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
   }
   if (cudaGetLastError() != cudaSuccess) return MM_ERR_LAUNCH;
-  sum_kernel<<<(unsigned)((a->dim * kSums + 255) / 256), 256, 0, s>>>(part, a->batch * pl.parts, (int)a->dim, a->dweight,
+  sum_kernel<<<(unsigned)((a->dim * kSums + 31) / 32), 256, 0, s>>>(part, a->batch * pl.parts, (int)a->dim, a->dweight,
                                                                      a->dbias);
   return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
 }

@@ -221,7 +221,7 @@ MM_DEV Incoming load_incoming(const Params& p, long long bc, int b, int d, int n
   const long long at = (bc * p.dim + d) * p.np + n0;
   if (p.longs > 1) {
     if (n0 < p.np) {
-      const long long bl = (long long)b * p.longs + (int)(bc % p.chunks) / kLong;
+      const long long bl = (long long)b * p.longs + (int)(bc % p.chunks) / p.per_long;
       r.k = *reinterpret_cast<const float4*>(p.klong + (bl * p.dim + d) * p.np + n0);
     }
   } else if (p.dstate) {
@@ -549,27 +549,42 @@ __global__ void __launch_bounds__(kWideThreads, 1) grad_wide_kernel(const Params
 }
 
 // ---- sums over groups and chunks -------------------------------------------------------------------
+// With more than 16 partials eight threads share a value (every eighth partial each): 5120 or 24 channels in groups of
+// 16 would otherwise be one chain of up to 320 loads. With fewer a thread has its own.
 template <typename T> __global__ void __launch_bounds__(256) reduce_kernel(const Params p, long long bc_blocks) {
-  if (blockIdx.x < bc_blocks) {  // dB and dC: over the groups of channels
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const long long per = (long long)p.chunks * p.passes * kNB * kT;
-    if (i >= p.batch * per) return;
-    const long long b = i / per, r = i % per;
-    const int step = (int)(r % kT), n = (int)(r / kT % (p.passes * kNB)), t = (int)(r / kT / (p.passes * kNB)) * kT + step;
-    if (n >= p.dstate_n || t >= p.seqlen) return;
+  __shared__ double sum[2][8][32];
+  const int lane = threadIdx.x % 32, part = threadIdx.x / 32;
+  if (blockIdx.x < bc_blocks) {  // dB and dC: over the groups of channels; a warp is 32 steps of a state
+    const int of = p.groups > 16 ? 8 : 1;
+    const long long per = (long long)p.chunks * p.passes * kNB;  // rows of 32 steps
+    const long long row = (long long)blockIdx.x * (8 / of) + part / of, b = row / per, r = row % per;
+    const int n = (int)(r % (p.passes * kNB)), t = (int)(r / (p.passes * kNB)) * kT + lane;
     double x = 0, y = 0;
-    for (int g = 0; g < p.groups; ++g) {
-      x += p.pB[(b * p.groups + g) * per + r];
-      y += p.pC[(b * p.groups + g) * per + r];
+    if (b < p.batch && n < p.dstate_n) {
+#pragma unroll 4
+      for (int g = part % of; g < p.groups; g += of) {
+        x += p.pB[((b * p.groups + g) * per + r) * kT + lane];
+        y += p.pC[((b * p.groups + g) * per + r) * kT + lane];
+      }
     }
+    if (of > 1) {
+      sum[0][part][lane] = x;
+      sum[1][part][lane] = y;
+      __syncthreads();
+      if (part > 0) return;
+      for (int k = 1; k < 8; ++k) {
+        x += sum[0][k][lane];
+        y += sum[1][k][lane];
+      }
+    }
+    if (b >= p.batch || n >= p.dstate_n || t >= p.seqlen) return;
     st_f32(static_cast<T*>(p.dB) + b * p.dBs[0] + n * p.dBs[1] + t * p.dBs[2], (float)x);
     st_f32(static_cast<T*>(p.dC) + b * p.dCs[0] + n * p.dCs[1] + t * p.dCs[2], (float)y);
     return;
   }
-  // dA, dD, dbias: over batch and chunks. Eight threads share a value, every eighth chunk each
+  // dA, dD, dbias: over batch and chunks
   const int dn = p.dim * p.np;
-  const long long v = ((long long)(blockIdx.x - bc_blocks) * 32) + threadIdx.x % 32;
-  const int part = threadIdx.x / 32;
+  const long long v = ((long long)(blockIdx.x - bc_blocks) * 32) + lane;
   const long long rows = (long long)p.batch * p.chunks;
   const float* src = nullptr;
   long long pitch = 0;
@@ -584,13 +599,14 @@ template <typename T> __global__ void __launch_bounds__(256) reduce_kernel(const
     pitch = p.dim;
   }
   double x = 0;
-  if (src)
+  if (src) {
+#pragma unroll 16
     for (long long r = part; r < rows; r += 8) x += src[r * pitch];
-  __shared__ double sum[8][32];
-  sum[part][threadIdx.x % 32] = x;
+  }
+  sum[0][part][lane] = x;
   __syncthreads();
   if (part != 0 || !src) return;
-  for (int k = 1; k < 8; ++k) x += sum[k][threadIdx.x];
+  for (int k = 1; k < 8; ++k) x += sum[0][k][lane];
   if (v < dn) {
     const int d = (int)(v / p.np), n = (int)(v % p.np);
     if (n < p.dstate_n) p.dA[(long long)d * p.dstate_n + n] = (float)x;
@@ -655,7 +671,8 @@ template <typename T, bool HAS_Z> int launch(const Params& p, int64_t dtype, cud
     grad_kernel<T, HAS_Z><<<(unsigned)(rows * p.groups), kGradThreads, kGradSmem<T>, s>>>(p);
   }
   if (cudaGetLastError() != cudaSuccess) return MM_ERR_LAUNCH;
-  const long long bc = (rows * p.passes * kNB * kT + 255) / 256;
+  static_assert(kT == 32, "a warp of reduce_kernel is a chunk of a state");
+  const long long bc = (rows * p.passes * kNB * (p.groups > 16 ? 8 : 1) + 7) / 8;
   const long long rest = ((long long)p.dim * (p.np + 2) + 31) / 32;
   if (bc + rest > 0x7fffffffLL) return MM_ERR_SHAPE;
   reduce_kernel<T><<<(unsigned)(bc + rest), 256, 0, s>>>(p, bc);

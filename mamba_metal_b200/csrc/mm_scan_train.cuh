@@ -8,7 +8,6 @@ namespace mm {
 namespace train {
 
 constexpr int kT = 32;     // steps of a chunk
-constexpr int kLong = 4;   // chunks of a long chunk
 constexpr int kK = 8;      // steps of a unit
 constexpr int kSegs = kT / kK;
 
@@ -25,7 +24,7 @@ struct Params {
   int by_channel;  // u is contiguous along channels
   int ahead;       // grad_kernel copies its raw inputs ahead: all contiguous along one axis, rows 16-byte aligned
   int np;          // states, rounded up to a multiple of four: rows of the buffers below
-  int chunks, longs;
+  int chunks, longs, per_long;  // chunks, long chunks, chunks of a long one
   // (batch, chunks, dim, np): the state every chunk starts from; the k it gets from the later chunks of its long one
   float *hst, *kst;
   float* later;  // (batch, chunks, dim): the sum of d over those
@@ -125,13 +124,13 @@ template <typename T> MM_DEV void store_steps(T* p, long long s, bool vec, int n
 
 // Where a thread's unit (eight steps of a channel) of a staged tile lies. Lanes run along whichever of time and
 // channels is contiguous in memory.
-template <int CH> MM_DEV void unit_of(int i, int by_channel, int& ch, int& seg) {
+template <int CH, int SEGS = kSegs> MM_DEV void unit_of(int i, int by_channel, int& ch, int& seg) {
   if (by_channel) {
     ch = i % CH;
     seg = i / CH;
   } else {
-    seg = i % (kSegs);
-    ch = i / (kSegs);
+    seg = i % SEGS;
+    ch = i / SEGS;
   }
 }
 
@@ -161,11 +160,17 @@ inline bool rows_aligned(const void* q, const int64_t* st, const MMScanArgs& f) 
   return aligned16(q) && st[2] == 1 && (f.batch <= 1 || st[0] * es % 16 == 0) && (f.dim <= 1 || st[1] * es % 16 == 0);
 }
 inline int chunks_of(const MMScanArgs& f) { return (int)((f.seqlen + kT - 1) / kT); }
-inline int longs_of(const MMScanArgs& f) { return (int)((f.seqlen + kT * kLong - 1) / (kT * kLong)); }
+// Chunks of a long one: four; fewer where that leaves an SM less than twelve warps of 32 channels to walk them
+inline int per_long_of(const MMScanArgs& f) {
+  int n = 4;
+  while (n > 1 && f.batch * ((f.dim + 31) / 32) * ((chunks_of(f) + n - 1) / n) < 12 * 148) n /= 2;
+  return n;
+}
+inline int longs_of(const MMScanArgs& f) { return (chunks_of(f) + per_long_of(f) - 1) / per_long_of(f); }
 inline int check_sizes(const MMScanArgs& f) {
   if (!dtype_size(f.dtype)) return MM_ERR_DTYPE;
   if (f.batch < 0 || f.dim < 0 || f.seqlen < 0 || f.dstate < 1 || f.dstate > MM_MAX_DSTATE || f.batch > 0x7fffffffLL ||
-      f.dim > 0x7fffffffLL / (2 * MM_MAX_DSTATE) || f.seqlen > 0x7fffffffLL - kT * kLong)
+      f.dim > 0x7fffffffLL / (2 * MM_MAX_DSTATE) || f.seqlen > 0x7fffffffLL - 256)
     return MM_ERR_SHAPE;
   return MM_OK;
 }
@@ -203,6 +208,7 @@ inline void set_inputs(Params& p, const MMScanArgs& f) {
   p.np = (int)(f.dstate + 3) / 4 * 4;
   p.chunks = chunks_of(f);
   p.longs = longs_of(f);
+  p.per_long = per_long_of(f);
 }
 
 // Fills kst, later, klong and slong (mm_scan_walk.cu): the part of the gradient that runs through time

@@ -1,8 +1,8 @@
 // The parts of the selective scan's training kernels that run through time: the forward pass, and the gradient's
 // reverse recurrence.
 //
-// Time is cut into long chunks of 128 steps. A warp takes 32 channels (lane = channel, all states in registers) of
-// one long chunk and walks its steps:
+// Time is cut into long chunks of up to 128 steps. A warp takes 32 channels (a lane each, all its states in registers)
+// of one long chunk and walks its steps:
 //   kState: from zero, what the chunk adds to the state that comes into it;
 //   kOut:   from the state that comes into it, y, and h at the start of every 32 steps (what the gradient needs);
 //   kBack:  in reverse from zero, k_{t-1} = a_t (C_t e_t + k_t), and k at the end of every 32 steps.
@@ -10,8 +10,11 @@
 // chunk's decay. d, d u and e are computed once per element by the lane that loads it and pass through shared
 // memory as [step][channel]; warps share nothing, so no block barriers.
 //
-// Bound by the MUFU: one ex2 for each state and step, 16 per clock and SM; a walk of 8x1536x4096 with 16 states is
-// 805 M of them, 0.18 ms at 1.9 GHz.
+// Bound by the MUFU (one ex2 for each state and step, 16 per clock and SM: 805 M, 0.18 ms at 1.9 GHz for a walk of
+// 8x1536x4096 with 16 states) and close behind by the registers' way in from shared memory, 128 bytes per clock: a
+// step's B and C arrive as 32 lanes x 128 bytes. Measured there, f16: kState 0.28 ms, kOut 0.45, kBack 0.33, with
+// four blocks of four warps on an SM (five and six spill: kOut 0.50 and 0.58); tiles of 32 steps 0.32, 0.55, 0.39;
+// two channels a lane, which share B and C but leave 12 warps, 0.30, 0.53, 0.48.
 #include "mm_scan_train.cuh"
 
 namespace mm {
@@ -19,151 +22,168 @@ namespace train {
 
 enum Walk { kState, kOut, kBack };
 constexpr int kWarps = 4;
-constexpr int kTile = kT * 33;  // floats of a [step][channel] tile, padded
+constexpr int kSub = 16;  // steps staged at a time
 
-template <int MODE, int NM> constexpr int kWarpFloats = 2 * kTile + (MODE == kOut ? 2 : 1) * kT * NM;
+constexpr int kTile = kSub * 33;
+template <int MODE, int NM> constexpr int kWarpFloats = 2 * kTile + (MODE == kOut ? 2 : 1) * kSub * NM;
 
-// B or C of 32 steps as [step][state]
+// B or C of a tile's steps as [step][state]; lanes l and l + 16 share a step
 template <typename T, int NM>
 MM_DEV void stage_states(const void* base, const long long (&st)[3], const Params& p, int b, int t0, int lane, float* out) {
 #pragma unroll 4
-  for (int j = 0; j < NM / 4; ++j)
-    *reinterpret_cast<float4*>(out + lane * NM + 4 * j) = load_BC(static_cast<const T*>(base), st, b, 4 * j, t0 + lane, p);
+  for (int j = lane / kSub; j < NM / 4; j += 2)
+    *reinterpret_cast<float4*>(out + lane % kSub * NM + 4 * j) =
+        load_BC(static_cast<const T*>(base), st, b, 4 * j, t0 + lane % kSub, p);
 }
 
 template <int MODE, typename T, int NM>
-__global__ void __launch_bounds__(kWarps * 32) walk_kernel(const Params p) {
+__global__ void __launch_bounds__(kWarps * 32, NM <= 16 ? 4 : NM <= 32 ? 3 : 2) walk_kernel(const Params p) {
+  constexpr int PITCH = 33, UNITS = kSub / kK;
   extern __shared__ float4 smem4[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* sd = reinterpret_cast<float*>(smem4) + warp * ((kWarpFloats<MODE, NM> + 3) / 4 * 4);
+  float* sB = reinterpret_cast<float*>(smem4) + warp * ((kWarpFloats<MODE, NM> + 3) / 4 * 4);  // B, or C
+  float* sC = sB + kSub * NM;
+  float* sd = sC + (MODE == kOut ? kSub * NM : 0);
   float* sx = sd + kTile;  // d u (then y without D u and the gate), or e
-  float* sB = sx + kTile;  // B, or C
-  float* sC = sB + (MODE == kOut ? kT * NM : 0);
   const int groups = (p.dim + 31) / 32;
   const long long item = (long long)blockIdx.x * kWarps + warp;
   if (item >= (long long)p.batch * p.longs * groups) return;
   const int d0 = (int)(item % groups) * 32, d = d0 + lane;
   const long long bl = item / groups;
   const int l = (int)(bl % p.longs), b = (int)(bl / p.longs);
+  const int begin = l * p.per_long * kT, end = min(p.seqlen, begin + p.per_long * kT);
+
   const bool mine = d < p.dim;
-  const long long row = (bl * p.dim + d) * p.np;
 
   f2_t A[NM / 2], h[NM / 2];
+  float sum = 0.f;
 #pragma unroll
   for (int j = 0; j < NM / 4; ++j) {
     const float4 a = mine ? load_A(p, d, 4 * j) : f4(0.f, 0.f, 0.f, 0.f);
     A[2 * j] = mul1(f2_pack(a.x, a.y), kLog2e);
     A[2 * j + 1] = mul1(f2_pack(a.z, a.w), kLog2e);
     float4 x = f4(0.f, 0.f, 0.f, 0.f);
-    if (MODE == kOut && p.longs > 1 && mine && 4 * j < p.np) x = *reinterpret_cast<const float4*>(p.hlong + row + 4 * j);
+    if (MODE == kOut && p.longs > 1 && mine && 4 * j < p.np)
+      x = *reinterpret_cast<const float4*>(p.hlong + (bl * p.dim + d) * p.np + 4 * j);
     h[2 * j] = f2_pack(x.x, x.y);
     h[2 * j + 1] = f2_pack(x.z, x.w);
   }
-  auto put = [&](float* to) {
+  // the lane's states to their row of `to`, (.., dim, np)
+  auto put = [&](float* to, long long row) {
+    if (!mine) return;
 #pragma unroll
     for (int j = 0; j < NM / 4; ++j)
       if (4 * j < p.np) {
         const float2 x = f2_unpack(h[2 * j]), y = f2_unpack(h[2 * j + 1]);
-        *reinterpret_cast<float4*>(to + 4 * j) = f4(x.x, x.y, y.x, y.y);
+        *reinterpret_cast<float4*>(to + (row * p.dim + d) * p.np + 4 * j) = f4(x.x, x.y, y.x, y.y);
       }
   };
-  float sum = 0.f;
 
-  for (int i = 0; i < kLong; ++i) {
-    const int c = l * kLong + (MODE == kBack ? kLong - 1 - i : i), t0 = c * kT;
-    if (t0 >= p.seqlen) continue;
+  const int tiles = (end - begin + kSub - 1) / kSub;
+  for (int i = 0; i < tiles; ++i) {
+    const int t0 = begin + (MODE == kBack ? tiles - 1 - i : i) * kSub;
     __syncwarp();
-    // d and d u or e; zeros where there are no steps or channels: a = 1 there, and nothing is added
-#pragma unroll 1
-    for (int j = 0; j < kSegs; ++j) {
-      int ch, seg;
-      unit_of<32>(lane + 32 * j, p.by_channel, ch, seg);
-      const int t = t0 + seg * kK, n = d0 + ch < p.dim ? min(kK, p.seqlen - t) : 0, dc = min(d0 + ch, p.dim - 1);
-      float raw[kK], x[kK], z[kK];
-      load_steps(static_cast<const T*>(p.delta) + b * p.ds[0] + dc * p.ds[1] + t * p.ds[2], p.ds[2], p.vec, n, raw);
-      if (MODE == kBack) {
-        load_steps(static_cast<const T*>(p.dy) + b * p.ys[0] + dc * p.ys[1] + t * p.ys[2], p.ys[2], p.vec, n, x);
-        if (p.z) load_steps(static_cast<const T*>(p.z) + b * p.zs[0] + dc * p.zs[1] + t * p.zs[2], p.zs[2], p.vec, n, z);
-      } else {
-        load_steps(static_cast<const T*>(p.u) + b * p.us[0] + dc * p.us[1] + t * p.us[2], p.us[2], p.vec, n, x);
-      }
-      const f2_t bias = dup(p.bias ? p.bias[dc] : 0.f);
+    Raw8<T> raw[UNITS], x[UNITS], z[UNITS];  // delta; u or dy; z: all loads in flight together
+    auto fetch = [&](const void* base, const long long (&st)[3], Raw8<T>(&r)[UNITS]) {
 #pragma unroll
-      for (int k = 0; k < kK; k += 2) {
-        float2 dt = f2_unpack(step_of(f2_add(f2_pack(raw[k], raw[k + 1]), bias), p.softplus));
-        dt.x = k < n ? dt.x : 0.f;
-        dt.y = k + 1 < n ? dt.y : 0.f;
-        f2_t v = f2_pack(x[k], x[k + 1]);
-        if (MODE != kBack)
-          v = f2_mul(v, f2_pack(dt.x, dt.y));
-        else if (p.z)
-          v = f2_mul(v, silu_of(f2_pack(z[k], z[k + 1])));
-        const float2 w = f2_unpack(v);
-        const int at = (seg * kK + k) * 33 + ch;
-        sd[at] = dt.x;
-        sd[at + 33] = dt.y;
-        sx[at] = w.x;
-        sx[at + 33] = w.y;
+      for (int j = 0; j < UNITS; ++j) {
+        int ch, seg;
+        unit_of<32, kSub / kK>(lane + 32 * j, p.by_channel, ch, seg);
+        const int t = t0 + seg * kK, n = d0 + ch < p.dim ? min(kK, p.seqlen - t) : 0;
+        r[j] = raw_load(static_cast<const T*>(base) + b * st[0] + (d0 + ch) * st[1] + t * st[2], st[2], p.vec, n);
       }
+    };
+    fetch(p.delta, p.ds, raw);
+    if (MODE == kBack) {
+      fetch(p.dy, p.ys, x);
+      if (p.z) fetch(p.z, p.zs, z);
+    } else {
+      fetch(p.u, p.us, x);
     }
     if (MODE != kBack) stage_states<T, NM>(p.B, p.Bs, p, b, t0, lane, sB);
     if (MODE == kOut) stage_states<T, NM>(p.C, p.Cs, p, b, t0, lane, sC);
     if (MODE == kBack) stage_states<T, NM>(p.C, p.Cs, p, b, t0, lane, sB);
-    const long long bc = (long long)b * p.chunks + c;
-    if (MODE == kOut && p.hst && mine) put(p.hst + (bc * p.dim + d) * p.np);
-    if (MODE == kBack && mine) {
-      put(p.kst + (bc * p.dim + d) * p.np);
-      p.later[bc * p.dim + d] = sum;
+    // d and d u or e; zeros where there are no steps or channels: a = 1 there, and nothing is added
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+      int ch, seg;
+      unit_of<32, kSub / kK>(lane + 32 * j, p.by_channel, ch, seg);
+      const int t = t0 + seg * kK, n = d0 + ch < p.dim ? min(kK, p.seqlen - t) : 0;
+      const f2_t bias = dup(p.bias && d0 + ch < p.dim ? p.bias[d0 + ch] : 0.f);
+#pragma unroll
+      for (int k = 0; k < kK; k += 2) {
+        float2 dt = f2_unpack(step_of(f2_add(f2_pack(raw_at(raw[j], k), raw_at(raw[j], k + 1)), bias), p.softplus));
+        dt.x = k < n ? dt.x : 0.f;
+        dt.y = k + 1 < n ? dt.y : 0.f;
+        f2_t v = f2_pack(raw_at(x[j], k), raw_at(x[j], k + 1));
+        if (MODE != kBack)
+          v = f2_mul(v, f2_pack(dt.x, dt.y));
+        else if (p.z)
+          v = f2_mul(v, silu_of(f2_pack(raw_at(z[j], k), raw_at(z[j], k + 1))));
+        const float2 w = f2_unpack(v);
+        const int at = (seg * kK + k) * PITCH + ch;
+        sd[at] = dt.x;
+        sd[at + PITCH] = dt.y;
+        sx[at] = w.x;
+        sx[at + PITCH] = w.y;
+      }
+    }
+    const long long bc = (long long)b * p.chunks + t0 / kT;
+    if (MODE == kOut && p.hst && t0 % kT == 0) put(p.hst, bc);
+    if (MODE == kBack && (t0 % kT == kT - kSub || i == 0)) {  // the chunk's last tile that has steps
+      put(p.kst, bc);
+      if (mine) p.later[bc * p.dim + d] = sum;
     }
     __syncwarp();
-#pragma unroll 4
-    for (int j = 0; j < kT; ++j) {
-      const int t = MODE == kBack ? kT - 1 - j : j;
-      const float dt = sd[t * 33 + lane], x = sx[t * 33 + lane];
-      sum += dt;
-      const f2_t dt2 = dup(dt), x2 = dup(x);
+#pragma unroll 2
+    for (int j = 0; j < kSub; ++j) {
+      const int t = MODE == kBack ? kSub - 1 - j : j;
       const ulonglong2* Bt = reinterpret_cast<const ulonglong2*>(sB + t * NM);
       const ulonglong2* Ct = reinterpret_cast<const ulonglong2*>(sC + t * NM);
+      const float dt = sd[t * PITCH + lane];
+      sum += dt;
+      const f2_t dt2 = dup(dt), x2 = dup(sx[t * PITCH + lane]);
       f2_t y0 = dup(0.f), y1 = y0;
 #pragma unroll
       for (int k = 0; k < NM / 4; ++k) {
         const ulonglong2 Bv = Bt[k];
+        f2_t &h0 = h[2 * k], &h1 = h[2 * k + 1];
         const f2_t a0 = ex2_pair(f2_mul(A[2 * k], dt2)), a1 = ex2_pair(f2_mul(A[2 * k + 1], dt2));
         if (MODE == kBack) {
-          h[2 * k] = f2_mul(a0, f2_fma(Bv.x, x2, h[2 * k]));
-          h[2 * k + 1] = f2_mul(a1, f2_fma(Bv.y, x2, h[2 * k + 1]));
+          h0 = f2_mul(a0, f2_fma(Bv.x, x2, h0));
+          h1 = f2_mul(a1, f2_fma(Bv.y, x2, h1));
         } else {
-          h[2 * k] = f2_fma(a0, h[2 * k], f2_mul(Bv.x, x2));
-          h[2 * k + 1] = f2_fma(a1, h[2 * k + 1], f2_mul(Bv.y, x2));
+          h0 = f2_fma(a0, h0, f2_mul(Bv.x, x2));
+          h1 = f2_fma(a1, h1, f2_mul(Bv.y, x2));
         }
         if (MODE == kOut) {
           const ulonglong2 Cv = Ct[k];
-          y0 = f2_fma(h[2 * k], Cv.x, y0);
-          y1 = f2_fma(h[2 * k + 1], Cv.y, y1);
+          y0 = f2_fma(h0, Cv.x, y0);
+          y1 = f2_fma(h1, Cv.y, y1);
         }
       }
       if (MODE == kOut) {
-        const float2 v = f2_unpack(f2_add(y0, y1));
-        sx[t * 33 + lane] = v.x + v.y;
+        const float2 w = f2_unpack(f2_add(y0, y1));
+        sx[t * PITCH + lane] = w.x + w.y;
       }
     }
     if (MODE == kOut && p.y) {
+      fetch(p.u, p.us, x);
+      if (p.z) fetch(p.z, p.zs, z);
       __syncwarp();
-#pragma unroll 1
-      for (int j = 0; j < kSegs; ++j) {
+#pragma unroll
+      for (int j = 0; j < UNITS; ++j) {
         int ch, seg;
-        unit_of<32>(lane + 32 * j, p.by_channel, ch, seg);
+        unit_of<32, kSub / kK>(lane + 32 * j, p.by_channel, ch, seg);
         if (d0 + ch >= p.dim) continue;
         const int t = t0 + seg * kK, n = min(kK, p.seqlen - t), dc = d0 + ch;
-        float u[kK], z[kK], out[kK];
-        load_steps(static_cast<const T*>(p.u) + b * p.us[0] + dc * p.us[1] + t * p.us[2], p.us[2], p.vec, n, u);
-        if (p.z) load_steps(static_cast<const T*>(p.z) + b * p.zs[0] + dc * p.zs[1] + t * p.zs[2], p.zs[2], p.vec, n, z);
+        float out[kK];
         const f2_t D = dup(p.D ? p.D[dc] : 0.f);
 #pragma unroll
         for (int k = 0; k < kK; k += 2) {
-          const int at = (seg * kK + k) * 33 + ch;
-          f2_t v = f2_fma(D, f2_pack(u[k], u[k + 1]), f2_pack(sx[at], sx[at + 33]));
-          if (p.z) v = f2_mul(v, silu_of(f2_pack(z[k], z[k + 1])));
+          const int at = (seg * kK + k) * PITCH + ch;
+          f2_t v = f2_fma(D, f2_pack(raw_at(x[j], k), raw_at(x[j], k + 1)), f2_pack(sx[at], sx[at + PITCH]));
+          if (p.z) v = f2_mul(v, silu_of(f2_pack(raw_at(z[j], k), raw_at(z[j], k + 1))));
           const float2 w = f2_unpack(v);
           out[k] = w.x;
           out[k + 1] = w.y;
@@ -172,9 +192,9 @@ __global__ void __launch_bounds__(kWarps * 32) walk_kernel(const Params p) {
       }
     }
   }
+  if (MODE == kState) put(p.hlong, bl);
+  if (MODE == kBack) put(p.klong, bl);
   if (!mine) return;
-  if (MODE == kState) put(p.hlong + row);
-  if (MODE == kBack) put(p.klong + row);
   if (MODE != kOut) p.slong[bl * p.dim + d] = sum;
   if (MODE == kOut && p.state_out && l == p.longs - 1) {
     float* out = p.state_out + ((long long)b * p.dim + d) * p.dstate_n;
