@@ -11,6 +11,8 @@ be differentiated once, and equal calls give equal bits.
 from __future__ import annotations
 
 import ctypes
+import struct
+from array import array
 from dataclasses import dataclass
 
 import torch
@@ -20,6 +22,50 @@ from mamba_metal_b200 import _lib, ops
 from mamba_metal_b200.selective_scan import MAX_DSTATE, _scan_dtype
 
 CHECKPOINT8_BLOCK = 32  # values of a row that share an exponent (MM_CHECKPOINT8_BLOCK)
+
+
+# ---- calls -------------------------------------------------------------------------------------------------
+# A short call is bound by its host side, so arguments go into their struct in one piece (all fields are 8 bytes wide,
+# in the order of include/mamba_b200.h), and device and stream are looked up without the context managers' cost.
+
+_ZERO3 = (0, 0, 0)
+
+
+def _p(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _s3(t: torch.Tensor | None):
+    return _ZERO3 if t is None else t.stride()
+
+
+def _bits(x: float) -> int:
+    return struct.unpack("q", struct.pack("d", x))[0]
+
+
+def _args(cls, *values):
+    return cls.from_buffer(array("q", values))
+
+
+def _size(name: str, args) -> int:
+    n = ctypes.c_size_t(0)
+    _lib.check(getattr(_lib.lib(), name)(ctypes.byref(args), ctypes.byref(n)), name)
+    return n.value
+
+
+def _run(name: str, dev: torch.device, args, *rest) -> None:
+    fn, index = getattr(_lib.lib(), name), dev.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(ctypes.byref(args), *rest, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(ctypes.byref(args), *rest, stream)
+    _lib.check(rc, name)
+
+
+def _workspace(size_name: str, args, dev: torch.device) -> torch.Tensor:
+    return torch.empty(_size(size_name, args), dtype=torch.uint8, device=dev)
 
 
 def _by_channel(t: torch.Tensor) -> bool:
@@ -42,24 +88,25 @@ def _laid_out(t: torch.Tensor, by_channel: bool) -> torch.Tensor:
     return t if t.stride(2) == 1 else t.contiguous()
 
 
+def _cast(t: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor | None:
+    return t if t is None or t.dtype == dtype else t.detach().to(dtype)
+
+
 def _f32(t: torch.Tensor | None) -> torch.Tensor | None:
-    return None if t is None else t.detach().float().contiguous()
+    t = _cast(t, torch.float32)
+    return t if t is None or t.is_contiguous() else t.detach().contiguous()
 
 
 def _like(grad: torch.Tensor | None, t: torch.Tensor | None) -> torch.Tensor | None:
-    return None if t is None else grad.reshape(t.shape).to(t.dtype)
+    return None if t is None else _cast(grad if grad.shape == t.shape else grad.view(t.shape), t.dtype)
 
 
 # ---- 8-bit activation checkpoints --------------------------------------------------------------------------
 
 
 def _checkpoint_args(x, codes, exponents):
-    a = _lib.MMCheckpoint8Args()
-    a.x, a.codes, a.exponents = x.data_ptr(), codes.data_ptr(), exponents.data_ptr()
-    a.dtype = _lib.DTYPE_CODE[x.dtype]
-    a.batch, a.dim, a.length = x.shape
-    a.x_stride, a.codes_stride, a.exponents_stride = (_lib.strides3(t) for t in (x, codes, exponents))
-    return a
+    return _args(_lib.MMCheckpoint8Args, _p(x), _p(codes), _p(exponents), _lib.DTYPE_CODE[x.dtype], *x.shape, *x.stride(),
+                 *codes.stride(), *exponents.stride())
 
 
 def _checkpoint_buffers(shape, device, by_channel: bool):
@@ -100,10 +147,7 @@ class Checkpoint8:
         codes, exponents = _rows3(self.codes), _rows3(self.exponents)
         dev = _lib.require_cuda(codes, exponents)
         out = _empty(codes.shape, dtype, dev, _by_channel(codes))
-        with torch.cuda.device(dev):
-            rc = _lib.lib().mm_checkpoint8_unpack(ctypes.byref(_checkpoint_args(out, codes, exponents)),
-                                                  _lib.stream_handle(dev))
-        _lib.check(rc, "mm_checkpoint8_unpack")
+        _run("mm_checkpoint8_unpack", dev, _checkpoint_args(out, codes, exponents))
         return out.view(self.shape) if self.codes.dim() != 3 else out
 
 
@@ -125,10 +169,7 @@ def checkpoint8(x: torch.Tensor) -> Checkpoint8:
     dev = _lib.require_cuda(x)
     rows = _rows3(x.detach())
     codes, exponents = _checkpoint_buffers(rows.shape, dev, _by_channel(rows))
-    with torch.cuda.device(dev):
-        rc = _lib.lib().mm_checkpoint8_pack(ctypes.byref(_checkpoint_args(rows, codes, exponents)),
-                                            _lib.stream_handle(dev))
-    _lib.check(rc, "mm_checkpoint8_pack")
+    _run("mm_checkpoint8_pack", dev, _checkpoint_args(rows, codes, exponents))
     if x.dim() < 3:
         codes, exponents = codes[(0,) * (3 - x.dim())], exponents[(0,) * (3 - x.dim())]
     elif x.dim() > 3:
@@ -152,16 +193,9 @@ def conv1d_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
     by_channel = _by_channel(x)
     out = _empty(x.shape, x.dtype, dev, by_channel)
     codes, exponents = _checkpoint_buffers(x.shape, dev, by_channel)
-    a = _lib.MMConvCheckpointArgs()
-    a.x, a.weight, a.bias, a.out = x.data_ptr(), w.data_ptr(), _lib.ptr(b), out.data_ptr()
-    a.codes, a.exponents = codes.data_ptr(), exponents.data_ptr()
-    a.dtype = _lib.DTYPE_CODE[x.dtype]
-    a.batch, a.dim, a.seqlen, a.width = *x.shape, ops.D_CONV
-    a.x_stride, a.out_stride, a.codes_stride, a.exponents_stride = (_lib.strides3(t) for t in (x, out, codes, exponents))
-    a.silu = int(bool(silu))
-    with torch.cuda.device(dev):
-        rc = _lib.lib().mm_causal_conv1d_fwd_checkpoint8(ctypes.byref(a), _lib.stream_handle(dev))
-    _lib.check(rc, "mm_causal_conv1d_fwd_checkpoint8")
+    a = _args(_lib.MMConvCheckpointArgs, _p(x), _p(w), _p(b), _p(out), _p(codes), _p(exponents), _lib.DTYPE_CODE[x.dtype],
+              *x.shape, ops.D_CONV, *x.stride(), *out.stride(), *codes.stride(), *exponents.stride(), bool(silu))
+    _run("mm_causal_conv1d_fwd_checkpoint8", dev, a)
     return out, Checkpoint8(codes, exponents, x.dtype)
 
 
@@ -183,26 +217,12 @@ def causal_conv1d_backward(dout: torch.Tensor, x: torch.Tensor | Checkpoint8, we
     dx = _empty(src.shape, dout.dtype, dev, by_channel)
     dw = torch.empty((dim, ops.D_CONV), dtype=torch.float32, device=dev)
     db = torch.empty((dim,), dtype=torch.float32, device=dev)
-    a = _lib.MMConvBwdArgs()
-    if held:
-        a.codes, a.exponents = src.data_ptr(), x.exponents.data_ptr()
-        a.codes_stride, a.exponents_stride = _lib.strides3(src), _lib.strides3(x.exponents)
-    else:
-        a.x, a.x_stride = src.data_ptr(), _lib.strides3(src)
-    a.weight, a.bias, a.dout, a.dx = w.data_ptr(), _lib.ptr(b), dout.data_ptr(), dx.data_ptr()
-    a.dweight, a.dbias = dw.data_ptr(), db.data_ptr()
-    a.dtype = _lib.DTYPE_CODE[dout.dtype]
-    a.batch, a.dim, a.seqlen, a.width = batch, dim, seqlen, ops.D_CONV
-    a.dout_stride, a.dx_stride = _lib.strides3(dout), _lib.strides3(dx)
-    a.silu = int(bool(silu))
-    lib = _lib.lib()
-    nbytes = ctypes.c_size_t(0)
-    _lib.check(lib.mm_causal_conv1d_bwd_workspace_size(ctypes.byref(a), ctypes.byref(nbytes)),
-               "mm_causal_conv1d_bwd_workspace_size")
-    ws = torch.empty(int(nbytes.value), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.mm_causal_conv1d_bwd(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
-    _lib.check(rc, "mm_causal_conv1d_bwd")
+    a = _args(_lib.MMConvBwdArgs, 0 if held else _p(src), _p(src) if held else 0, _p(x.exponents) if held else 0, _p(w), _p(b),
+              _p(dout), _p(dx), _p(dw), _p(db), _lib.DTYPE_CODE[dout.dtype], batch, dim, seqlen, ops.D_CONV,
+              *(_ZERO3 if held else src.stride()), *(src.stride() if held else _ZERO3),
+              *(x.exponents.stride() if held else _ZERO3), *dout.stride(), *dx.stride(), bool(silu))
+    ws = _workspace("mm_causal_conv1d_bwd_workspace_size", a, dev)
+    _run("mm_causal_conv1d_bwd", dev, a, ws.data_ptr(), ws.numel())
     return dx, dw, db
 
 
@@ -276,25 +296,13 @@ def selective_scan_backward(dy: torch.Tensor, u, delta, A, B, C, *, D=None, z=No
     g = {"u": act(), "delta": act(), "z": None if z is None else act(), "A": f32(dim, n),
          "B": _empty(B.shape, u.dtype, dev, _by_channel(B)), "C": _empty(C.shape, u.dtype, dev, _by_channel(C)),
          "D": None if D is None else f32(dim), "delta_bias": None if delta_bias is None else f32(dim)}
-    a = _lib.MMScanBwdArgs()
-    _scan_args(u, delta, A, B, C, D, z, delta_bias, delta_softplus, a.fwd)
-    nbytes = ctypes.c_size_t(0)
-    lib = _lib.lib()
-    _lib.check(lib.mm_selective_scan_states_size(ctypes.byref(a.fwd), ctypes.byref(nbytes)),
-               "mm_selective_scan_states_size")
-    assert states.numel() * 4 == nbytes.value, "states of another call"
-    a.states = states.data_ptr()
-    a.dy, a.dstate = dy.data_ptr(), _lib.ptr(dstate)
-    a.du, a.ddelta, a.dA, a.dB, a.dC = (g[k].data_ptr() for k in ("u", "delta", "A", "B", "C"))
-    a.dD, a.dz, a.ddelta_bias = (_lib.ptr(g[k]) for k in ("D", "z", "delta_bias"))
-    a.dy_stride, a.du_stride, a.ddelta_stride, a.dz_stride, a.dB_stride, a.dC_stride = \
-        (_lib.strides3(t) for t in (dy, g["u"], g["delta"], g["z"], g["B"], g["C"]))
-    _lib.check(lib.mm_selective_scan_bwd_workspace_size(ctypes.byref(a), ctypes.byref(nbytes)),
-               "mm_selective_scan_bwd_workspace_size")
-    ws = torch.empty(int(nbytes.value), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.mm_selective_scan_bwd(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
-    _lib.check(rc, "mm_selective_scan_bwd")
+    f = _scan_args(u, delta, A, B, C, D, z, delta_bias, delta_softplus)
+    a = _args(_lib.MMScanBwdArgs, *f, _p(states), _p(dy), _p(dstate), *(_p(g[k]) for k in ("u", "delta", "A", "B", "C", "D", "z")),
+              _p(g["delta_bias"]), *dy.stride(), *g["u"].stride(), *g["delta"].stride(), *_s3(g["z"]), *g["B"].stride(),
+              *g["C"].stride())
+    assert states.numel() * 4 == _size("mm_selective_scan_states_size", a.fwd), "states of another call"
+    ws = _workspace("mm_selective_scan_bwd_workspace_size", a, dev)
+    _run("mm_selective_scan_bwd", dev, a, ws.data_ptr(), ws.numel())
     return g
 
 
@@ -318,32 +326,18 @@ def selective_scan_states(u, delta, A, B, C, *, D=None, z=None, delta_bias=None,
         raise TypeError(f"unsupported dtype {u.dtype}")
     y = _empty(u.shape, u.dtype, dev, _by_channel(u)) if outputs else None
     state = torch.empty((batch, dim, n), dtype=torch.float32, device=dev) if outputs else None
-    a = _scan_args(u, delta, A, B, C, D, z, delta_bias, delta_softplus)
-    a.y, a.y_stride, a.state_out = _lib.ptr(y), _lib.strides3(y), _lib.ptr(state)
-    lib = _lib.lib()
-    nbytes, wbytes = ctypes.c_size_t(0), ctypes.c_size_t(0)
-    _lib.check(lib.mm_selective_scan_states_size(ctypes.byref(a), ctypes.byref(nbytes)), "mm_selective_scan_states_size")
-    _lib.check(lib.mm_selective_scan_train_workspace_size(ctypes.byref(a), ctypes.byref(wbytes)),
-               "mm_selective_scan_train_workspace_size")
-    states = torch.empty(nbytes.value // 4, dtype=torch.float32, device=dev)
-    ws = torch.empty(wbytes.value, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.mm_selective_scan_train_fwd(ctypes.byref(a), states.data_ptr(), ws.data_ptr(), ws.numel(),
-                                             _lib.stream_handle(dev))
-    _lib.check(rc, "mm_selective_scan_train_fwd")
+    a = _args(_lib.MMScanArgs, *_scan_args(u, delta, A, B, C, D, z, delta_bias, delta_softplus, y, state))
+    states = torch.empty(_size("mm_selective_scan_states_size", a) // 4, dtype=torch.float32, device=dev)
+    ws = _workspace("mm_selective_scan_train_workspace_size", a, dev)
+    _run("mm_selective_scan_train_fwd", dev, a, states.data_ptr(), ws.data_ptr(), ws.numel())
     return y, state, states
 
 
-def _scan_args(u, delta, A, B, C, D, z, delta_bias, softplus, f=None):
-    f = _lib.MMScanArgs() if f is None else f
-    f.u, f.delta, f.A, f.B, f.C, f.D, f.z, f.delta_bias = (_lib.ptr(t) for t in (u, delta, A, B, C, D, z, delta_bias))
-    f.dtype = _lib.DTYPE_CODE[u.dtype]
-    f.batch, f.dim, f.seqlen = u.shape
-    f.dstate = A.shape[1]
-    f.u_stride, f.delta_stride, f.z_stride, f.B_stride, f.C_stride = (_lib.strides3(t) for t in (u, delta, z, B, C))
-    f.A_stride = (ctypes.c_int64 * 2)(*A.stride())
-    f.delta_softplus = int(bool(softplus))
-    return f
+def _scan_args(u, delta, A, B, C, D, z, delta_bias, softplus, y=None, state=None):
+    """The fields of MMScanArgs, in order."""
+    return (_p(u), _p(delta), _p(A), _p(B), _p(C), _p(D), _p(z), _p(y), _p(state), _lib.DTYPE_CODE[u.dtype], u.shape[0],
+            u.shape[1], A.shape[1], u.shape[2], *u.stride(), *delta.stride(), *_s3(z), *_s3(y), *B.stride(), *C.stride(),
+            *A.stride(), bool(softplus), 0, 0, _p(delta_bias))
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -351,14 +345,13 @@ class _SelectiveScan(torch.autograd.Function):
     def forward(ctx, u, delta, A, B, C, D, z, delta_bias, softplus):
         ctx.set_materialize_grads(False)
         dtype = _scan_dtype(u, delta, B, C, z)
-        cast = lambda t: None if t is None else t.detach().to(dtype)
-        uc, dc, Bc, Cc, zc = map(cast, (u, delta, B, C, z))
-        Af, Df, bf = A.detach().float(), _f32(D), _f32(delta_bias)
+        uc, dc, Bc, Cc, zc = (_cast(t, dtype) for t in (u, delta, B, C, z))
+        Af, Df, bf = _cast(A, torch.float32), _f32(D), _f32(delta_bias)
         y, state, states = selective_scan_states(uc, dc, Af, Bc, Cc, D=Df, z=zc, delta_bias=bf, delta_softplus=softplus)
         ctx.softplus = softplus
         ctx.dtypes = tuple(None if t is None else t.dtype for t in (u, delta, A, B, C, D, z, delta_bias))
         ctx.save_for_backward(uc, dc, Af, Bc, Cc, Df, zc, bf, states)
-        return y.to(u.dtype), state
+        return _cast(y, u.dtype), state
 
     @staticmethod
     @once_differentiable
@@ -366,11 +359,11 @@ class _SelectiveScan(torch.autograd.Function):
         u, delta, A, B, C, D, z, bias, states = ctx.saved_tensors
         if dy is None and dstate is None:
             return (None,) * 9
-        dy = torch.zeros_like(u) if dy is None else dy.to(u.dtype)
+        dy = torch.zeros_like(u) if dy is None else _cast(dy, u.dtype)
         g = selective_scan_backward(dy, u, delta, A, B, C, D=D, z=z, delta_bias=bias, delta_softplus=ctx.softplus,
                                     dstate=_f32(dstate), states=states)
         names = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")
-        return (*(None if t is None else g[k].to(t) for k, t in zip(names, ctx.dtypes)), None)
+        return (*(None if t is None else _cast(g[k], t) for k, t in zip(names, ctx.dtypes)), None)
 
 
 def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
@@ -406,22 +399,13 @@ class _PreferenceLoss(torch.autograd.Function):
         x = logits.detach()
         if vocab > 1 and x.stride(2) != 1:
             x = x.contiguous()
-        a = _lib.MMPreferenceArgs()
-        a.logits, a.labels, a.ref = x.data_ptr(), labels.data_ptr(), ref.data_ptr()
-        a.loss, a.chosen, a.rejected, a.stats, a.slope = (t.data_ptr() for t in (loss, chosen, rejected, stats, slope))
-        a.dtype = _lib.DTYPE_CODE[x.dtype]
-        a.pairs, a.length, a.vocab = pairs, length, vocab
-        a.logits_stride = (ctypes.c_int64 * 2)(*x.stride()[:2])
-        a.ignore_index, a.beta, a.smoothing = ignore_index, beta, smoothing
-        lib = _lib.lib()
-        nbytes = ctypes.c_size_t(0)
-        _lib.check(lib.mm_preference_loss_workspace_size(ctypes.byref(a), ctypes.byref(nbytes)),
-                   "mm_preference_loss_workspace_size")
-        ws = torch.empty(int(nbytes.value), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            rc = lib.mm_preference_loss_fwd(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
-        _lib.check(rc, "mm_preference_loss_fwd")
-        ctx.args = a
+        values = (_lib.DTYPE_CODE[x.dtype], pairs, length, vocab, *x.stride()[:2])
+        rest = (ignore_index, _bits(beta), _bits(smoothing))
+        a = _args(_lib.MMPreferenceArgs, _p(x), _p(labels), _p(ref), _p(loss), _p(chosen), _p(rejected), _p(stats), _p(slope), 0, 0,
+                  *values, 0, 0, *rest)
+        ws = _workspace("mm_preference_loss_workspace_size", a, dev)
+        _run("mm_preference_loss_fwd", dev, a, ws.data_ptr(), ws.numel())
+        ctx.args = values, rest
         ctx.save_for_backward(x, labels, stats, slope)
         ctx.mark_non_differentiable(chosen, rejected)
         return loss, chosen, rejected
@@ -432,15 +416,12 @@ class _PreferenceLoss(torch.autograd.Function):
         if grad_loss is None:
             return (None,) * 6
         x, labels, stats, slope = ctx.saved_tensors
-        grad = grad_loss.float().contiguous()
+        grad = _f32(grad_loss)
         dlogits = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        a = ctx.args
-        a.logits, a.labels, a.stats, a.slope = (t.data_ptr() for t in (x, labels, stats, slope))
-        a.grad_loss, a.dlogits = grad.data_ptr(), dlogits.data_ptr()
-        a.dlogits_stride = (ctypes.c_int64 * 2)(*dlogits.stride()[:2])
-        with torch.cuda.device(x.device):
-            rc = _lib.lib().mm_preference_loss_bwd(ctypes.byref(a), _lib.stream_handle(x.device))
-        _lib.check(rc, "mm_preference_loss_bwd")
+        values, rest = ctx.args
+        a = _args(_lib.MMPreferenceArgs, _p(x), _p(labels), 0, 0, 0, 0, _p(stats), _p(slope), _p(grad), _p(dlogits), *values,
+                  *dlogits.stride()[:2], *rest)
+        _run("mm_preference_loss_bwd", x.device, a)
         return dlogits, None, None, None, None, None
 
 
