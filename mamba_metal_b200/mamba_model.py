@@ -119,6 +119,19 @@ class MambaModel(nn.Module):
         """input_ids: (B, L) -> logits (B, L, vocab_size)."""
         return self._stack(input_ids, "forward")[0]
 
+    def forward_train(self, input_ids: torch.Tensor, checkpoint8: bool = True) -> torch.Tensor:
+        """``forward`` with gradients for all parameters: input_ids (B, L) -> logits (B, L, vocab_size). With
+        ``checkpoint8`` every block holds the activations that its backward pass needs in 8 bits."""
+        from mamba_metal_b200 import training
+
+        eps = self.cfg.rms_norm_eps
+        residual = self.embeddings(input_ids).float()
+        for layer in self.layers:
+            h = training.rms_norm(residual, layer.norm.weight, eps, self.dtype)
+            residual = residual + layer.mixer.forward_train(h, checkpoint8)
+        h = training.rms_norm(residual, self.norm_f.weight, eps, self.dtype)
+        return F.linear(h, self.embeddings.weight)
+
     def init_state(self, batch_size: int = 1):
         """Zero float32 conv and SSM state per layer (mamba_model.py:80-91)."""
         dev = self.embeddings.weight.device

@@ -16,6 +16,7 @@ from array import array
 from dataclasses import dataclass
 
 import torch
+import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from mamba_metal_b200 import _lib, ops
@@ -447,3 +448,120 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
     _lib.require_cuda(logits, labels, ref_logps)
     return _PreferenceLoss.apply(logits, labels.contiguous(), _f32(ref_logps), float(beta), float(label_smoothing),
                                  int(ignore_index))
+
+
+# ---- a Mamba block ---------------------------------------------------------------------------------------------
+
+
+def _proj(w: torch.Tensor, a: torch.Tensor) -> torch.Tensor:
+    """w (out, c) applied to the channels of a (batch, c, time), in a's layout."""
+    return F.linear(a.transpose(1, 2), w).transpose(1, 2) if _by_channel(a) else torch.matmul(w, a)
+
+
+def _outer(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """sum over batch and time of a (batch, i, time) times b (batch, j, time): (i, j), one product over all tokens."""
+    i, j = a.shape[1], b.shape[1]
+    if _by_channel(a) and _by_channel(b):
+        return a.transpose(1, 2).reshape(-1, i).t() @ b.transpose(1, 2).reshape(-1, j)
+    return a.transpose(0, 1).reshape(i, -1) @ b.transpose(0, 1).reshape(j, -1).t()
+
+
+class _Block(torch.autograd.Function):
+    """MambaBlock.forward that keeps its activations (its input, the conv's, the gate, the scan's output) in 8 bits and
+    computes the rest again in the backward pass, from the values they stand for."""
+
+    @staticmethod
+    def forward(ctx, x, in_w, conv_w, conv_b, x_w, dt_w, dt_b, A_log, D, out_w, by_channel):
+        E, R, N = conv_w.shape[0], dt_w.shape[1], A_log.shape[1]
+        dtype = in_w.dtype
+        xt = _cast(x, dtype).transpose(1, 2)
+        xt = _laid_out(xt, by_channel)
+        xz = _proj(in_w, xt)
+        xc, cx = conv1d_checkpoint8(xz[:, :E], conv_w, conv_b)
+        x_dbl = _proj(x_w, xc)
+        dt = _proj(dt_w, x_dbl[:, :R])
+        A, Df, bf = -torch.exp(A_log.float()), _f32(D), _f32(dt_b)
+        y, _, _ = selective_scan_states(xc, dt, A, x_dbl[:, R:R + N], x_dbl[:, R + N:], D=Df, z=xz[:, E:], delta_bias=bf,
+                                        delta_softplus=True)
+        out = _proj(out_w, y).transpose(1, 2)
+        held = [cx, checkpoint8(xt), checkpoint8(xz[:, E:]), checkpoint8(y)]
+        ctx.x_dtype = x.dtype
+        ctx.save_for_backward(x_dbl, in_w, conv_w, conv_b, x_w, dt_w, dt_b, A_log, D, out_w,
+                              *(t for c in held for t in (c.codes, c.exponents)))
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x_dbl, in_w, conv_w, conv_b, x_w, dt_w, dt_b, A_log, D, out_w, *held = ctx.saved_tensors
+        E, R, N = conv_w.shape[0], dt_w.shape[1], A_log.shape[1]
+        dtype = in_w.dtype
+        cx, cxt, cz, cy = (Checkpoint8(held[2 * i], held[2 * i + 1], dtype) for i in range(4))
+        by_channel = _by_channel(cx.codes)
+        xt, z, y = cxt.restore(), cz.restore(), cy.restore()
+        xc = _empty(z.shape, dtype, z.device, by_channel)
+        ops.causal_conv1d(cx.restore(), conv_w, conv_b, silu=True, out=xc)
+        A, Df, bf = -torch.exp(A_log.float()), _f32(D), _f32(dt_b)
+        dt = _proj(dt_w, x_dbl[:, :R])
+        do = _laid_out(_cast(dout, dtype).transpose(1, 2), by_channel)
+        d_out_w = _outer(do, y)
+        g = selective_scan_backward(_proj(out_w.t(), do), xc, dt, A, x_dbl[:, R:R + N], x_dbl[:, R + N:], D=Df, z=z,
+                                    delta_bias=bf, delta_softplus=True)
+        d_dt_w = _outer(g["delta"], x_dbl[:, :R])
+        d_dbl = _laid_out(torch.cat([_proj(dt_w.t(), g["delta"]), g["B"], g["C"]], 1), by_channel)
+        d_x_w = _outer(d_dbl, xc)
+        dx_in, dw, db = causal_conv1d_backward(g["u"] + _proj(x_w.t(), d_dbl), cx, conv_w, conv_b)
+        dxz = _laid_out(torch.cat([dx_in, g["z"]], 1), by_channel)
+        d_in_w = _outer(dxz, xt)
+        dx = _proj(in_w.t(), dxz).transpose(1, 2)
+        return (_cast(dx, ctx.x_dtype), d_in_w, _like(dw, conv_w), _like(db, conv_b), d_x_w, d_dt_w, _like(g["delta_bias"], dt_b),
+                _cast(g["A"] * A, A_log.dtype), _like(g["D"], D), d_out_w, None)
+
+
+def mamba_block(block, x: torch.Tensor, checkpoint8: bool = True) -> torch.Tensor:
+    """Differentiable ``MambaBlock`` forward: x (batch, length, d_model) to the same, with gradients for x and all of the
+    block's parameters (``MambaBlock.forward_train`` calls it). With ``checkpoint8`` the activations that the
+    backward pass needs are held in 8 bits, about 1.03 bytes an element of its input, the conv's input, the gate and
+    the scan's output; without it autograd holds them, and every intermediate, as they are."""
+    if block.tp_reduce is not None:
+        raise ValueError("tensor-parallel blocks have no training pass")
+    _lib.require_cuda(x, block.in_proj.weight)
+    E, R, N = block.d_inner, block.dt_rank, block.d_state
+    # as in the inference pass: rows along time where they are 16-byte aligned, else along channels
+    by_channel = (x.shape[1] * block.in_proj.weight.dtype.itemsize) % 16 != 0 and x.shape[1] > 1
+    if checkpoint8:
+        return _Block.apply(x, block.in_proj.weight, block.conv1d.weight, block.conv1d.bias, block.x_proj.weight,
+                            block.dt_proj.weight, block.dt_proj.bias, block.A_log, block.D, block.out_proj.weight, by_channel)
+    xz = _proj(block.in_proj.weight, _laid_out(x.to(block.in_proj.weight.dtype).transpose(1, 2), by_channel))
+    xc = causal_conv1d(xz[:, :E], block.conv1d.weight, block.conv1d.bias)
+    x_dbl = _proj(block.x_proj.weight, xc)
+    y = selective_scan(xc, _proj(block.dt_proj.weight, x_dbl[:, :R]), -torch.exp(block.A_log.float()), x_dbl[:, R:R + N],
+                       x_dbl[:, R + N:], D=block.D, z=xz[:, E:], delta_bias=block.dt_proj.bias, delta_softplus=True)
+    return _proj(block.out_proj.weight, y).transpose(1, 2)
+
+
+class _RMSNorm(torch.autograd.Function):
+    """The package's RMSNorm over the last axis of a float32 tensor, result in ``dtype``; the gradient in float32."""
+
+    @staticmethod
+    def forward(ctx, x, weight, eps, dtype):
+        ctx.save_for_backward(x, weight)
+        ctx.eps = eps
+        return ops.add_rmsnorm(x.contiguous(), None, weight, eps, dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight = ctx.saved_tensors
+        r = torch.rsqrt((x * x).mean(-1, keepdim=True) + ctx.eps)
+        unit, g = x * r, g.float()
+        dw = (g * unit).flatten(0, -2).sum(0)
+        g = g * weight
+        return r * (g - unit * (g * unit).mean(-1, keepdim=True)), dw, None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, dtype: torch.dtype) -> torch.Tensor:
+    """Differentiable RMSNorm of a float32 ``x`` over its last axis, in ``dtype``."""
+    assert x.dtype == torch.float32 and weight.dtype == torch.float32 and tuple(weight.shape) == tuple(x.shape[-1:])
+    _lib.require_cuda(x, weight)
+    return _RMSNorm.apply(x, weight, eps, dtype)
