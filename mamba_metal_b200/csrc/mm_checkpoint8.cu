@@ -15,9 +15,10 @@ struct Params {
 };
 
 // Time contiguous: a lane takes 8 consecutive values, so four lanes share a block and agree on its maximum by
-// two shuffles. VEC: 16-byte accesses of x and 8-byte ones of codes. A warp covers CPT * 256 values of one row, with
-// all its loads in flight before the first is used (bf16 10240 x 32768: CPT 4 against 1).
-template <typename T, bool PACK, bool VEC, int CPT>
+// two shuffles. A warp covers CPT * 256 values of one row, with all its loads in flight before the first is used
+// (bf16 10240 x 32768, packed and restored: CPT 1 625 us, CPT 4 374). ACCESS: that of x; codes are taken by 8-byte words
+// but for kAnyStride.
+template <typename T, bool PACK, int ACCESS, int CPT>
 __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per_row) {
   const int lane = threadIdx.x & 31;
   const long long gw = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -33,7 +34,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
       const int t = begin + j * 256;
-      raw[j] = raw_load(x + t * p.xs[2], p.xs[2], VEC, min(8, p.length - t));
+      raw[j] = raw_load(x + t * p.xs[2], p.xs[2], ACCESS, min(8, p.length - t));
     }
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
@@ -50,7 +51,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per
       int c[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) c[k] = ck_code(raw_at(raw[j], k), inv);
-      if (VEC && n == 8) {
+      if (ACCESS != kAnyStride && n == 8) {
         __stcs(reinterpret_cast<uint2*>(codes + t), make_uint2(ck_pack4(c[0], c[1], c[2], c[3]), ck_pack4(c[4], c[5], c[6], c[7])));
       } else {
 #pragma unroll
@@ -66,24 +67,23 @@ __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per
       const int t = begin + j * 256;
       if (t >= p.length) continue;
       scale[j] = ck_scale(exps[(long long)(t / kCkBlock) * p.es[2]]);
-      if (VEC && t + 8 <= p.length) raw[j] = __ldcs(reinterpret_cast<const uint2*>(codes + t));
+      if (ACCESS != kAnyStride && t + 8 <= p.length) raw[j] = __ldcs(reinterpret_cast<const uint2*>(codes + t));
     }
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
       const int t = begin + j * 256, n = min(8, p.length - t);
-      if (VEC && n == 8) {
-        float v[8];
+      float v[8];
+      if (ACCESS != kAnyStride && n == 8) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           v[k] = ck_restore<T>(ck_byte(raw[j].x, k), scale[j]);
           v[k + 4] = ck_restore<T>(ck_byte(raw[j].y, k), scale[j]);
         }
-        ck_store8<T>(x + t, v);
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < n) st_f32(x + (t + k) * p.xs[2], ck_restore<T>(codes[(t + k) * p.cs[2]], scale[j]));
+        for (int k = 0; k < 8; ++k) v[k] = k < n ? ck_restore<T>(codes[(t + k) * p.cs[2]], scale[j]) : 0.f;
       }
+      row_store(x + t * p.xs[2], p.xs[2], ACCESS, n, v);
     }
   }
 }
@@ -144,15 +144,21 @@ template <typename T, bool PACK> int launch(const MMCheckpoint8Args* a, cudaStre
     const int wpr = (int)((a->length + (few ? 255 : 1023)) / (few ? 256 : 1024));
     const long long grid = (p.rows * wpr + 7) / 8;
     if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
-    const bool vec = (p.xs[2] == 1 && p.cs[2] == 1) &&
-                     ck_rows_aligned(a->x, a->x_stride, a->batch, a->dim, (int)sizeof(T), 16) &&
-                     ck_rows_aligned(a->codes, a->codes_stride, a->batch, a->dim, 1, 8);
-    if (vec)
-      few ? rows_kernel<T, PACK, true, 1><<<(unsigned)grid, 256, 0, s>>>(p, wpr)
-          : rows_kernel<T, PACK, true, 4><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
-    else
-      few ? rows_kernel<T, PACK, false, 1><<<(unsigned)grid, 256, 0, s>>>(p, wpr)
-          : rows_kernel<T, PACK, false, 4><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
+    Access access = ck_access(a->x, a->x_stride, a->batch, a->dim, a->length, (int)sizeof(T));
+    if ((a->length > 1 && p.cs[2] != 1) || !ck_rows_aligned(a->codes, a->codes_stride, a->batch, a->dim, 1, 8)) access = kAnyStride;
+    switch (access) {
+      case kAligned:
+        few ? rows_kernel<T, PACK, kAligned, 1><<<(unsigned)grid, 256, 0, s>>>(p, wpr)
+            : rows_kernel<T, PACK, kAligned, 4><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
+        break;
+      case kContiguous:
+        few ? rows_kernel<T, PACK, kContiguous, 1><<<(unsigned)grid, 256, 0, s>>>(p, wpr)
+            : rows_kernel<T, PACK, kContiguous, 4><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
+        break;
+      default:
+        few ? rows_kernel<T, PACK, kAnyStride, 1><<<(unsigned)grid, 256, 0, s>>>(p, wpr)
+            : rows_kernel<T, PACK, kAnyStride, 4><<<(unsigned)grid, 256, 0, s>>>(p, wpr);
+    }
   }
   return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
 }

@@ -43,20 +43,15 @@ template <typename T> MM_DEV float ck_restore(int code, float scale) {
   return v > CkMax<T>::v ? CkMax<T>::v : v < -CkMax<T>::v ? -CkMax<T>::v : v;  // NaN passes both
 }
 
-template <typename T> MM_DEV void ck_store8(T* p, const float (&v)[8]) {
-#pragma unroll
-  for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
-    uint4 a;
-    constexpr int pairs = 8 / (int)sizeof(T);
-#pragma unroll
-    for (int k = 0; k < pairs; ++k) vec_set_pair<T>(a, k, v[2 * (h * pairs + k)], v[2 * (h * pairs + k) + 1]);
-    __stcs(reinterpret_cast<uint4*>(p) + h, a);
-  }
-}
-
 inline bool ck_rows_aligned(const void* p, const int64_t* st, int64_t batch, int64_t dim, int elem, int align) {
   return (reinterpret_cast<uintptr_t>(p) % align) == 0 && (batch <= 1 || (st[0] * elem) % align == 0) &&
          (dim <= 1 || (st[1] * elem) % align == 0);
+}
+
+// Access of a tensor's rows (contiguous along time where n of them have more than one step)
+inline Access ck_access(const void* p, const int64_t* st, int64_t batch, int64_t dim, int64_t steps, int elem) {
+  if (steps > 1 && st[2] != 1) return kAnyStride;
+  return ck_rows_aligned(p, st, batch, dim, elem, 16) ? kAligned : kContiguous;
 }
 
 }  // namespace mm

@@ -210,15 +210,51 @@ template <> MM_DEV void vec_set<__nv_bfloat16>(uint4& v, int k, float x) {
   u4_set_word(v, k >> 1, (k & 1) ? ((w & 0xffffu) | (h << 16)) : ((w & 0xffff0000u) | h));
 }
 
+// ---- Rows of eight values a lane, at any alignment ----------------------------------------------------
+// How a tensor's rows may be accessed: by elements at any stride; contiguous, by aligned 16-byte words that are
+// shifted together; aligned, by 16-byte words.
+enum Access { kAnyStride = 0, kContiguous = 1, kAligned = 2 };
+
 // Eight values of a row as they lie in memory
 template <typename T> struct Raw8 {
   uint4 v[sizeof(T) / 2];
 };
-template <typename T> MM_DEV Raw8<T> raw_load(const T* p, long long s, bool vec, int n) {
+// W words that begin `bytes` (0 .. 15) into c
+template <int W> MM_DEV void shift_words(const unsigned (&c)[W + 4], int bytes, unsigned (&x)[W]) {
+  unsigned a[W + 2], b[W + 1];
+#pragma unroll
+  for (int i = 0; i < W + 2; ++i) a[i] = (bytes & 8) ? c[i + 2] : c[i];
+#pragma unroll
+  for (int i = 0; i < W + 1; ++i) b[i] = (bytes & 4) ? a[i + 1] : a[i];
+#pragma unroll
+  for (int i = 0; i < W; ++i) x[i] = __funnelshift_r(b[i], b[i + 1], (bytes & 3) * 8);
+}
+// Every aligned word that is read holds a byte of the eight values, so nothing outside their pages is touched.
+template <typename T> MM_DEV Raw8<T> raw_load_shifted(const T* p) {
+  constexpr int W = 2 * sizeof(T);
+  const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+  const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - off);
+  unsigned c[W + 4], x[W];
+#pragma unroll
+  for (int h = 0; h < W / 4 + 1; ++h) {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (h < W / 4 || off) w = q[h];
+    c[4 * h] = w.x, c[4 * h + 1] = w.y, c[4 * h + 2] = w.z, c[4 * h + 3] = w.w;
+  }
+  shift_words<W>(c, off, x);
   Raw8<T> r;
-  if (vec && n == 8) {
+#pragma unroll
+  for (int h = 0; h < W / 4; ++h) r.v[h] = make_uint4(x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]);
+  return r;
+}
+// n of the eight exist; the others are 0
+template <typename T> MM_DEV Raw8<T> raw_load(const T* p, long long s, int access, int n) {
+  Raw8<T> r;
+  if (access == kAligned && n == 8) {
 #pragma unroll
     for (int h = 0; h < (int)sizeof(T) / 2; ++h) r.v[h] = __ldcs(reinterpret_cast<const uint4*>(p) + h);
+  } else if (access == kContiguous && n == 8) {
+    r = raw_load_shifted(p);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -228,6 +264,69 @@ template <typename T> MM_DEV Raw8<T> raw_load(const T* p, long long s, bool vec,
 }
 template <typename T> MM_DEV float raw_at(const Raw8<T>& r, int k) {
   return vec_elem<T>(r.v[k * sizeof(T) / 16], k % (16 / (int)sizeof(T)));
+}
+template <typename T> MM_DEV Raw8<T> raw_pack(const float (&v)[8]) {
+  Raw8<T> r;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    vec_set_pair<T>(r.v[2 * k * sizeof(T) / 16], k % (8 / (int)sizeof(T)), v[2 * k], v[2 * k + 1]);
+  return r;
+}
+
+// Stores eight values a lane, consecutive over the lanes of a full warp (all of which call it), n of each lane's (all 8
+// but in the row's last lanes, none after it). Contiguous rows: a lane stores the aligned words that end with or
+// inside its values, the first of which begins with the end of its neighbour's.
+template <typename T> MM_DEV void row_store(T* p, long long s, int access, int n, const float (&v)[8]) {
+  constexpr int E = 16 / (int)sizeof(T), W = 2 * sizeof(T);
+  const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+  if (access == kAnyStride || (access == kContiguous && off == 0) || access == kAligned) {
+    if (access != kAnyStride && n == 8) {
+      const Raw8<T> r = raw_pack<T>(v);
+#pragma unroll
+      for (int h = 0; h < W / 4; ++h) __stcs(reinterpret_cast<uint4*>(p) + h, r.v[h]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < n) st_f32(p + k * s, v[k]);
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 31, before = __shfl_up_sync(0xffffffffu, n, 1), head = E - off / (int)sizeof(T);
+  const Raw8<T> r = raw_pack<T>(v);
+  unsigned c[W + 4], x[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) c[i + 4] = u4_word(r.v[i / 4], i % 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = __shfl_up_sync(0xffffffffu, c[W + i], 1);
+  shift_words<W>(c, 16 - off, x);
+  uint4* q = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(p) - off);
+  if (lane > 0 && before == 8 && n >= head) {
+    __stcs(q, make_uint4(x[0], x[1], x[2], x[3]));
+  } else {
+    uint4 w;
+    u4_set_word(w, 0, c[0]), u4_set_word(w, 1, c[1]), u4_set_word(w, 2, c[2]), u4_set_word(w, 3, c[3]);
+#pragma unroll
+    for (int k = 0; k < E; ++k)  // the neighbour's values 8 - E + k
+      if (lane > 0 && k >= head && 8 - E + k < before) st_f32(p + (k - E), vec_elem<T>(w, k));
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+      if (k < head && k < n) st_f32(p + k, v[k]);
+  }
+#pragma unroll
+  for (int h = 1; h < W / 4; ++h) {
+    if (n >= head + h * E) {
+      __stcs(q + h, make_uint4(x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k >= head + (h - 1) * E && k < head + h * E && k < n) st_f32(p + k, v[k]);
+    }
+  }
+  if (lane == 31) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k >= head + (W / 4 - 1) * E && k < n) st_f32(p + k, v[k]);
+  }
 }
 
 // ---- cp.async (LDGSTS) staging --------------------------------------------------------------------

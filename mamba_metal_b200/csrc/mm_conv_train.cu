@@ -8,6 +8,8 @@
 // kernel adds the partials in a fixed order.
 #include "mm_checkpoint8.cuh"
 
+#include <type_traits>
+
 namespace mm {
 namespace convt {
 
@@ -61,7 +63,7 @@ MM_DEV f2_t taps(const f2_t (&w)[kW], f2_t bias, f2_t a, f2_t b, f2_t c, f2_t d)
 // 8x1536x4096 f16 against CPT 1). Halos come from the neighbouring lanes, and for the warp's first and last lane
 // from memory.
 
-template <typename T, bool VEC, int CPT>
+template <typename T, int ACCESS, int CPT>
 __global__ void __launch_bounds__(256) fwd_rows_kernel(const Params p, int warps_per_row) {
   const int lane = threadIdx.x & 31;
   const long long gw = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -75,7 +77,7 @@ __global__ void __launch_bounds__(256) fwd_rows_kernel(const Params p, int warps
 #pragma unroll
   for (int j = 0; j < CPT; ++j) {
     const int t = begin + j * 256 + lane * kE;
-    x[j] = raw_load(xr + (long long)t * p.xs[2], p.xs[2], VEC, min(kE, p.seqlen - t));
+    x[j] = raw_load(xr + (long long)t * p.xs[2], p.xs[2], ACCESS, min(kE, p.seqlen - t));
   }
   float before[3];  // the three steps before the warp's chunk
 #pragma unroll
@@ -102,16 +104,15 @@ __global__ void __launch_bounds__(256) fwd_rows_kernel(const Params p, int warps
     }
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    if (n <= 0) continue;
     float o[kE];
 #pragma unroll
     for (int k = 0; k < kE; ++k)
       o[k] = act(fmaf(w.w, win[k + 3], fmaf(w.z, win[k + 2], fmaf(w.y, win[k + 1], fmaf(w.x, win[k], bb)))), p.silu);
     const unsigned byte = ck_exponent(m);
     const float inv = ck_inverse_scale(byte);
-    if ((lane & 3) == 0) p.exps_out[b * p.es[0] + d * p.es[1] + (long long)(t0 / kCkBlock) * p.es[2]] = (uint8_t)byte;
-    if (VEC && n == kE) {
-      ck_store8<T>(orow + t0, o);
+    if ((lane & 3) == 0 && n > 0) p.exps_out[b * p.es[0] + d * p.es[1] + (long long)(t0 / kCkBlock) * p.es[2]] = (uint8_t)byte;
+    row_store(orow + (long long)t0 * p.os[2], p.os[2], ACCESS, n, o);
+    if (ACCESS != kAnyStride && n == kE) {
       uint2 c;
       c.x = ck_pack4(ck_code(win[3], inv), ck_code(win[4], inv), ck_code(win[5], inv), ck_code(win[6], inv));
       c.y = ck_pack4(ck_code(win[7], inv), ck_code(win[8], inv), ck_code(win[9], inv), ck_code(win[10], inv));
@@ -119,10 +120,7 @@ __global__ void __launch_bounds__(256) fwd_rows_kernel(const Params p, int warps
     } else {
 #pragma unroll
       for (int k = 0; k < kE; ++k)
-        if (k < n) {
-          st_f32(orow + (long long)(t0 + k) * p.os[2], o[k]);
-          crow[(long long)(t0 + k) * p.cs[2]] = (int8_t)ck_code(win[k + 3], inv);
-        }
+        if (k < n) crow[(long long)(t0 + k) * p.cs[2]] = (int8_t)ck_code(win[k + 3], inv);
     }
   }
 }
@@ -154,12 +152,12 @@ template <typename T, bool CK> struct Source {
     float scale;
     MM_DEV float at(int k) const { return CK ? (float)ck_byte(k < 4 ? c.x : c.y, k & 3) * scale : raw_at(x, k); }
   };
-  MM_DEV Eight load(int t0, bool vec, int n) const {
+  MM_DEV Eight load(int t0, int access, int n) const {
     Eight r = {};
     if (!CK) {
-      r.x = raw_load(x + (long long)t0 * xs, xs, vec, n);
+      r.x = raw_load(x + (long long)t0 * xs, xs, access, n);
     } else if (n > 0) {
-      if (vec && n == kE) {
+      if (access != kAnyStride && n == kE) {
         r.c = __ldcs(reinterpret_cast<const uint2*>(codes + t0));
       } else {
         int v[kE];
@@ -174,7 +172,7 @@ template <typename T, bool CK> struct Source {
 };
 
 // The chunks from the last to the first, so that the three dpre after a chunk are known
-template <typename T, bool CK, bool VEC, int CPT>
+template <typename T, bool CK, int ACCESS, int CPT>
 __global__ void __launch_bounds__(256) bwd_rows_kernel(const Params p, int warps_per_row) {
   const int lane = threadIdx.x & 31;
   const long long gw = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -190,8 +188,8 @@ __global__ void __launch_bounds__(256) bwd_rows_kernel(const Params p, int warps
 #pragma unroll
   for (int j = 0; j < CPT; ++j) {
     const int t = begin + j * 256 + lane * kE, n = min(kE, p.seqlen - t);
-    x[j] = src.load(t, VEC, n);
-    g[j] = raw_load(grow + (long long)t * p.gs[2], p.gs[2], VEC, n);
+    x[j] = src.load(t, ACCESS, n);
+    g[j] = raw_load(grow + (long long)t * p.gs[2], p.gs[2], ACCESS, n);
   }
   float before[3], after[3];  // x before the warp's steps; dpre of the three steps that follow the chunk at hand
   const float4 w = *reinterpret_cast<const float4*>(p.w + (long long)d * kW);
@@ -240,13 +238,7 @@ __global__ void __launch_bounds__(256) bwd_rows_kernel(const Params p, int warps
 #pragma unroll
     for (int k = 0; k < kE; ++k)
       o[k] = fmaf(w.w, dp[k], fmaf(w.z, dp[k + 1], fmaf(w.y, dp[k + 2], w.x * dp[k + 3])));
-    if (VEC && n == kE) {
-      ck_store8<T>(orow + t0, o);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kE; ++k)
-        if (k < n) st_f32(orow + (long long)(t0 + k) * p.os[2], o[k]);
-    }
+    row_store(orow + (long long)t0 * p.os[2], p.os[2], ACCESS, n, o);
   }
 #pragma unroll
   for (int j = 0; j < kSums; ++j)
@@ -335,25 +327,30 @@ template <int C, bool VEC> MM_DEV void store_bytes(void* q, long long s, int n, 
   }
 }
 
+// Channels of a thread: d, d + step, ..; neighbours by words of 8 bytes, or, where those do not fit the rows, 32 apart so
+// that a warp's elements are side by side (bf16 4x5119x5601, forward and backward: by fours 1156 us).
 struct Walk {
-  int b, d, t0, t1, run, n;  // n: channels of this thread that exist
+  int b, d, step, t0, t1, run, n;  // n: channels of this thread that exist
 };
-template <int C> MM_DEV bool walk_of(const Params& p, int run, int runs, Walk& k) {
-  const int cg = (p.dim + C - 1) / C;
+template <int C, bool VEC> __host__ __device__ inline int walkers(int dim) { return VEC ? (dim + C - 1) / C : (dim + 32 * C - 1) / (32 * C) * 32; }
+template <int C, bool VEC> MM_DEV bool walk_of(const Params& p, int run, int runs, Walk& k) {
+  const int cg = walkers<C, VEC>(p.dim);
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= (long long)p.batch * runs * cg) return false;
-  k.d = (int)(i % cg) * C;
+  const int j = (int)(i % cg);
+  k.step = VEC ? 1 : 32;
+  k.d = VEC ? j * C : j / 32 * 32 * C + j % 32;
   k.run = (int)(i / cg % runs);
   k.b = (int)(i / cg / runs);
   k.t0 = k.run * run;
   k.t1 = min(p.seqlen, k.t0 + run);
-  k.n = min(C, p.dim - k.d);
-  return true;
+  k.n = VEC ? min(C, p.dim - k.d) : min(C, (p.dim - k.d + 31) / 32);
+  return k.n > 0;
 }
 template <int C> MM_DEV void load_weights(const Params& p, const Walk& k, f2_t (&w)[C / 2][kW], f2_t (&bb)[C / 2]) {
 #pragma unroll
   for (int c = 0; c < C / 2; ++c) {
-    const int d = min(k.d + 2 * c, p.dim - 1), e = min(k.d + 2 * c + 1, p.dim - 1);
+    const int d = min(k.d + 2 * c * k.step, p.dim - 1), e = min(k.d + (2 * c + 1) * k.step, p.dim - 1);
     const float4 v = *reinterpret_cast<const float4*>(p.w + (long long)d * kW);
     const float4 u = *reinterpret_cast<const float4*>(p.w + (long long)e * kW);
     w[c][0] = f2_pack(v.x, u.x), w[c][1] = f2_pack(v.y, u.y), w[c][2] = f2_pack(v.z, u.z), w[c][3] = f2_pack(v.w, u.w);
@@ -365,7 +362,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int run, int runs) {
   constexpr int C = kC<T>, H = C / 2;
   Walk k;
-  if (!walk_of<C>(p, run, runs, k)) return;
+  if (!walk_of<C, VEC>(p, run, runs, k)) return;
   const T* x = static_cast<const T*>(p.x) + k.b * p.xs[0] + k.d * p.xs[1];
   T* out = static_cast<T*>(p.out) + k.b * p.os[0] + k.d * p.os[1];
   int8_t* codes = p.codes_out + k.b * p.cs[0] + k.d * p.cs[1];
@@ -376,7 +373,7 @@ __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int ru
   for (int j = 0; j < 3; ++j) {
 #pragma unroll
     for (int c = 0; c < H; ++c) win[j][c] = both(0.f);
-    if (k.t0 > 0) load_few<T, VEC>(x + (long long)(k.t0 - 3 + j) * p.xs[2], p.xs[1], k.n, win[j]);
+    if (k.t0 > 0) load_few<T, VEC>(x + (long long)(k.t0 - 3 + j) * p.xs[2], k.step * p.xs[1], k.n, win[j]);
   }
   // Twice over each block: for its maxima, then, out of L1, for everything else. (Holding the block in registers
   // instead leaves 8 warps an SM: bf16 4x5120x5601 255 us.)
@@ -389,7 +386,7 @@ __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int ru
 #pragma unroll 8
     for (int i = 0; i < n; ++i) {
       f2_t v[H];
-      load_few<T, VEC>(xb + i * p.xs[2], p.xs[1], k.n, v);
+      load_few<T, VEC>(xb + i * p.xs[2], k.step * p.xs[1], k.n, v);
 #pragma unroll
       for (int c = 0; c < H; ++c) {
         const float2 q = f2_unpack(v[c]);
@@ -405,11 +402,11 @@ __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int ru
       inv[c] = ck_inverse_scale(byte);
       bytes |= byte << (8 * c);
     }
-    store_bytes<C, false>(exps + (long long)(tb / kCkBlock) * p.es[2], p.es[1], k.n, bytes);
+    store_bytes<C, false>(exps + (long long)(tb / kCkBlock) * p.es[2], k.step * p.es[1], k.n, bytes);
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
       f2_t v[H], o[H];
-      load_few<T, VEC>(xb + i * p.xs[2], p.xs[1], k.n, v);
+      load_few<T, VEC>(xb + i * p.xs[2], k.step * p.xs[1], k.n, v);
       unsigned code = 0;
 #pragma unroll
       for (int c = 0; c < H; ++c) {
@@ -421,8 +418,8 @@ __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int ru
         win[1][c] = win[2][c];
         win[2][c] = v[c];
       }
-      store_few<T, VEC>(out + (long long)(tb + i) * p.os[2], p.os[1], k.n, o);
-      store_bytes<C, VEC>(codes + (long long)(tb + i) * p.cs[2], p.cs[1], k.n, code);
+      store_few<T, VEC>(out + (long long)(tb + i) * p.os[2], k.step * p.os[1], k.n, o);
+      store_bytes<C, VEC>(codes + (long long)(tb + i) * p.cs[2], k.step * p.cs[1], k.n, code);
     }
   }
 }
@@ -435,7 +432,7 @@ __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int
     constexpr int C = kC<T>, H = C / 2, kU = 8;
   static_assert(kU > 3 && kCkBlock % kU == 0, "from the second group on, step t - 3 is the run's own");
   Walk k;
-  if (!walk_of<C>(p, run, runs, k)) return;
+  if (!walk_of<C, VEC>(p, run, runs, k)) return;
   const T* x = CK ? nullptr : static_cast<const T*>(p.x) + k.b * p.xs[0] + k.d * p.xs[1];
   const int8_t* codes = CK ? p.codes + k.b * p.cs[0] + k.d * p.cs[1] : nullptr;
   const uint8_t* exps = CK ? p.exps + k.b * p.es[0] + k.d * p.es[1] : nullptr;
@@ -444,12 +441,12 @@ __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int
   f2_t w[H][kW], bb[H], win[3][H], dp[3][H], sum[kSums][H], scale[H];
   load_weights<C>(p, k, w, bb);
   auto scales = [&](int t) {  // of the block that holds step t
-    const unsigned e = load_bytes<C, false>(exps + (long long)(t / kCkBlock) * p.es[2], p.es[1], k.n);
+    const unsigned e = load_bytes<C, false>(exps + (long long)(t / kCkBlock) * p.es[2], k.step * p.es[1], k.n);
 #pragma unroll
     for (int c = 0; c < H; ++c)
       scale[c] = f2_pack(ck_scale((e >> (16 * c)) & 0xff), ck_scale((e >> (16 * c + 8)) & 0xff));
   };
-  auto code_row = [&](int t) { return load_bytes<C, VEC>(codes + (long long)t * p.cs[2], p.cs[1], k.n); };
+  auto code_row = [&](int t) { return load_bytes<C, VEC>(codes + (long long)t * p.cs[2], k.step * p.cs[1], k.n); };
   auto value = [&](unsigned v, int c) {
     return f2_mul(f2_pack((float)ck_byte(v, 2 * c), (float)ck_byte(v, 2 * c + 1)), scale[c]);
   };
@@ -464,7 +461,7 @@ __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int
 #pragma unroll
         for (int c = 0; c < H; ++c) win[j][c] = value(v, c);
       } else {
-        load_few<T, VEC>(x + (long long)(k.t0 - 3 + j) * p.xs[2], p.xs[1], k.n, win[j]);
+        load_few<T, VEC>(x + (long long)(k.t0 - 3 + j) * p.xs[2], k.step * p.xs[1], k.n, win[j]);
       }
     }
   }
@@ -480,8 +477,8 @@ __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int
     if (CK)
       code[i] = code_row(t);
     else
-      v[i] = fetch_few<T, VEC>(x + (long long)t * p.xs[2], p.xs[1], k.n);
-    g[i] = fetch_few<T, VEC>(dout + (long long)t * p.gs[2], p.gs[1], k.n);
+      v[i] = fetch_few<T, VEC>(x + (long long)t * p.xs[2], k.step * p.xs[1], k.n);
+    g[i] = fetch_few<T, VEC>(dout + (long long)t * p.gs[2], k.step * p.gs[1], k.n);
   };
   auto fetch_some = [&](int i, int t) {
     code[i] = 0;
@@ -518,7 +515,7 @@ __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int
       dp[1][c] = dp[2][c];
       dp[2][c] = q;
     }
-    if (inside || (t - 3 >= k.t0 && t < k.t1 + 3)) store_few<T, VEC>(dx + (long long)(t - 3) * p.os[2], p.os[1], k.n, o);
+    if (inside || (t - 3 >= k.t0 && t < k.t1 + 3)) store_few<T, VEC>(dx + (long long)(t - 3) * p.os[2], k.step * p.os[1], k.n, o);
   };
 #pragma unroll
   for (int i = 0; i < kU; ++i) fetch_some(i, k.t0 + i);
@@ -538,8 +535,8 @@ __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int
 #pragma unroll
     for (int j = 0; j < kSums; ++j) {
       const float2 v = f2_unpack(sum[j][c]);
-      if (2 * c < k.n) out[2 * c * kSums + j] = v.x;
-      if (2 * c + 1 < k.n) out[(2 * c + 1) * kSums + j] = v.y;
+      if (2 * c < k.n) out[2 * c * k.step * kSums + j] = v.x;
+      if (2 * c + 1 < k.n) out[(2 * c + 1) * k.step * kSums + j] = v.y;
     }
 }
 
@@ -587,6 +584,15 @@ inline Plan make_plan(int64_t dtype, int64_t batch, int64_t dim, int64_t seqlen,
   return pl;
 }
 
+inline Access least(Access a, Access b) { return a < b ? a : b; }
+// run(std::integral_constant<int, access>)
+template <typename F> void with_access(Access access, F run) {
+  switch (access) {
+    case kAligned: return run(std::integral_constant<int, kAligned>{});
+    case kContiguous: return run(std::integral_constant<int, kContiguous>{});
+    default: return run(std::integral_constant<int, kAnyStride>{});
+  }
+}
 inline bool unit(const int64_t* st, int64_t n, int i) { return n <= 1 || st[i] == 1; }
 
 inline int check(int64_t dtype, int64_t batch, int64_t dim, int64_t seqlen, int64_t width) {
@@ -632,25 +638,27 @@ template <typename T> int launch_fwd(const MMConvCheckpointArgs* a, cudaStream_t
   const Plan pl = make_plan(a->dtype, a->batch, a->dim, a->seqlen, all_columns(a->dim, a->seqlen, st, 3));
   const int es = (int)sizeof(T);
   if (pl.columns) {
-    const long long threads = a->batch * pl.parts * ((a->dim + kC<T> - 1) / kC<T>), grid = (threads + 255) / 256;
+    const bool vec = columns_aligned(a->x, a->x_stride, a->dim, es, kC<T>) &&
+                     columns_aligned(a->out, a->out_stride, a->dim, es, kC<T>) &&
+                     columns_aligned(a->codes, a->codes_stride, a->dim, 1, kC<T>);
+    const long long per = vec ? walkers<kC<T>, true>((int)a->dim) : walkers<kC<T>, false>((int)a->dim);
+    const long long grid = (a->batch * pl.parts * per + 255) / 256;
     if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
-    if (columns_aligned(a->x, a->x_stride, a->dim, es, kC<T>) && columns_aligned(a->out, a->out_stride, a->dim, es, kC<T>) &&
-        columns_aligned(a->codes, a->codes_stride, a->dim, 1, kC<T>))
-      fwd_columns_kernel<T, true><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts);
-    else
-      fwd_columns_kernel<T, false><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts);
+    vec ? fwd_columns_kernel<T, true><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts)
+        : fwd_columns_kernel<T, false><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts);
   } else {
     const long long grid = (a->batch * a->dim * pl.parts + 7) / 8;
     if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
-    if (unit(a->x_stride, a->seqlen, 2) && unit(a->out_stride, a->seqlen, 2) && unit(a->codes_stride, a->seqlen, 2) &&
-        ck_rows_aligned(a->x, a->x_stride, a->batch, a->dim, es, 16) &&
-        ck_rows_aligned(a->out, a->out_stride, a->batch, a->dim, es, 16) &&
-        ck_rows_aligned(a->codes, a->codes_stride, a->batch, a->dim, 1, 8))
-      pl.run == 256 ? fwd_rows_kernel<T, true, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
-                    : fwd_rows_kernel<T, true, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
-    else
-      pl.run == 256 ? fwd_rows_kernel<T, false, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
-                    : fwd_rows_kernel<T, false, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
+    Access access = least(ck_access(a->x, a->x_stride, a->batch, a->dim, a->seqlen, es),
+                          ck_access(a->out, a->out_stride, a->batch, a->dim, a->seqlen, es));
+    if (!unit(a->codes_stride, a->seqlen, 2) || !ck_rows_aligned(a->codes, a->codes_stride, a->batch, a->dim, 1, 8))
+      access = kAnyStride;
+    auto run = [&](auto level) {
+      constexpr int A = decltype(level)::value;
+      pl.run == 256 ? fwd_rows_kernel<T, A, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
+                    : fwd_rows_kernel<T, A, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
+    };
+    with_access(access, run);
   }
   return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
 }
@@ -682,27 +690,29 @@ template <typename T, bool CK> int launch_bwd(const MMConvBwdArgs* a, float* par
   const Plan pl = bwd_plan(a);
   const int es = (int)sizeof(T);
   if (pl.columns) {
-    const long long threads = a->batch * pl.parts * ((a->dim + kC<T> - 1) / kC<T>), grid = (threads + 255) / 256;
+    const bool src = CK ? columns_aligned(a->codes, a->codes_stride, a->dim, 1, kC<T>)
+                        : columns_aligned(a->x, a->x_stride, a->dim, es, kC<T>);
+    const bool vec = src && columns_aligned(a->dout, a->dout_stride, a->dim, es, kC<T>) &&
+                     columns_aligned(a->dx, a->dx_stride, a->dim, es, kC<T>);
+    const long long per = vec ? walkers<kC<T>, true>((int)a->dim) : walkers<kC<T>, false>((int)a->dim);
+    const long long grid = (a->batch * pl.parts * per + 255) / 256;
     if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
-    const bool src = CK ? columns_aligned(a->codes, a->codes_stride, a->dim, 1, kC<T>) : columns_aligned(a->x, a->x_stride, a->dim, es, kC<T>);
-    if (src && columns_aligned(a->dout, a->dout_stride, a->dim, es, kC<T>) && columns_aligned(a->dx, a->dx_stride, a->dim, es, kC<T>))
-      bwd_columns_kernel<T, CK, true><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts);
-    else
-      bwd_columns_kernel<T, CK, false><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts);
+    vec ? bwd_columns_kernel<T, CK, true><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts)
+        : bwd_columns_kernel<T, CK, false><<<(unsigned)grid, 256, 0, s>>>(p, pl.run, pl.parts);
   } else {
     const long long grid = (a->batch * a->dim * pl.parts + 7) / 8;
     if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
-    const int64_t* ss = CK ? a->codes_stride : a->x_stride;
-    const bool src = CK ? ck_rows_aligned(a->codes, a->codes_stride, a->batch, a->dim, 1, 8)
-                        : ck_rows_aligned(a->x, a->x_stride, a->batch, a->dim, es, 16);
-    if (src && unit(ss, a->seqlen, 2) && unit(a->dout_stride, a->seqlen, 2) && unit(a->dx_stride, a->seqlen, 2) &&
-        ck_rows_aligned(a->dout, a->dout_stride, a->batch, a->dim, es, 16) &&
-        ck_rows_aligned(a->dx, a->dx_stride, a->batch, a->dim, es, 16))
-      pl.run == 256 ? bwd_rows_kernel<T, CK, true, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
-                    : bwd_rows_kernel<T, CK, true, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
-    else
-      pl.run == 256 ? bwd_rows_kernel<T, CK, false, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
-                    : bwd_rows_kernel<T, CK, false, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
+    Access access = least(ck_access(a->dout, a->dout_stride, a->batch, a->dim, a->seqlen, es),
+                          ck_access(a->dx, a->dx_stride, a->batch, a->dim, a->seqlen, es));
+    if (!CK) access = least(access, ck_access(a->x, a->x_stride, a->batch, a->dim, a->seqlen, es));
+    if (CK && (!unit(a->codes_stride, a->seqlen, 2) || !ck_rows_aligned(a->codes, a->codes_stride, a->batch, a->dim, 1, 8)))
+      access = kAnyStride;
+    auto run = [&](auto level) {
+      constexpr int A = decltype(level)::value;
+      pl.run == 256 ? bwd_rows_kernel<T, CK, A, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
+                    : bwd_rows_kernel<T, CK, A, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
+    };
+    with_access(access, run);
   }
   if (cudaGetLastError() != cudaSuccess) return MM_ERR_LAUNCH;
   sum_kernel<<<(unsigned)((a->dim * kSums + 31) / 32), 256, 0, s>>>(part, a->batch * pl.parts, (int)a->dim, a->dweight,

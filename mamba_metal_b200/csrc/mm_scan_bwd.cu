@@ -23,10 +23,10 @@ struct Raw {
 };
 template <typename T, bool HAS_Z> MM_DEV void load_unit(const Params& p, int b, int d, int t, Raw& r) {
   const int n = min(kK, p.seqlen - t);
-  load_steps(static_cast<const T*>(p.delta) + b * p.ds[0] + d * p.ds[1] + t * p.ds[2], p.ds[2], p.vec, n, r.dt);
-  load_steps(static_cast<const T*>(p.u) + b * p.us[0] + d * p.us[1] + t * p.us[2], p.us[2], p.vec, n, r.u);
-  load_steps(static_cast<const T*>(p.dy) + b * p.ys[0] + d * p.ys[1] + t * p.ys[2], p.ys[2], p.vec, n, r.e);
-  if (HAS_Z) load_steps(static_cast<const T*>(p.z) + b * p.zs[0] + d * p.zs[1] + t * p.zs[2], p.zs[2], p.vec, n, r.g);
+  load_steps(static_cast<const T*>(p.delta) + b * p.ds[0] + d * p.ds[1] + t * p.ds[2], p.ds[2], p.access, n, r.dt);
+  load_steps(static_cast<const T*>(p.u) + b * p.us[0] + d * p.us[1] + t * p.us[2], p.us[2], p.access, n, r.u);
+  load_steps(static_cast<const T*>(p.dy) + b * p.ys[0] + d * p.ys[1] + t * p.ys[2], p.ys[2], p.access, n, r.e);
+  if (HAS_Z) load_steps(static_cast<const T*>(p.z) + b * p.zs[0] + d * p.zs[1] + t * p.zs[2], p.zs[2], p.access, n, r.g);
 }
 
 // d, d u and e (zeros where there are no steps: a = 1 there, so states and k pass through)
@@ -281,7 +281,7 @@ MM_DEV void finish_unit(const Params& p, int b, int d, int t, int seg, const Raw
     sum = f2_fma(e[k], f2_pack(r.u[2 * k], r.u[2 * k + 1]), sum);
   }
   sumD = f2_unpack(sum).x + f2_unpack(sum).y;
-  store_steps(static_cast<T*>(p.du) + b * p.dus[0] + d * p.dus[1] + t * p.dus[2], p.dus[2], p.vec, n, out);
+  store_steps(static_cast<T*>(p.du) + b * p.dus[0] + d * p.dus[1] + t * p.dus[2], p.dus[2], p.access, n, out);
   fetch_unit(rec + R::s2, seg, x);
 #pragma unroll
   for (int k = 0; k < kK / 2; ++k)
@@ -290,14 +290,14 @@ MM_DEV void finish_unit(const Params& p, int b, int d, int t, int seg, const Raw
   sumb = 0.f;
 #pragma unroll
   for (int k = 0; k < kK; ++k) sumb += k < n ? out[k] : 0.f;
-  store_steps(static_cast<T*>(p.ddelta) + b * p.dds[0] + d * p.dds[1] + t * p.dds[2], p.dds[2], p.vec, n, out);
+  store_steps(static_cast<T*>(p.ddelta) + b * p.dds[0] + d * p.dds[1] + t * p.dds[2], p.dds[2], p.access, n, out);
   if (HAS_Z) {
     fetch_unit(rec + R::s3, seg, x);
 #pragma unroll
     for (int k = 0; k < kK / 2; ++k)
       put(k, f2_mul(f2_mul(f2_pack(r.e[2 * k], r.e[2 * k + 1]), f2_fma(D, f2_pack(r.u[2 * k], r.u[2 * k + 1]), x[k])),
                     silu_slope(f2_pack(r.g[2 * k], r.g[2 * k + 1]))));
-    store_steps(static_cast<T*>(p.dz) + b * p.dzs[0] + d * p.dzs[1] + t * p.dzs[2], p.dzs[2], p.vec, n, out);
+    store_steps(static_cast<T*>(p.dz) + b * p.dzs[0] + d * p.dzs[1] + t * p.dzs[2], p.dzs[2], p.access, n, out);
   }
 }
 
@@ -367,11 +367,11 @@ MM_DEV void load_unit(const Params& p, int b, int d, int t, Raw& r, const T* raw
     return;
   }
   const T* x = raw + (p.by_channel ? seg * kK * kTile<T> + ch : ch * kT + seg * kK);
-  const int st = p.by_channel ? kTile<T> : 1;
-  load_steps(x, st, !p.by_channel, kK, r.dt);
-  load_steps(x + kRawOne<T>, st, !p.by_channel, kK, r.u);
-  load_steps(x + 2 * kRawOne<T>, st, !p.by_channel, kK, r.e);
-  if (HAS_Z) load_steps(x + 3 * kRawOne<T>, st, !p.by_channel, kK, r.g);
+  const int st = p.by_channel ? kTile<T> : 1, access = p.by_channel ? kAnyStride : kAligned;
+  load_steps(x, st, access, kK, r.dt);
+  load_steps(x + kRawOne<T>, st, access, kK, r.u);
+  load_steps(x + 2 * kRawOne<T>, st, access, kK, r.e);
+  if (HAS_Z) load_steps(x + 3 * kRawOne<T>, st, access, kK, r.g);
 }
 
 template <typename T, bool HAS_Z>
@@ -739,16 +739,16 @@ extern "C" int mm_selective_scan_bwd(const MMScanBwdArgs* a, void* workspace, si
   copy3(p.dzs, a->dz_stride);
   copy3(p.dBs, a->dB_stride);
   copy3(p.dCs, a->dC_stride);
-  p.vec = rows_aligned(f.u, f.u_stride, f) && rows_aligned(f.delta, f.delta_stride, f) &&
-          rows_aligned(a->dy, a->dy_stride, f) && rows_aligned(a->du, a->du_stride, f) &&
-          rows_aligned(a->ddelta, a->ddelta_stride, f) &&
-          (!f.z || (rows_aligned(f.z, f.z_stride, f) && rows_aligned(a->dz, a->dz_stride, f)));
-  p.by_channel = !p.vec && f.u_stride[1] == 1 && f.u_stride[2] != 1;
+  Access access = least(access_of(f.u, f.u_stride, f), access_of(f.delta, f.delta_stride, f));
+  access = least(access, least(access_of(a->dy, a->dy_stride, f), access_of(a->du, a->du_stride, f)));
+  access = least(access, access_of(a->ddelta, a->ddelta_stride, f));
+  if (f.z) access = least(access, least(access_of(f.z, f.z_stride, f), access_of(a->dz, a->dz_stride, f)));
+  set_access(p, access, f);
   const void* act[4] = {f.u, f.delta, a->dy, f.z};
   const int64_t* act_stride[4] = {f.u_stride, f.delta_stride, a->dy_stride, f.z_stride};
   p.ahead = 1;
   for (int i = 0; i < (f.z ? 4 : 3); ++i)
-    if (!(p.by_channel ? columns_aligned(act[i], act_stride[i], f) : rows_aligned(act[i], act_stride[i], f))) p.ahead = 0;
+    if (!(p.by_channel ? columns_aligned(act[i], act_stride[i], f) : access_of(act[i], act_stride[i], f) == kAligned)) p.ahead = 0;
   p.passes = l.passes;
   p.groups = l.groups;
   p.tiles = l.tiles;

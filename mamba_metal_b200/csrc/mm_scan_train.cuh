@@ -20,7 +20,7 @@ struct Params {
   long long dus[3], dds[3], dzs[3], dBs[3], dCs[3];
   int batch, dim, dstate_n, seqlen;
   int softplus;
-  int vec;         // every activation's rows are contiguous in time and 16-byte aligned
+  int access;      // of the activations' rows along time: the least that any of them allows
   int by_channel;  // u is contiguous along channels
   int ahead;       // grad_kernel copies its raw inputs ahead: all contiguous along one axis, rows 16-byte aligned
   int np;          // states, rounded up to a multiple of four: rows of the buffers below
@@ -87,8 +87,8 @@ MM_DEV f2_t step_slope(f2_t raw, int softplus) {
 }
 
 // Eight consecutive steps of one channel; n of them exist
-template <typename T> MM_DEV void load_steps(const T* p, long long s, bool vec, int n, float (&v)[kK]) {
-  if (vec && n == kK) {
+template <typename T> MM_DEV void load_steps(const T* p, long long s, int access, int n, float (&v)[kK]) {
+  if (access == kAligned && n == kK) {
 #pragma unroll
     for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
       const uint4 a = *(reinterpret_cast<const uint4*>(p) + h);
@@ -100,20 +100,33 @@ template <typename T> MM_DEV void load_steps(const T* p, long long s, bool vec, 
         v[2 * (h * pairs + k) + 1] = q.y;
       }
     }
+  } else if (access == kContiguous && n == kK) {
+    const Raw8<T> r = raw_load_shifted(p);
+#pragma unroll
+    for (int k = 0; k < kK; ++k) v[k] = raw_at(r, k);
   } else {
 #pragma unroll
     for (int k = 0; k < kK; ++k) v[k] = k < n ? ld_f32(p + k * s) : 0.f;
   }
 }
-template <typename T> MM_DEV void store_steps(T* p, long long s, bool vec, int n, const float (&v)[kK]) {
-  if (vec && n == kK) {
+template <typename T> MM_DEV void store_steps(T* p, long long s, int access, int n, const float (&v)[kK]) {
+  if (access == kAligned && n == kK) {
+    const Raw8<T> r = raw_pack<T>(v);
 #pragma unroll
-    for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
-      uint4 a;
-      constexpr int pairs = 8 / (int)sizeof(T);
+    for (int h = 0; h < (int)sizeof(T) / 2; ++h) __stcs(reinterpret_cast<uint4*>(p) + h, r.v[h]);
+  } else if (sizeof(T) == 2 && access == kContiguous && n == kK) {
+    // by words of 4 bytes; from an odd element on, one element, three words, one element
+    const Raw8<T> r = raw_pack<T>(v);
+    unsigned* q = reinterpret_cast<unsigned*>(p);
+    if (reinterpret_cast<uintptr_t>(p) & 2) {
+      q = reinterpret_cast<unsigned*>(p + 1);
+      st_f32(p, v[0]);
 #pragma unroll
-      for (int k = 0; k < pairs; ++k) vec_set_pair<T>(a, k, v[2 * (h * pairs + k)], v[2 * (h * pairs + k) + 1]);
-      __stcs(reinterpret_cast<uint4*>(p) + h, a);
+      for (int k = 0; k < 3; ++k) q[k] = __funnelshift_r(u4_word(r.v[0], k), u4_word(r.v[0], k + 1), 16);
+      st_f32(p + kK - 1, v[kK - 1]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) q[k] = u4_word(r.v[0], k);
     }
   } else {
 #pragma unroll
@@ -155,9 +168,17 @@ MM_DEV float4 load_BC(const T* base, const long long (&st)[3], int b, int n0, in
 inline void copy3(long long (&to)[3], const int64_t* from) {
   for (int i = 0; i < 3; ++i) to[i] = from[i];
 }
-inline bool rows_aligned(const void* q, const int64_t* st, const MMScanArgs& f) {
+inline Access access_of(const void* q, const int64_t* st, const MMScanArgs& f) {
   const int es = dtype_size(f.dtype);
-  return aligned16(q) && st[2] == 1 && (f.batch <= 1 || st[0] * es % 16 == 0) && (f.dim <= 1 || st[1] * es % 16 == 0);
+  if (f.seqlen > 1 && st[2] != 1) return kAnyStride;
+  return aligned16(q) && (f.batch <= 1 || st[0] * es % 16 == 0) && (f.dim <= 1 || st[1] * es % 16 == 0) ? kAligned : kContiguous;
+}
+inline Access least(Access a, Access b) { return a < b ? a : b; }
+// float32's contiguous rows off a 16-byte boundary go element by element: the shifted words' registers cost
+// grad_kernel more (f32 8x1536x2047: 1.26 ms, by elements 0.99)
+inline void set_access(Params& p, Access access, const MMScanArgs& f) {
+  p.access = access == kContiguous && f.dtype == MM_F32 ? kAnyStride : access;
+  p.by_channel = access == kAnyStride && f.u_stride[1] == 1;
 }
 inline int chunks_of(const MMScanArgs& f) { return (int)((f.seqlen + kT - 1) / kT); }
 // Chunks of a long one: four; fewer where that leaves an SM less than twelve warps of 32 channels to walk them

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kWarps * 32, NM <= 16 ? 4 : NM <= 32 ? 3 : 2) 
         int ch, seg;
         unit_of<32, kSub / kK>(lane + 32 * j, p.by_channel, ch, seg);
         const int t = t0 + seg * kK, n = d0 + ch < p.dim ? min(kK, p.seqlen - t) : 0;
-        r[j] = raw_load(static_cast<const T*>(base) + b * st[0] + (d0 + ch) * st[1] + t * st[2], st[2], p.vec, n);
+        r[j] = raw_load(static_cast<const T*>(base) + b * st[0] + (d0 + ch) * st[1] + t * st[2], st[2], p.access, n);
       }
     };
     fetch(p.delta, p.ds, raw);
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kWarps * 32, NM <= 16 ? 4 : NM <= 32 ? 3 : 2) 
           out[k] = w.x;
           out[k + 1] = w.y;
         }
-        store_steps(static_cast<T*>(p.y) + b * p.ys[0] + dc * p.ys[1] + t * p.ys[2], p.ys[2], p.vec, n, out);
+        store_steps(static_cast<T*>(p.y) + b * p.ys[0] + dc * p.ys[1] + t * p.ys[2], p.ys[2], p.access, n, out);
       }
     }
   }
@@ -333,9 +333,10 @@ extern "C" int mm_selective_scan_train_fwd(const MMScanArgs* a, float* states, v
   p.y = a->y;
   p.state_out = a->state_out;
   copy3(p.ys, a->y_stride);
-  p.vec = rows_aligned(a->u, a->u_stride, *a) && rows_aligned(a->delta, a->delta_stride, *a) &&
-          (!a->y || rows_aligned(a->y, a->y_stride, *a)) && (!a->z || rows_aligned(a->z, a->z_stride, *a));
-  p.by_channel = !p.vec && a->u_stride[1] == 1 && a->u_stride[2] != 1;
+  Access access = least(access_of(a->u, a->u_stride, *a), access_of(a->delta, a->delta_stride, *a));
+  if (a->y) access = least(access, access_of(a->y, a->y_stride, *a));
+  if (a->z) access = least(access, access_of(a->z, a->z_stride, *a));
+  set_access(p, access, *a);
   p.hst = p.chunks > 1 ? states : nullptr;
   p.hlong = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.hlong);
   p.slong = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.slong);

@@ -202,6 +202,38 @@ def test_scan_gradient_repeats_and_other_streams():
         assert torch.equal(first[k], second[k]), k
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("first", [0, 1, 2, 3, 5, 7])
+def test_rows_at_any_alignment(first, dtype):
+    """Views whose rows begin at every place inside an aligned word, with the neighbours of the views left alone."""
+    b, d, n = 2, 5, 301
+    g = torch.Generator().manual_seed(first)
+    big = randn(g, b, d, n + 16).to(dtype).to(DEV)
+    x = big[..., first:first + n]
+    c = training.checkpoint8(x)
+    values, exponents = checkpoint_ref(x.double().cpu())
+    assert np.array_equal(c.exponents.cpu().numpy(), exponents)
+    out = torch.full((b, d, n + 16), 7.0, dtype=dtype, device=DEV)
+    view = out[..., first:first + n]
+    a = training._checkpoint_args(view, c.codes, c.exponents)
+    training._run("mm_checkpoint8_unpack", view.device, a)
+    assert np.array_equal(view.double().cpu().numpy(), values)
+    assert (out[..., :first] == 7).all() and (out[..., first + n:] == 7).all()
+    w = torch.randn(d, 4, device=DEV)
+    whole = x.contiguous()
+    y, held = training.conv1d_checkpoint8(x, w, None)
+    z, same = training.conv1d_checkpoint8(whole, w, None)
+    assert torch.equal(y, z) and torch.equal(held.codes, same.codes)
+    for p, q in zip(training.causal_conv1d_backward(x, x, w, None), training.causal_conv1d_backward(whole, whole, w, None)):
+        assert torch.equal(p, q)
+    A = -torch.rand(d, 4, device=DEV)
+    B = torch.randn(b, 4, n, device=DEV, dtype=dtype)
+    left = training.selective_scan_backward(x, x, x, A, B, B, z=x, delta_softplus=True)
+    right = training.selective_scan_backward(whole, whole, whole, A, B, B, z=whole, delta_softplus=True)
+    for k in ("u", "delta", "A", "B", "C", "z"):
+        assert torch.equal(left[k], right[k]), k
+
+
 def test_empty_sequences():
     u = torch.empty(2, 3, 0, device=DEV, requires_grad=True)
     A = torch.full((3, 4), -1.0, device=DEV, requires_grad=True)
@@ -242,7 +274,8 @@ def checkpoint_ref(x):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("layout", LAYOUTS)
-@pytest.mark.parametrize("shape", [(1, 1, 1), (2, 3, 31), (1, 5, 32), (2, 7, 33), (1, 40, 256), (3, 6, 1000)])
+@pytest.mark.parametrize("shape", [(1, 1, 1), (2, 3, 31), (1, 5, 32), (2, 7, 33), (1, 40, 256), (3, 6, 1000), (2, 3, 2309),
+                                   (1, 9, 1025)])
 def test_checkpoint(shape, layout, dtype):
     g = torch.Generator().manual_seed(sum(shape))
     x, ref = put(randn(g, *shape) * torch.exp(3 * randn(g, shape[0], shape[1], 1)), dtype, layout)
@@ -298,7 +331,8 @@ def conv_ref(x, w, bias, silu):
 @pytest.mark.parametrize("held", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("layout", LAYOUTS)
-@pytest.mark.parametrize("shape", [(1, 1, 1), (2, 3, 2), (1, 5, 4), (2, 8, 33), (1, 66, 256), (2, 7, 259), (1, 24, 1032)])
+@pytest.mark.parametrize("shape", [(1, 1, 1), (2, 3, 2), (1, 5, 4), (2, 8, 33), (1, 66, 256), (2, 7, 259), (1, 24, 1032),
+                                   (2, 3, 2309), (1, 9, 1025), (1, 300, 70)])
 def test_conv_gradient(shape, layout, dtype, held):
     b, d, n = shape
     silu, with_bias = n != 4, d != 3
