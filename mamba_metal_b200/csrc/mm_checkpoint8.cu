@@ -83,7 +83,10 @@ __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = k < n ? ck_restore<T>(codes[(t + k) * p.cs[2]], scale[j]) : 0.f;
       }
-      row_store(x + t * p.xs[2], p.xs[2], ACCESS, n, v);
+      if (ACCESS == kAligned && n == 8)
+        row_store(x + t, 1, ACCESS, 8, v);
+      else
+        row_store(x + t * p.xs[2], p.xs[2], ACCESS, n, v);
     }
   }
 }
