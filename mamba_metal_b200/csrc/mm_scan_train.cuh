@@ -181,10 +181,12 @@ inline void set_access(Params& p, Access access, const MMScanArgs& f) {
   p.by_channel = access == kAnyStride && f.u_stride[1] == 1;
 }
 inline int chunks_of(const MMScanArgs& f) { return (int)((f.seqlen + kT - 1) / kT); }
-// Chunks of a long one: four; fewer where that leaves an SM less than twelve warps of 32 channels to walk them
+// Chunks of a long one: four; fewer where that leaves an SM less than twelve warps of 32 channels to walk them. Two chunks
+// are always one long chunk, which needs no joining: three launches fewer for the same device time (bf16 1x1536x48
+// forward and backward 51 us, split 54; 1x1536x64 60, split 56; three or four chunks lose: 1x1536x128 100, split 58).
 inline int per_long_of(const MMScanArgs& f) {
   int n = 4;
-  while (n > 1 && f.batch * ((f.dim + 31) / 32) * ((chunks_of(f) + n - 1) / n) < 12 * 148) n /= 2;
+  while (chunks_of(f) > 2 && n > 1 && f.batch * ((f.dim + 31) / 32) * ((chunks_of(f) + n - 1) / n) < 12 * 148) n /= 2;
   return n;
 }
 inline int longs_of(const MMScanArgs& f) { return (chunks_of(f) + per_long_of(f) - 1) / per_long_of(f); }

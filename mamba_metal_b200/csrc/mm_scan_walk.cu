@@ -243,7 +243,8 @@ template <int MODE, typename T, int NM> int launch_walk(const Params& p, cudaStr
   const long long items = (long long)p.batch * p.longs * ((p.dim + 31) / 32), grid = (items + kWarps - 1) / kWarps;
   if (grid > 0x7fffffffLL) return MM_ERR_SHAPE;
   constexpr int smem = kWarps * ((kWarpFloats<MODE, NM> + 3) / 4 * 4) * (int)sizeof(float);
-  if (cudaFuncSetAttribute(walk_kernel<MODE, T, NM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(walk_kernel<MODE, T, NM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return MM_ERR_LAUNCH;
   walk_kernel<MODE, T, NM><<<(unsigned)grid, kWarps * 32, smem, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
@@ -285,7 +286,7 @@ int make_layout(const MMScanArgs* a, Layout* l) {
   Offsets o;
   l->hlong = o.take(n * ((a->dstate + 3) / 4 * 4));
   l->slong = o.take(n);
-  l->bytes = o.at + 256;
+  l->bytes = o.at;
   return MM_OK;
 }
 }  // namespace
@@ -327,7 +328,8 @@ extern "C" int mm_selective_scan_train_fwd(const MMScanArgs* a, float* states, v
   }
   if (!a->u || !a->delta || !a->A || !a->B || !a->C) return MM_ERR_ARG;
   if (chunks_of(*a) > 1 && (!states || reinterpret_cast<uintptr_t>(states) % 16)) return MM_ERR_ARG;
-  if (!workspace || workspace_bytes < l.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return MM_ERR_WORKSPACE;
+  if (l.bytes && (!workspace || workspace_bytes < l.bytes || reinterpret_cast<uintptr_t>(workspace) % 256))
+    return MM_ERR_WORKSPACE;
   Params p = {};
   set_inputs(p, *a);
   p.y = a->y;

@@ -65,8 +65,10 @@ def _run(name: str, dev: torch.device, args, *rest) -> None:
     _lib.check(rc, name)
 
 
-def _workspace(size_name: str, args, dev: torch.device) -> torch.Tensor:
-    return torch.empty(_size(size_name, args), dtype=torch.uint8, device=dev)
+def _run_with_workspace(name: str, size_name: str, dev: torch.device, args, *before) -> None:
+    nbytes = _size(size_name, args)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _run(name, dev, args, *before, _p(ws), nbytes)
 
 
 def _by_channel(t: torch.Tensor) -> bool:
@@ -105,20 +107,32 @@ def _like(grad: torch.Tensor | None, t: torch.Tensor | None) -> torch.Tensor | N
 # ---- 8-bit activation checkpoints --------------------------------------------------------------------------
 
 
+def _three(t: torch.Tensor):
+    """(sizes, strides) of ``t``, up to three axes, as (batch, rows, length)."""
+    size, stride = t.shape, t.stride()
+    return ((1,) * (3 - len(size)) + tuple(size), (0,) * (3 - len(size)) + stride)
+
+
 def _checkpoint_args(x, codes, exponents):
-    return _args(_lib.MMCheckpoint8Args, _p(x), _p(codes), _p(exponents), _lib.DTYPE_CODE[x.dtype], *x.shape, *x.stride(),
-                 *codes.stride(), *exponents.stride())
+    size, stride = _three(x)
+    return _args(_lib.MMCheckpoint8Args, _p(x), _p(codes), _p(exponents), _lib.DTYPE_CODE[x.dtype], *size, *stride,
+                 *_three(codes)[1], *_three(exponents)[1])
 
 
 def _checkpoint_buffers(shape, device, by_channel: bool):
-    """Codes and exponents for a (batch, channels, time) tensor, laid out like it. Rows of codes start on multiples
-    of the block, so that they can be written and read in vectors whatever the length."""
-    b, d, n = shape
+    """Codes and exponents for a tensor of up to three axes, laid out like it. Rows of codes start on multiples of the
+    block, so that they can be written and read in vectors whatever the length."""
+    n = shape[-1]
     blocks = -(-n // CHECKPOINT8_BLOCK)
-    exponents = _empty((b, d, blocks), torch.uint8, device, by_channel)
     if by_channel:
-        return _empty(shape, torch.int8, device, True), exponents
-    return torch.empty((b, d, blocks * CHECKPOINT8_BLOCK), dtype=torch.int8, device=device)[..., :n], exponents
+        lead, d = tuple(shape[:-2]), shape[-2]
+        return (torch.empty((*lead, n, d), dtype=torch.int8, device=device).transpose(-1, -2),
+                torch.empty((*lead, blocks, d), dtype=torch.uint8, device=device).transpose(-1, -2))
+    pitch, strides = blocks * CHECKPOINT8_BLOCK, [1]
+    for size in reversed(shape[1:]):
+        strides.insert(0, strides[0] * (pitch if len(strides) == 1 else size))
+    return (torch.empty_strided(shape, strides, dtype=torch.int8, device=device),
+            torch.empty((*shape[:-1], blocks), dtype=torch.uint8, device=device))
 
 
 @dataclass(frozen=True)
@@ -145,18 +159,18 @@ class Checkpoint8:
         dtype = dtype or self.dtype
         if dtype not in _lib.DTYPE_CODE:
             raise TypeError(f"unsupported dtype {dtype}")
-        codes, exponents = _rows3(self.codes), _rows3(self.exponents)
+        codes, exponents = _up_to_three(self.codes), _up_to_three(self.exponents)
         dev = _lib.require_cuda(codes, exponents)
-        out = _empty(codes.shape, dtype, dev, _by_channel(codes))
+        if codes.dim() > 1 and _by_channel(codes):
+            out = torch.empty((*codes.shape[:-2], codes.shape[-1], codes.shape[-2]), dtype=dtype, device=dev).transpose(-1, -2)
+        else:
+            out = torch.empty(codes.shape, dtype=dtype, device=dev)
         _run("mm_checkpoint8_unpack", dev, _checkpoint_args(out, codes, exponents))
-        return out.view(self.shape) if self.codes.dim() != 3 else out
+        return out if self.codes.dim() <= 3 else out.view(self.shape)
 
 
-def _rows3(t: torch.Tensor) -> torch.Tensor:
-    """(..., length) as (batch, rows, length), a view for up to three axes."""
-    if t.dim() > 3:
-        return t.flatten(0, -3)
-    return t.reshape((1,) * (3 - t.dim()) + tuple(t.shape)) if t.dim() < 3 else t
+def _up_to_three(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dim() <= 3 else t.flatten(0, -3)
 
 
 def checkpoint8(x: torch.Tensor) -> Checkpoint8:
@@ -168,12 +182,10 @@ def checkpoint8(x: torch.Tensor) -> Checkpoint8:
     if x.dtype not in _lib.DTYPE_CODE:
         raise TypeError(f"unsupported dtype {x.dtype}")
     dev = _lib.require_cuda(x)
-    rows = _rows3(x.detach())
-    codes, exponents = _checkpoint_buffers(rows.shape, dev, _by_channel(rows))
+    rows = _up_to_three(x)
+    codes, exponents = _checkpoint_buffers(rows.shape, dev, rows.dim() > 1 and _by_channel(rows))
     _run("mm_checkpoint8_pack", dev, _checkpoint_args(rows, codes, exponents))
-    if x.dim() < 3:
-        codes, exponents = codes[(0,) * (3 - x.dim())], exponents[(0,) * (3 - x.dim())]
-    elif x.dim() > 3:
+    if x.dim() > 3:
         codes, exponents = codes.unflatten(0, x.shape[:-2]), exponents.unflatten(0, x.shape[:-2])
     return Checkpoint8(codes, exponents, x.dtype)
 
@@ -222,8 +234,7 @@ def causal_conv1d_backward(dout: torch.Tensor, x: torch.Tensor | Checkpoint8, we
               _p(dout), _p(dx), _p(dw), _p(db), _lib.DTYPE_CODE[dout.dtype], batch, dim, seqlen, ops.D_CONV,
               *(_ZERO3 if held else src.stride()), *(src.stride() if held else _ZERO3),
               *(x.exponents.stride() if held else _ZERO3), *dout.stride(), *dx.stride(), bool(silu))
-    ws = _workspace("mm_causal_conv1d_bwd_workspace_size", a, dev)
-    _run("mm_causal_conv1d_bwd", dev, a, ws.data_ptr(), ws.numel())
+    _run_with_workspace("mm_causal_conv1d_bwd", "mm_causal_conv1d_bwd_workspace_size", dev, a)
     return dx, dw, db
 
 
@@ -302,8 +313,7 @@ def selective_scan_backward(dy: torch.Tensor, u, delta, A, B, C, *, D=None, z=No
               _p(g["delta_bias"]), *dy.stride(), *g["u"].stride(), *g["delta"].stride(), *_s3(g["z"]), *g["B"].stride(),
               *g["C"].stride())
     assert states.numel() * 4 == _size("mm_selective_scan_states_size", a.fwd), "states of another call"
-    ws = _workspace("mm_selective_scan_bwd_workspace_size", a, dev)
-    _run("mm_selective_scan_bwd", dev, a, ws.data_ptr(), ws.numel())
+    _run_with_workspace("mm_selective_scan_bwd", "mm_selective_scan_bwd_workspace_size", dev, a)
     return g
 
 
@@ -325,12 +335,16 @@ def selective_scan_states(u, delta, A, B, C, *, D=None, z=None, delta_bias=None,
     assert A.dtype == torch.float32
     if u.dtype not in _lib.DTYPE_CODE:
         raise TypeError(f"unsupported dtype {u.dtype}")
+    return _scan_forward(u, delta, A, B, C, D, z, delta_bias, delta_softplus, outputs)
+
+
+def _scan_forward(u, delta, A, B, C, D, z, delta_bias, delta_softplus, outputs=True):
+    dev = u.device
     y = _empty(u.shape, u.dtype, dev, _by_channel(u)) if outputs else None
-    state = torch.empty((batch, dim, n), dtype=torch.float32, device=dev) if outputs else None
+    state = torch.empty((u.shape[0], u.shape[1], A.shape[1]), dtype=torch.float32, device=dev) if outputs else None
     a = _args(_lib.MMScanArgs, *_scan_args(u, delta, A, B, C, D, z, delta_bias, delta_softplus, y, state))
     states = torch.empty(_size("mm_selective_scan_states_size", a) // 4, dtype=torch.float32, device=dev)
-    ws = _workspace("mm_selective_scan_train_workspace_size", a, dev)
-    _run("mm_selective_scan_train_fwd", dev, a, states.data_ptr(), ws.data_ptr(), ws.numel())
+    _run_with_workspace("mm_selective_scan_train_fwd", "mm_selective_scan_train_workspace_size", dev, a, states.data_ptr())
     return y, state, states
 
 
@@ -348,7 +362,7 @@ class _SelectiveScan(torch.autograd.Function):
         dtype = _scan_dtype(u, delta, B, C, z)
         uc, dc, Bc, Cc, zc = (_cast(t, dtype) for t in (u, delta, B, C, z))
         Af, Df, bf = _cast(A, torch.float32), _f32(D), _f32(delta_bias)
-        y, state, states = selective_scan_states(uc, dc, Af, Bc, Cc, D=Df, z=zc, delta_bias=bf, delta_softplus=softplus)
+        y, state, states = _scan_forward(uc, dc, Af, Bc, Cc, Df, zc, bf, softplus)
         ctx.softplus = softplus
         ctx.dtypes = tuple(None if t is None else t.dtype for t in (u, delta, A, B, C, D, z, delta_bias))
         ctx.save_for_backward(uc, dc, Af, Bc, Cc, Df, zc, bf, states)
@@ -396,18 +410,19 @@ class _PreferenceLoss(torch.autograd.Function):
         rows, length, vocab = logits.shape
         dev, pairs = logits.device, rows // 2
         f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)
-        loss, chosen, rejected, stats, slope = f32(), f32(pairs), f32(pairs), f32(rows, length, 2), f32(rows)
+        loss, chosen, rejected = f32(), f32(pairs), f32(pairs)
+        stats = f32(rows * (2 * length + 1))  # and the answers' slopes behind them
         x = logits.detach()
         if vocab > 1 and x.stride(2) != 1:
             x = x.contiguous()
         values = (_lib.DTYPE_CODE[x.dtype], pairs, length, vocab, *x.stride()[:2])
         rest = (ignore_index, _bits(beta), _bits(smoothing))
-        a = _args(_lib.MMPreferenceArgs, _p(x), _p(labels), _p(ref), _p(loss), _p(chosen), _p(rejected), _p(stats), _p(slope), 0, 0,
+        a = _args(_lib.MMPreferenceArgs, _p(x), _p(labels), _p(ref), _p(loss), _p(chosen), _p(rejected), _p(stats),
+                  _p(stats) + 8 * rows * length, 0, 0,
                   *values, 0, 0, *rest)
-        ws = _workspace("mm_preference_loss_workspace_size", a, dev)
-        _run("mm_preference_loss_fwd", dev, a, ws.data_ptr(), ws.numel())
+        _run_with_workspace("mm_preference_loss_fwd", "mm_preference_loss_workspace_size", dev, a)
         ctx.args = values, rest
-        ctx.save_for_backward(x, labels, stats, slope)
+        ctx.save_for_backward(x, labels, stats)
         ctx.mark_non_differentiable(chosen, rejected)
         return loss, chosen, rejected
 
@@ -416,11 +431,12 @@ class _PreferenceLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, *_):
         if grad_loss is None:
             return (None,) * 6
-        x, labels, stats, slope = ctx.saved_tensors
+        x, labels, stats = ctx.saved_tensors
         grad = _f32(grad_loss)
         dlogits = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         values, rest = ctx.args
-        a = _args(_lib.MMPreferenceArgs, _p(x), _p(labels), 0, 0, 0, 0, _p(stats), _p(slope), _p(grad), _p(dlogits), *values,
+        a = _args(_lib.MMPreferenceArgs, _p(x), _p(labels), 0, 0, 0, 0, _p(stats), _p(stats) + 8 * labels.numel(), _p(grad),
+                  _p(dlogits), *values,
                   *dlogits.stride()[:2], *rest)
         _run("mm_preference_loss_bwd", x.device, a)
         return dlogits, None, None, None, None, None
