@@ -25,6 +25,7 @@ struct Params {
   int ahead;       // grad_kernel copies its raw inputs ahead: all contiguous along one axis, rows 16-byte aligned
   int np;          // states, rounded up to a multiple of four: rows of the buffers below
   int chunks, longs, per_long;  // chunks, long chunks, chunks of a long one
+  int whole;                    // a single long chunk, walked by the kernels of mm_scan_rows.cu
   // (batch, chunks, dim, np): the state every chunk starts from; the k it gets from the later chunks of its long one
   float *hst, *kst;
   float* later;  // (batch, chunks, dim): the sum of d over those
@@ -181,10 +182,13 @@ inline void set_access(Params& p, Access access, const MMScanArgs& f) {
   p.by_channel = access == kAnyStride && f.u_stride[1] == 1;
 }
 inline int chunks_of(const MMScanArgs& f) { return (int)((f.seqlen + kT - 1) / kT); }
+// Up to 256 steps of up to 16 states are walked whole, by the kernels of mm_scan_rows.cu: one launch, and nothing to join
+// (bf16 1x1536 forward: 128 steps 12 us, cut 29; 256 21 and 29; 512 40 and 35).
+inline bool walked_whole(const MMScanArgs& f) { return f.dstate <= 16 && f.seqlen <= 256; }
 // Chunks of a long one: four; fewer where that leaves an SM less than twelve warps of 32 channels to walk them. Two chunks
-// are always one long chunk, which needs no joining: three launches fewer for the same device time (bf16 1x1536x48
-// forward and backward 51 us, split 54; 1x1536x64 60, split 56; three or four chunks lose: 1x1536x128 100, split 58).
+// are one long chunk, which needs no joining.
 inline int per_long_of(const MMScanArgs& f) {
+  if (walked_whole(f)) return f.seqlen > 0 ? chunks_of(f) : 1;
   int n = 4;
   while (chunks_of(f) > 2 && n > 1 && f.batch * ((f.dim + 31) / 32) * ((chunks_of(f) + n - 1) / n) < 12 * 148) n /= 2;
   return n;
@@ -232,10 +236,13 @@ inline void set_inputs(Params& p, const MMScanArgs& f) {
   p.chunks = chunks_of(f);
   p.longs = longs_of(f);
   p.per_long = per_long_of(f);
+  p.whole = walked_whole(f);
 }
 
 // Fills kst, later, klong and slong (mm_scan_walk.cu): the part of the gradient that runs through time
 int walk_back(const Params& p, int64_t dtype, cudaStream_t s);
+// Over whole sequences of up to 16 states (mm_scan_rows.cu): y, state_out and hst, or kst and later
+template <bool BACK> int walk_rows(const Params& p, int64_t dtype, cudaStream_t s);
 
 }  // namespace train
 }  // namespace mm

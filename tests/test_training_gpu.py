@@ -127,6 +127,26 @@ def test_scan_gradient_many_tiles():
     check_scan((8, 1000, 4, 330), torch.float32, "channel_first", ALL, seed=5)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("shape", [(2, 9, 16, 256), (2, 9, 16, 257), (1, 33, 7, 255), (1, 8191, 2, 263), (1, 8197, 9, 259)])
+def test_scan_gradient_where_the_walks_change(shape, layout, dtype):
+    """Lengths and channel counts around those from which whole sequences are walked, cut into long chunks or not."""
+    check_scan(shape, dtype, layout, ALL, seed=11)
+
+
+@pytest.mark.parametrize("shape", [(1, 40, 16, 100), (1, 40, 16, 300), (1, 8200, 6, 290)])
+def test_scan_states_alone(shape):
+    """The states are the same whether or not the outputs are asked for."""
+    gpu, _, _, _ = scan_inputs(shape, torch.float16, "channel_first", ALL, 13)
+    u, delta, A, B, C, D, z, bias = (gpu[k] for k in NAMES)
+    call = lambda outputs: training.selective_scan_states(u, delta, A, B, C, D=D, z=z, delta_bias=bias, delta_softplus=True,
+                                                          outputs=outputs)
+    y, state, states = call(True)
+    none, nothing, alone = call(False)
+    assert none is None and nothing is None and torch.equal(states, alone)
+
+
 def test_scan_gradient_softplus_cutoff():
     """Steps on both sides of the cutoff at 20, and steps whose decay leaves nothing of the state."""
     shape, opts = (1, 6, 4, 70), frozenset(("softplus",))
