@@ -14,6 +14,7 @@ import ctypes
 import struct
 from array import array
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 import torch.nn.functional as F
@@ -65,8 +66,7 @@ def _run(name: str, dev: torch.device, args, *rest) -> None:
     _lib.check(rc, name)
 
 
-def _run_with_workspace(name: str, size_name: str, dev: torch.device, args, *before) -> None:
-    nbytes = _size(size_name, args)
+def _run_with_workspace(name: str, nbytes: int, dev: torch.device, args, *before) -> None:
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _run(name, dev, args, *before, _p(ws), nbytes)
 
@@ -234,7 +234,7 @@ def causal_conv1d_backward(dout: torch.Tensor, x: torch.Tensor | Checkpoint8, we
               _p(dout), _p(dx), _p(dw), _p(db), _lib.DTYPE_CODE[dout.dtype], batch, dim, seqlen, ops.D_CONV,
               *(_ZERO3 if held else src.stride()), *(src.stride() if held else _ZERO3),
               *(x.exponents.stride() if held else _ZERO3), *dout.stride(), *dx.stride(), bool(silu))
-    _run_with_workspace("mm_causal_conv1d_bwd", "mm_causal_conv1d_bwd_workspace_size", dev, a)
+    _run_with_workspace("mm_causal_conv1d_bwd", _size("mm_causal_conv1d_bwd_workspace_size", a), dev, a)
     return dx, dw, db
 
 
@@ -312,8 +312,9 @@ def selective_scan_backward(dy: torch.Tensor, u, delta, A, B, C, *, D=None, z=No
     a = _args(_lib.MMScanBwdArgs, *f, _p(states), _p(dy), _p(dstate), *(_p(g[k]) for k in ("u", "delta", "A", "B", "C", "D", "z")),
               _p(g["delta_bias"]), *dy.stride(), *g["u"].stride(), *g["delta"].stride(), *_s3(g["z"]), *g["B"].stride(),
               *g["C"].stride())
-    assert states.numel() * 4 == _size("mm_selective_scan_states_size", a.fwd), "states of another call"
-    _run_with_workspace("mm_selective_scan_bwd", "mm_selective_scan_bwd_workspace_size", dev, a)
+    states_bytes, _, nbytes = _scan_sizes(_lib.DTYPE_CODE[u.dtype], batch, dim, n, seqlen)
+    assert states.numel() * 4 == states_bytes, "states of another call"
+    _run_with_workspace("mm_selective_scan_bwd", nbytes, dev, a)
     return g
 
 
@@ -343,8 +344,9 @@ def _scan_forward(u, delta, A, B, C, D, z, delta_bias, delta_softplus, outputs=T
     y = _empty(u.shape, u.dtype, dev, _by_channel(u)) if outputs else None
     state = torch.empty((u.shape[0], u.shape[1], A.shape[1]), dtype=torch.float32, device=dev) if outputs else None
     a = _args(_lib.MMScanArgs, *_scan_args(u, delta, A, B, C, D, z, delta_bias, delta_softplus, y, state))
-    states = torch.empty(_size("mm_selective_scan_states_size", a) // 4, dtype=torch.float32, device=dev)
-    _run_with_workspace("mm_selective_scan_train_fwd", "mm_selective_scan_train_workspace_size", dev, a, states.data_ptr())
+    states_bytes, nbytes, _ = _scan_sizes(_lib.DTYPE_CODE[u.dtype], u.shape[0], u.shape[1], A.shape[1], u.shape[2])
+    states = torch.empty(states_bytes // 4, dtype=torch.float32, device=dev)
+    _run_with_workspace("mm_selective_scan_train_fwd", nbytes, dev, a, states.data_ptr())
     return y, state, states
 
 
@@ -353,6 +355,14 @@ def _scan_args(u, delta, A, B, C, D, z, delta_bias, softplus, y=None, state=None
     return (_p(u), _p(delta), _p(A), _p(B), _p(C), _p(D), _p(z), _p(y), _p(state), _lib.DTYPE_CODE[u.dtype], u.shape[0],
             u.shape[1], A.shape[1], u.shape[2], *u.stride(), *delta.stride(), *_s3(z), *_s3(y), *B.stride(), *C.stride(),
             *A.stride(), bool(softplus), 0, 0, _p(delta_bias))
+
+
+@lru_cache(maxsize=256)
+def _scan_sizes(dtype: int, batch: int, dim: int, dstate: int, seqlen: int):
+    """Bytes of the states and of the forward and the backward pass's workspaces, which follow from the sizes alone."""
+    f = _lib.MMScanArgs(dtype=dtype, batch=batch, dim=dim, dstate=dstate, seqlen=seqlen)
+    return (_size("mm_selective_scan_states_size", f), _size("mm_selective_scan_train_workspace_size", f),
+            _size("mm_selective_scan_bwd_workspace_size", _lib.MMScanBwdArgs(fwd=f)))
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -403,6 +413,12 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
 # ---- preference loss ---------------------------------------------------------------------------------------
 
 
+@lru_cache(maxsize=256)
+def _preference_bytes(dtype: int, pairs: int, length: int, vocab: int) -> int:
+    return _size("mm_preference_loss_workspace_size",
+                 _lib.MMPreferenceArgs(dtype=dtype, pairs=pairs, length=length, vocab=vocab, beta=1.0))
+
+
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ref, beta, smoothing, ignore_index):
@@ -418,9 +434,8 @@ class _PreferenceLoss(torch.autograd.Function):
         values = (_lib.DTYPE_CODE[x.dtype], pairs, length, vocab, *x.stride()[:2])
         rest = (ignore_index, _bits(beta), _bits(smoothing))
         a = _args(_lib.MMPreferenceArgs, _p(x), _p(labels), _p(ref), _p(loss), _p(chosen), _p(rejected), _p(stats),
-                  _p(stats) + 8 * rows * length, 0, 0,
-                  *values, 0, 0, *rest)
-        _run_with_workspace("mm_preference_loss_fwd", "mm_preference_loss_workspace_size", dev, a)
+                  _p(stats) + 8 * rows * length, 0, 0, *values, 0, 0, *rest)
+        _run_with_workspace("mm_preference_loss_fwd", _preference_bytes(*values[:4]), dev, a)
         ctx.args = values, rest
         ctx.save_for_backward(x, labels, stats)
         ctx.mark_non_differentiable(chosen, rejected)
@@ -436,8 +451,7 @@ class _PreferenceLoss(torch.autograd.Function):
         dlogits = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         values, rest = ctx.args
         a = _args(_lib.MMPreferenceArgs, _p(x), _p(labels), 0, 0, 0, 0, _p(stats), _p(stats) + 8 * labels.numel(), _p(grad),
-                  _p(dlogits), *values,
-                  *dlogits.stride()[:2], *rest)
+                  _p(dlogits), *values, *dlogits.stride()[:2], *rest)
         _run("mm_preference_loss_bwd", x.device, a)
         return dlogits, None, None, None, None, None
 
