@@ -15,9 +15,10 @@ struct Params {
 };
 
 // Time contiguous: a lane takes 8 consecutive values, so four lanes share a block and agree on its maximum by
-// two shuffles. A warp covers CPT * 256 values of one row, with all its loads in flight before the first is used
-// (bf16 10240 x 32768, packed and restored: CPT 1 625 us, CPT 4 374). ACCESS: that of x; codes are taken by 8-byte words
-// but for kAnyStride.
+// two shuffles. A warp covers CPT * 256 values of one row, with all its loads in flight before the first is used:
+// memory is the bound, and bytes in flight decide (bf16 10240 x 32768, packed and restored: CPT 1 625 us, 2 450, 4 370:
+// 1.02 GB each way, 5.5 TB/s; in blocks of 512 threads 390). Short rows take CPT 1, or half their warps had nothing
+// to do. ACCESS: that of x; codes are taken by 8-byte words but for kAnyStride.
 template <typename T, bool PACK, int ACCESS, int CPT>
 __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per_row) {
   const int lane = threadIdx.x & 31;
@@ -61,27 +62,30 @@ __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per
     }
   } else {
     uint2 raw[CPT];
-    float scale[CPT];
+    // one load for the scales of the warp's blocks: the four lanes of a block hold those of its four chunks
+    const int first = begin + (lane & 3) * 256;
+    unsigned mine = 0;
+    if ((lane & 3) < CPT && first - (lane & 3) * 8 < p.length) mine = exps[(long long)(first / kCkBlock) * p.es[2]];
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
       const int t = begin + j * 256;
       if (t >= p.length) continue;
-      scale[j] = ck_scale(exps[(long long)(t / kCkBlock) * p.es[2]]);
       if (ACCESS != kAnyStride && t + 8 <= p.length) raw[j] = __ldcs(reinterpret_cast<const uint2*>(codes + t));
     }
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
       const int t = begin + j * 256, n = min(8, p.length - t);
       float v[8];
+      const float scale = ck_scale(__shfl_sync(0xffffffffu, mine, (lane & ~3) | j));
       if (ACCESS != kAnyStride && n == 8) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          v[k] = ck_restore<T>(ck_byte(raw[j].x, k), scale[j]);
-          v[k + 4] = ck_restore<T>(ck_byte(raw[j].y, k), scale[j]);
+          v[k] = ck_restore<T>(ck_byte(raw[j].x, k), scale);
+          v[k + 4] = ck_restore<T>(ck_byte(raw[j].y, k), scale);
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = k < n ? ck_restore<T>(codes[(t + k) * p.cs[2]], scale[j]) : 0.f;
+        for (int k = 0; k < 8; ++k) v[k] = k < n ? ck_restore<T>(codes[(t + k) * p.cs[2]], scale) : 0.f;
       }
       if (ACCESS == kAligned && n == 8)
         row_store(x + t, 1, ACCESS, 8, v);
@@ -91,7 +95,8 @@ __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per
   }
 }
 
-// Channels contiguous: a thread takes one block of one channel, so a warp's accesses run along channels.
+// Channels contiguous: a thread takes one block of one channel, so a warp's accesses run along channels. It keeps
+// the block in registers from the maximum to the codes.
 template <typename T, bool PACK>
 __global__ void __launch_bounds__(256) columns_kernel(const Params p, int blocks) {
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;

@@ -252,7 +252,7 @@ template <typename T> MM_DEV Raw8<T> raw_load(const T* p, long long s, int acces
   Raw8<T> r;
   if (access == kAligned && n == 8) {
 #pragma unroll
-    for (int h = 0; h < (int)sizeof(T) / 2; ++h) r.v[h] = __ldcs(reinterpret_cast<const uint4*>(p) + h);
+    for (int h = 0; h < (int)sizeof(T) / 2; ++h) r.v[h] = *(reinterpret_cast<const uint4*>(p) + h);
   } else if (access == kContiguous && n == 8) {
     r = raw_load_shifted(p);
   } else {

@@ -59,9 +59,10 @@ MM_DEV f2_t taps(const f2_t (&w)[kW], f2_t bias, f2_t a, f2_t b, f2_t c, f2_t d)
 
 // ---- time contiguous --------------------------------------------------------------------------------
 // A warp covers CPT * 256 consecutive steps of one row: chunk j of lane l are the 8 steps from 256 j + 8 l. All
-// its loads are in flight before the first is used (8 KB a warp at CPT 4, which the memory needs: 84 -> 46 us for
-// 8x1536x4096 f16 against CPT 1). Halos come from the neighbouring lanes, and for the warp's first and last lane
-// from memory.
+// its loads are in flight before the first is used, 8 KB a warp at CPT 4 (f16 8x1536x4096, CPT 1 and 4: forward 84
+// and 62 us, the latter 4.1 TB/s). Halos come from the neighbouring lanes, and for the warp's first and last lane
+// from memory. Rows of up to 512 steps take CPT 1, or half their warps had nothing to do. Rows off a 16-byte boundary
+// (bf16 4x5120x5601: forward 271 us, backward 398) pay for the shifting of words, two thirds more than aligned ones.
 
 template <typename T, int ACCESS, int CPT>
 __global__ void __launch_bounds__(256) fwd_rows_kernel(const Params p, int warps_per_row) {
@@ -171,7 +172,9 @@ template <typename T, bool CK> struct Source {
   }
 };
 
-// The chunks from the last to the first, so that the three dpre after a chunk are known
+// The chunks from the last to the first, so that the three dpre after a chunk are known. Bound by instructions rather
+// than memory: an element takes its pre-activation again, silu', four taps for dx and five sums (f16 8x1536x4096 from
+// the checkpoint 105 us, 2.4 TB/s; from x itself 85, 3.6).
 template <typename T, bool CK, int ACCESS, int CPT>
 __global__ void __launch_bounds__(256) bwd_rows_kernel(const Params p, int warps_per_row) {
   const int lane = threadIdx.x & 31;
@@ -375,8 +378,8 @@ __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int ru
     for (int c = 0; c < H; ++c) win[j][c] = both(0.f);
     if (k.t0 > 0) load_few<T, VEC>(x + (long long)(k.t0 - 3 + j) * p.xs[2], k.step * p.xs[1], k.n, win[j]);
   }
-  // Twice over each block: for its maxima, then, out of L1, for everything else. (Holding the block in registers
-  // instead leaves 8 warps an SM: bf16 4x5120x5601 255 us.)
+  // Twice over each block: for its maxima, then, out of L1, for everything else (bf16 4x5120x5601 198 us, 2.9 TB/s;
+  // the block held in registers instead leaves 8 warps an SM, 255 us).
   for (int tb = k.t0; tb < k.t1; tb += kCkBlock) {
     const int n = min(kCkBlock, k.t1 - tb);
     const T* xb = x + (long long)tb * p.xs[2];
@@ -426,10 +429,11 @@ __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int ru
 
 // Backward: step t completes dx[t-3] from the last four dpre; three steps past the run finish its end. Only the
 // run's own steps enter the sums. The loads of the next eight steps are in flight while eight are worked on; two
-// CTAs of an SM (128 registers) hide them best.
+// CTAs of an SM (128 registers) hide them best (bf16 4x5120x5601 from the checkpoint 271 us, 2.1 TB/s; what bounds it is
+// the instructions of an element, as above).
 template <typename T, bool CK, bool VEC>
 __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int run, int runs) {
-    constexpr int C = kC<T>, H = C / 2, kU = 8;
+  constexpr int C = kC<T>, H = C / 2, kU = 8;
   static_assert(kU > 3 && kCkBlock % kU == 0, "from the second group on, step t - 3 is the run's own");
   Walk k;
   if (!walk_of<C, VEC>(p, run, runs, k)) return;
@@ -540,7 +544,8 @@ __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int
     }
 }
 
-// Sums the partials of every channel in a fixed order, in 64 bits: eight threads share a value.
+// Sums the partials of every channel in a fixed order, in 64 bits: eight threads share a value (4 us for 32 partials of
+// 1536 channels, 22 for 352 of 5120).
 __global__ void __launch_bounds__(256) sum_kernel(const float* part, long long parts, int dim, float* dw, float* db) {
   __shared__ double sum[8][32];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;

@@ -323,8 +323,12 @@ template <bool ADD> MM_DEV void put_sums(float* at, int lane, const f2_t (&acc)[
 
 // ---- up to 16 states ----
 // Three CTAs of four warps per SM (the registers' limit) take (chunk, group of channels) items tile by tile: some are
-// in their elementwise parts while others work. The raw inputs of the
-// next tile arrive by cp.async meanwhile.
+// in their elementwise parts while others work. The raw inputs of the next tile arrive by cp.async meanwhile.
+//
+// f16 8x1536x4096, 16 states: 1.25 ms. 478 instructions for 32 steps of a channel, 0.51 of them a clock and scheduler
+// with three warps on each; the way in from shared memory is 59 % taken, the FMA pipe 46 %, memory (0.7 TB/s) hardly.
+// What did not pay: tiles of 64 steps with four states a lane, which halve the shuffles but leave two CTAs an SM; warps
+// for the elementwise parts beside warps for the states, whose registers then spill.
 constexpr int kGradThreads = 128;
 // float32's raw inputs take twice the room, and a tile of half the channels keeps three CTAs on an SM
 template <typename T> constexpr int kTile = sizeof(T) == 4 ? 16 : 32;
@@ -467,7 +471,8 @@ __global__ void __launch_bounds__(kGradThreads, 3) grad_kernel(const Params p) {
 }
 
 // ---- more than 16 states ----
-// The same in passes of 16 states over one staged tile of channels per CTA; every warp does all of it.
+// The same in passes of 16 states over one staged tile of channels per CTA; every warp does all of it (bf16 8x1536x512
+// with 64 states 0.86 ms; a state and step takes 1.4 times what it takes with 16, for the staging of every pass).
 constexpr int kWideThreads = 128;
 constexpr int kWideCh = 32;
 constexpr int kWideSmem = kWideCh * Passes::size * 4 + 4 * kTemp * 16 + 4 * 2 * kNB * kT * 4;
@@ -550,7 +555,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grad_wide_kernel(const Params
 
 // ---- sums over groups and chunks -------------------------------------------------------------------
 // With more than 16 partials eight threads share a value (every eighth partial each): 5120 or 24 channels in groups of
-// 16 would otherwise be one chain of up to 320 loads. With fewer a thread has its own.
+// 16 would otherwise be one chain of up to 320 loads. With fewer a thread has its own (f16 8x1536x4096 37 us).
 template <typename T> __global__ void __launch_bounds__(256) reduce_kernel(const Params p, long long bc_blocks) {
   __shared__ double sum[2][8][32];
   const int lane = threadIdx.x % 32, part = threadIdx.x / 32;

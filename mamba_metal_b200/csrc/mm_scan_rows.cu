@@ -71,8 +71,11 @@ template <bool BACK, typename T, int S> __global__ void __launch_bounds__(kThrea
   unit_of<kCh>(tid, p.by_channel, uch, useg);
   const bool unit = d0 + uch < p.dim;
   const f2_t bias = dup(p.bias && unit ? p.bias[d0 + uch] : 0.f), D = dup(!BACK && p.D && unit ? p.D[d0 + uch] : 0.f);
-  // and its part of B and C: four states of a step
-  const int n0 = 4 * (tid / 32), tq = tid % 32;
+  // and its part of B and C: four states of a step; threads run along whichever of time and states is contiguous
+  // (f16 8x1536x4096, channels contiguous: along time 0.89 ms, along states 0.86)
+  constexpr int Q = NM / 4;
+  const bool across = p.Cs[1] == 1, brings = tid < kT * Q;
+  const int tq = across ? tid / Q : tid % kT, n0 = 4 * (across ? tid % Q : tid / kT);
 
   f2_t A[S / 2], h[S / 2];
 #pragma unroll
@@ -98,7 +101,7 @@ template <bool BACK, typename T, int S> __global__ void __launch_bounds__(kThrea
     raw = fetch(p.delta, p.ds, t0);
     xs = BACK ? fetch(p.dy, p.ys, t0) : fetch(p.u, p.us, t0);
     if (p.z && (BACK || p.y)) zs = fetch(p.z, p.zs, t0);
-    if (n0 < NM) {
+    if (brings) {
       Bq = BACK ? load_quad<T>(p.C, p.Cs, b, n0, t0 + tq, p) : load_quad<T>(p.B, p.Bs, b, n0, t0 + tq, p);
       if (!BACK) Cq = load_quad<T>(p.C, p.Cs, b, n0, t0 + tq, p);
     }
@@ -121,7 +124,7 @@ template <bool BACK, typename T, int S> __global__ void __launch_bounds__(kThrea
       to[k * kCh] = make_float2(dt.x, w.x);
       to[(k + 1) * kCh] = make_float2(dt.y, w.y);
     }
-    if (n0 < NM) {
+    if (brings) {
       *reinterpret_cast<float4*>(sB + (buf * kT + tq) * NM + n0) = floats_of(Bq);
       if (!BACK) *reinterpret_cast<float4*>(sC + (buf * kT + tq) * NM + n0) = floats_of(Cq);
     }

@@ -55,7 +55,8 @@ MM_DEV f2_t silu_slope(f2_t z) {
   const f2_t s = sigmoid(z);
   return f2_mul(s, f2_fma(z, f2_sub(dup(1.f), s), dup(1.f)));
 }
-// exp(x) for x <= 20: 2^(x log2 e) with the product's rounding error carried along
+// exp(x) for x <= 20: 2^(x log2 e), log2 e in two words after Cody and Waite, with the product's rounding error carried
+// along
 MM_DEV f2_t exp_of(f2_t x) {
   const f2_t y = f2_mul(x, dup(kLog2e));
   const f2_t rest = f2_fma(x, dup(1.925963033e-8f), f2_fma(x, dup(kLog2e), f2_mul(y, dup(-1.f))));  // log2 e's second word
@@ -68,7 +69,7 @@ MM_DEV f2_t clamped(f2_t x) {
   return f2_pack(fminf(fmaxf(v.x, -120.f), 20.f), fminf(fmaxf(v.y, -120.f), 20.f));
 }
 // softplus with the forward's cutoff at 20, without a branch (several run side by side). log(1 + e): below
-// e = 0.4 as 2 artanh(e / (2 + e)), whose series keeps the relative accuracy of small steps (truncated below
+// e = 0.4 as 2 artanh(e / (2 + e)), whose Taylor series keeps the relative accuracy of small steps (truncated below
 // 1e-7); above, where the result is no longer small against 1, as lg2(1 + e).
 MM_DEV f2_t step_of(f2_t raw, int softplus) {
   const f2_t e = exp_of(clamped(raw));

@@ -12,9 +12,10 @@
 //
 // Bound by the MUFU (one ex2 for each state and step, 16 per clock and SM: 805 M, 0.18 ms at 1.9 GHz for a walk of
 // 8x1536x4096 with 16 states) and close behind by the registers' way in from shared memory, 128 bytes per clock: a
-// step's B and C arrive as 32 lanes x 128 bytes. Measured there, f16: kState 0.28 ms, kOut 0.45, kBack 0.33, with
+// step's B and C arrive as 32 lanes x 128 bytes. Measured there, f16: kState 0.28 ms, kOut 0.45, kBack 0.31, with
 // four blocks of four warps on an SM (five and six spill: kOut 0.50 and 0.58); tiles of 32 steps 0.32, 0.55, 0.39;
-// two channels a lane, which share B and C but leave 12 warps, 0.30, 0.53, 0.48.
+// two channels a lane, which share B and C but leave 12 warps, 0.30, 0.53, 0.48. The forward pass now walks that size
+// whole (mm_scan_rows.cu); f32 1x1536x5601 (31 us of MUFU): 63, 92 and 71 us.
 #include "mm_scan_train.cuh"
 
 namespace mm {
