@@ -454,7 +454,8 @@ int mm_preference_loss_bwd(const MMPreferenceArgs* args, mm_stream_t stream);
 /* mm_selective_scan_fwd for training: the same function, in kernels whose sums do not depend on timing, with
  * softplus at full relative accuracy for small steps, and with the states that the gradient starts from:
  * states (fp32, size from mm_selective_scan_states_size, 16-byte aligned) receives h before every 32nd step. y
- * may be NULL: only states (and state_out) are computed. piece_tiles and options are not read. */
+ * may be NULL: only states (and state_out) are computed. piece_tiles and options are not read. Either size can be 0
+ * (short calls); the pointer may then be NULL. */
 int mm_selective_scan_states_size(const MMScanArgs* args, size_t* bytes);
 int mm_selective_scan_train_workspace_size(const MMScanArgs* args, size_t* bytes);
 int mm_selective_scan_train_fwd(const MMScanArgs* args, float* states, void* workspace, size_t workspace_bytes,
