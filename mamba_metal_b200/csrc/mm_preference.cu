@@ -2,8 +2,8 @@
 //
 // The logits are all that counts: (tokens, vocab) read once forward (a running maximum and sum of exponentials),
 // read again and answered with the gradient backward; ignored tokens' logits are not read at all. Both passes are bound
-// by memory: for 8200 of 16384 rows of 50280 bf16 values 155 us (5.3 TB/s) and 383 us (6.4 TB/s, with the zeros of the
-// ignored rows), for 1865 of 3108 rows of 50277 float32 values 76 us (4.9 TB/s) and 158 us (6.3 TB/s). Sums over the
+// by memory: for 8200 of 16384 rows of 50280 bf16 values 151 us (5.5 TB/s) and 383 us (6.4 TB/s, with the zeros of the
+// ignored rows), for 1865 of 3108 rows of 50277 float32 values 77 us (4.9 TB/s) and 158 us (6.3 TB/s). Sums over the
 // tokens of an answer and over the pairs are taken in 64 bits and in a fixed order: an answer's log-probability
 // is a sum of a thousand values near -10 of which the loss sees small differences.
 #include "mm_common.cuh"
@@ -12,9 +12,9 @@ namespace mm {
 namespace pref {
 
 constexpr int kThreads = 512;
-// Forward, so that a thread has about 24 vectors of a row of 50280: with 512 threads 189 us for 8200 rows of bf16,
-// with 256 156; for 1865 rows of float32 76 and 80.
-template <typename T> constexpr int kStatsThreads = sizeof(T) == 4 ? 512 : 256;
+// Forward with the loss, repeated on the same rows: 8200 rows of 50280 bf16 values in blocks of 64, 128, 256 and 512 threads 151, 149, 163 and
+// 190 us (without loading ahead 152, 149, 157, 189), 1865 rows of 50277 float32 values in 128, 256 and 512 81, 77 and 81.
+template <typename T> constexpr int kStatsThreads = sizeof(T) == 4 ? 256 : 128;
 
 struct Params {
   const void* logits;
@@ -72,12 +72,16 @@ __global__ void __launch_bounds__(kStatsThreads<T>) stats_kernel(const Params p)
     a.m = m;
   };
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
-  constexpr int kU = 4;  // vectors in flight
-  for (int i = v0 + threadIdx.x; i < v1; i += kU * kStatsThreads<T>) {
-    uint4 q[kU];
+  constexpr int kU = 4;  // vectors that are on their way while as many are worked on
+  uint4 q[kU], next[kU];
+  auto load = [&](uint4 (&r)[kU], int i) {
 #pragma unroll
     for (int u = 0; u < kU; ++u)
-      if (i + u * kStatsThreads<T> < v1) q[u] = xv[i + u * kStatsThreads<T>];
+      if (i + u * kStatsThreads<T> < v1) r[u] = xv[i + u * kStatsThreads<T>];
+  };
+  load(q, v0 + threadIdx.x);
+  for (int i = v0 + threadIdx.x; i < v1; i += kU * kStatsThreads<T>) {
+    load(next, i + kU * kStatsThreads<T>);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       if (i + u * kStatsThreads<T> >= v1) break;
@@ -91,6 +95,8 @@ __global__ void __launch_bounds__(kStatsThreads<T>) stats_kernel(const Params p)
       a.s = fmaf(a.s, ex2((a.m - z) * kLog2e), s);
       a.m = m;
     }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) q[u] = next[u];
   }
   if (split == 0)
     for (int i = threadIdx.x; i < head; i += kStatsThreads<T>) add1(ld_f32(x + i));
