@@ -12,8 +12,9 @@ namespace mm {
 namespace pref {
 
 constexpr int kThreads = 512;
-// Forward with the loss, repeated on the same rows: 8200 rows of 50280 bf16 values in blocks of 64, 128, 256 and 512 threads 151, 149, 163 and
-// 190 us (without loading ahead 152, 149, 157, 189), 1865 rows of 50277 float32 values in 128, 256 and 512 81, 77 and 81.
+// Forward with the loss, repeated on the same rows: 8200 rows of 50280 bf16 values in blocks of 64, 128, 256 and 512
+// threads 151, 149, 163 and 190 us (without loading ahead 152, 149, 157, 189), 1865 rows of 50277 float32 values in
+// 128, 256 and 512 81, 77 and 81.
 template <typename T> constexpr int kStatsThreads = sizeof(T) == 4 ? 256 : 128;
 
 struct Params {
