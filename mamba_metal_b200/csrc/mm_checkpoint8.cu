@@ -16,9 +16,10 @@ struct Params {
 
 // Time contiguous: a lane takes 8 consecutive values, so four lanes share a block and agree on its maximum by
 // two shuffles. A warp covers CPT * 256 values of one row, with all its loads in flight before the first is used:
-// memory is the bound, and bytes in flight decide (bf16 10240 x 32768, packed and restored: CPT 1 625 us, 2 450, 4 370:
-// 1.02 GB each way, 5.5 TB/s; in blocks of 512 threads 390). Short rows take CPT 1, or half their warps had nothing
-// to do. ACCESS: that of x; codes are taken by 8-byte words but for kAnyStride.
+// memory is the bound, and bytes in flight decide (bf16 10240 x 32768: packed in 170 us and restored in 163, 1.02 GB
+// each way, 6.0 and 6.2 TB/s. Before the codes were made and read without conversion instructions, together: CPT 4
+// 370, 2 450, 1 625; blocks of 512 threads 390). Short rows take CPT 1, or half their warps had nothing to do.
+// ACCESS: that of x; codes are taken by 8-byte words but for kAnyStride.
 template <typename T, bool PACK, int ACCESS, int CPT>
 __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per_row) {
   const int lane = threadIdx.x & 31;
@@ -40,18 +41,20 @@ __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
       const int t = begin + j * 256, n = min(8, p.length - t);  // values of this lane; none past the row's end
-      unsigned m = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) m = max(m, ck_abs_bits(raw_at(raw[j], k)));
+      unsigned m = ck_max_bits(raw[j]);
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
       if (n <= 0) continue;
       const unsigned byte = ck_exponent(m);
       const float inv = ck_inverse_scale(byte);
       if ((lane & 3) == 0) exps[(long long)(t / kCkBlock) * p.es[2]] = (uint8_t)byte;
-      int c[8];
+      unsigned c[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) c[k] = ck_code(raw_at(raw[j], k), inv);
+      for (int k = 0; k < 8; k += 2) {
+        const uint2 w = ck_code_pair(f2_pack(raw_at(raw[j], k), raw_at(raw[j], k + 1)), f2_pack(inv, inv));
+        c[k] = w.x;
+        c[k + 1] = w.y;
+      }
       if (ACCESS != kAnyStride && n == 8) {
         __stcs(reinterpret_cast<uint2*>(codes + t), make_uint2(ck_pack4(c[0], c[1], c[2], c[3]), ck_pack4(c[4], c[5], c[6], c[7])));
       } else {
@@ -76,12 +79,14 @@ __global__ void __launch_bounds__(256) rows_kernel(const Params p, int warps_per
     for (int j = 0; j < CPT; ++j) {
       const int t = begin + j * 256, n = min(8, p.length - t);
       float v[8];
-      const float scale = ck_scale(__shfl_sync(0xffffffffu, mine, (lane & ~3) | j));
+      const unsigned byte = __shfl_sync(0xffffffffu, mine, (lane & ~3) | j);
+      const float scale = ck_scale(byte);
       if (ACCESS != kAnyStride && n == 8) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[k] = ck_restore<T>(ck_byte(raw[j].x, k), scale);
-          v[k + 4] = ck_restore<T>(ck_byte(raw[j].y, k), scale);
+        for (int k = 0; k < 8; ++k) v[k] = ck_value(k < 4 ? raw[j].x : raw[j].y, k & 3) * scale;
+        if (!ck_in_range<T>(byte)) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = ck_restore<T>(v[k], 1.f);
         }
       } else {
 #pragma unroll

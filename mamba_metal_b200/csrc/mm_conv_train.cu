@@ -60,9 +60,9 @@ MM_DEV f2_t taps(const f2_t (&w)[kW], f2_t bias, f2_t a, f2_t b, f2_t c, f2_t d)
 // ---- time contiguous --------------------------------------------------------------------------------
 // A warp covers CPT * 256 consecutive steps of one row: chunk j of lane l are the 8 steps from 256 j + 8 l. All
 // its loads are in flight before the first is used, 8 KB a warp at CPT 4 (f16 8x1536x4096, CPT 1 and 4: forward 84
-// and 62 us, the latter 4.1 TB/s). Halos come from the neighbouring lanes, and for the warp's first and last lane
+// and 62 us; 58 now, 4.4 TB/s). Halos come from the neighbouring lanes, and for the warp's first and last lane
 // from memory. Rows of up to 512 steps take CPT 1, or half their warps had nothing to do. Rows off a 16-byte boundary
-// (bf16 4x5120x5601: forward 271 us, backward 398) pay for the shifting of words, two thirds more than aligned ones.
+// (bf16 4x5120x5601: forward 264 us, backward 398) pay for the shifting of words, two thirds more than aligned ones.
 
 template <typename T, int ACCESS, int CPT>
 __global__ void __launch_bounds__(256) fwd_rows_kernel(const Params p, int warps_per_row) {
@@ -91,12 +91,9 @@ __global__ void __launch_bounds__(256) fwd_rows_kernel(const Params p, int warps
   for (int j = 0; j < CPT; ++j) {
     const int t0 = begin + j * 256 + lane * kE, n = min(kE, p.seqlen - t0);
     float win[kE + 3];
-    unsigned m = 0;
+    unsigned m = ck_max_bits(x[j]);
 #pragma unroll
-    for (int k = 0; k < kE; ++k) {
-      win[k + 3] = raw_at(x[j], k);
-      m = max(m, ck_abs_bits(win[k + 3]));
-    }
+    for (int k = 0; k < kE; ++k) win[k + 3] = raw_at(x[j], k);
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       const float v = __shfl_sync(0xffffffffu, win[kE + k], (lane + 31) & 31);  // lane 0 takes lane 31's for the next chunk
@@ -151,7 +148,7 @@ template <typename T, bool CK> struct Source {
     Raw8<T> x;
     uint2 c;
     float scale;
-    MM_DEV float at(int k) const { return CK ? (float)ck_byte(k < 4 ? c.x : c.y, k & 3) * scale : raw_at(x, k); }
+    MM_DEV float at(int k) const { return CK ? ck_converted(k < 4 ? c.x : c.y, k & 3) * scale : raw_at(x, k); }
   };
   MM_DEV Eight load(int t0, int access, int n) const {
     Eight r = {};
@@ -378,7 +375,7 @@ __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int ru
     for (int c = 0; c < H; ++c) win[j][c] = both(0.f);
     if (k.t0 > 0) load_few<T, VEC>(x + (long long)(k.t0 - 3 + j) * p.xs[2], k.step * p.xs[1], k.n, win[j]);
   }
-  // Twice over each block: for its maxima, then, out of L1, for everything else (bf16 4x5120x5601 198 us, 2.9 TB/s;
+  // Twice over each block: for its maxima, then, out of L1, for everything else (bf16 4x5120x5601 187 us, 3.1 TB/s;
   // the block held in registers instead leaves 8 warps an SM, 255 us).
   for (int tb = k.t0; tb < k.t1; tb += kCkBlock) {
     const int n = min(kCkBlock, k.t1 - tb);
@@ -452,7 +449,7 @@ __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int
   };
   auto code_row = [&](int t) { return load_bytes<C, VEC>(codes + (long long)t * p.cs[2], k.step * p.cs[1], k.n); };
   auto value = [&](unsigned v, int c) {
-    return f2_mul(f2_pack((float)ck_byte(v, 2 * c), (float)ck_byte(v, 2 * c + 1)), scale[c]);
+    return f2_mul(f2_pack(ck_converted(v, 2 * c), ck_converted(v, 2 * c + 1)), scale[c]);
   };
   if (CK && k.t0 > 0) scales(k.t0 - 1);
 #pragma unroll
