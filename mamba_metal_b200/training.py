@@ -145,6 +145,13 @@ class Checkpoint8:
     exponents: torch.Tensor
     dtype: torch.dtype
 
+    def __post_init__(self):
+        # the kernels go by the codes' shape alone: fewer exponents than that asks for would be read past their end
+        shape = self.codes.shape
+        assert len(shape) >= 1 and self.exponents.shape == (*shape[:-1], -(-shape[-1] // CHECKPOINT8_BLOCK)), \
+            "exponents are one for every 32 codes of the last axis"
+        assert self.codes.dtype == torch.int8 and self.exponents.dtype == torch.uint8
+
     @property
     def shape(self) -> torch.Size:
         return self.codes.shape
