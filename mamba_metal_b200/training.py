@@ -230,7 +230,7 @@ def causal_conv1d_backward(dout: torch.Tensor, x: torch.Tensor | Checkpoint8, we
     assert weight.numel() == dim * ops.D_CONV and (bias is None or tuple(bias.shape) == (dim,))
     if dout.dtype not in _lib.DTYPE_CODE:
         raise TypeError(f"unsupported dtype {dout.dtype}")
-    dev = _lib.require_cuda(dout, src, weight, bias)
+    dev = _lib.require_cuda(dout, src, x.exponents if held else None, weight, bias)
     w, b = _f32(weight), _f32(bias)
     by_channel = _by_channel(src)
     dout = _laid_out(dout, by_channel)
@@ -292,7 +292,7 @@ def selective_scan_backward(dy: torch.Tensor, u, delta, A, B, C, *, D=None, z=No
     ``selective_scan_states`` returned for the same inputs; without it they are computed again. Returns a dict of
     "u", "delta", "B", "C", "z" (that dtype; "z" None without z) and "A", "D", "delta_bias" (float32; None where
     not given)."""
-    dev = _lib.require_cuda(dy, u, delta, A, B, C, D, z, delta_bias, dstate)
+    dev = _lib.require_cuda(dy, u, delta, A, B, C, D, z, delta_bias, dstate, states)
     batch, dim, seqlen = u.shape
     n = A.shape[1]
     assert dy.shape == u.shape == delta.shape and tuple(B.shape) == (batch, n, seqlen) == tuple(C.shape)
@@ -307,7 +307,7 @@ def selective_scan_backward(dy: torch.Tensor, u, delta, A, B, C, *, D=None, z=No
     if states is None:
         states = selective_scan_states(u, delta, A, B, C, D=D, z=z, delta_bias=delta_bias, delta_softplus=delta_softplus,
                                        outputs=False)[2]
-    assert states.dtype == torch.float32 and states.is_contiguous() and states.is_cuda
+    assert states.dtype == torch.float32 and states.is_contiguous()
     by_channel = _by_channel(u)
     dy = _laid_out(dy, by_channel)
     act = lambda: _empty(u.shape, u.dtype, dev, by_channel)

@@ -75,6 +75,28 @@ def test_checkpoint_parts_that_do_not_belong_together_are_refused():
             training.Checkpoint8(c, e, torch.float32)
 
 
+def test_everything_that_a_kernel_reads_is_asked_for_its_device(monkeypatch):
+    """Exponents and states too: a pointer of another GPU would be read by this one's kernel."""
+    class Stop(Exception):
+        pass
+
+    def stop(*tensors):
+        asked.extend(id(t) for t in tensors)
+        raise Stop
+
+    monkeypatch.setattr(_lib, "require_cuda", stop)
+    u, A, B = torch.zeros(1, 2, 40), torch.zeros(2, 4), torch.zeros(1, 4, 40)
+    states, w = torch.zeros(16), torch.zeros(2, 4)
+    c = training.Checkpoint8(torch.zeros(1, 2, 40, dtype=torch.int8), torch.zeros(1, 2, 2, dtype=torch.uint8), u.dtype)
+    for call, read in ((lambda: training.selective_scan_backward(u, u, u, A, B, B, states=states), (u, A, B, states)),
+                       (lambda: training.causal_conv1d_backward(u, c, w, None), (u, c.codes, c.exponents, w)),
+                       (c.restore, (c.codes, c.exponents))):
+        asked = []
+        with pytest.raises(Stop):
+            call()
+        assert all(id(t) in asked for t in read)
+
+
 def test_c_entries_refuse():
     lib = _lib.lib()
     c = _lib.MMCheckpoint8Args()
