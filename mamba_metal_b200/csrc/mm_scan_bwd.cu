@@ -659,6 +659,16 @@ int make_layout(const MMScanBwdArgs* a, Layout* l) {
   return MM_OK;
 }
 
+template <typename T> int reduce(const Params& p, cudaStream_t s) {
+  static_assert(kT == 32, "a warp of reduce_kernel is a chunk of a state");
+  const long long rows = (long long)p.batch * p.chunks;
+  const long long bc = (rows * p.passes * kNB * (p.groups > 16 ? 8 : 1) + 7) / 8;
+  const long long rest = ((long long)p.dim * (p.np + 2) + 31) / 32;
+  if (bc + rest > 0x7fffffffLL) return MM_ERR_SHAPE;
+  reduce_kernel<T><<<(unsigned)(bc + rest), 256, 0, s>>>(p, bc);
+  return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
+}
+
 template <typename T, bool HAS_Z> int launch(const Params& p, int64_t dtype, cudaStream_t s) {
   const long long rows = (long long)p.batch * p.chunks;
   if (rows * p.groups > 0x7fffffffLL) return MM_ERR_SHAPE;
@@ -675,16 +685,11 @@ template <typename T, bool HAS_Z> int launch(const Params& p, int64_t dtype, cud
       return MM_ERR_LAUNCH;
     grad_kernel<T, HAS_Z><<<(unsigned)(rows * p.groups), kGradThreads, kGradSmem<T>, s>>>(p);
   }
-  if (cudaGetLastError() != cudaSuccess) return MM_ERR_LAUNCH;
-  static_assert(kT == 32, "a warp of reduce_kernel is a chunk of a state");
-  const long long bc = (rows * p.passes * kNB * (p.groups > 16 ? 8 : 1) + 7) / 8;
-  const long long rest = ((long long)p.dim * (p.np + 2) + 31) / 32;
-  if (bc + rest > 0x7fffffffLL) return MM_ERR_SHAPE;
-  reduce_kernel<T><<<(unsigned)(bc + rest), 256, 0, s>>>(p, bc);
-  return cudaGetLastError() == cudaSuccess ? MM_OK : MM_ERR_LAUNCH;
+  return cudaGetLastError() == cudaSuccess ? reduce<T>(p, s) : MM_ERR_LAUNCH;
 }
 
 template <typename T> int launch_z(const Params& p, int64_t dtype, cudaStream_t s) {
+  if (p.dim == 0) return reduce<T>(p, s);  // dB and dC are sums over no channels
   return p.z ? launch<T, true>(p, dtype, s) : launch<T, false>(p, dtype, s);
 }
 
@@ -714,18 +719,19 @@ extern "C" int mm_selective_scan_bwd(const MMScanBwdArgs* a, void* workspace, si
   if (rc != MM_OK) return rc;
   const MMScanArgs& f = a->fwd;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (f.dim == 0) return MM_OK;
-  if (!a->dA) return MM_ERR_ARG;
+  if (f.dim > 0 && !a->dA) return MM_ERR_ARG;
   if (f.batch == 0 || f.seqlen == 0) {  // sums over nothing
+    if (f.dim == 0) return MM_OK;
     if (cudaMemsetAsync(a->dA, 0, sizeof(float) * f.dim * f.dstate, s) != cudaSuccess) return MM_ERR_LAUNCH;
     if (a->dD && cudaMemsetAsync(a->dD, 0, sizeof(float) * f.dim, s) != cudaSuccess) return MM_ERR_LAUNCH;
     if (a->ddelta_bias && cudaMemsetAsync(a->ddelta_bias, 0, sizeof(float) * f.dim, s) != cudaSuccess) return MM_ERR_LAUNCH;
     return MM_OK;
   }
-  if (!f.u || !f.delta || !f.A || !f.B || !f.C || !a->dy || !a->du || !a->ddelta || !a->dB || !a->dC || (f.z && !a->dz))
+  if (!a->dB || !a->dC) return MM_ERR_ARG;
+  if (f.dim > 0 && (!f.u || !f.delta || !f.A || !f.B || !f.C || !a->dy || !a->du || !a->ddelta || (f.z && !a->dz)))
     return MM_ERR_ARG;
   if (!workspace || workspace_bytes < l.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return MM_ERR_WORKSPACE;
-  if (chunks_of(f) > 1 && (!a->states || reinterpret_cast<uintptr_t>(a->states) % 16)) return MM_ERR_ARG;
+  if (f.dim > 0 && chunks_of(f) > 1 && (!a->states || reinterpret_cast<uintptr_t>(a->states) % 16)) return MM_ERR_ARG;
   Params p = {};
   set_inputs(p, f);
   p.dy = a->dy;

@@ -131,3 +131,13 @@ def test_c_entries_refuse():
     rc, one = size_of(lib.mm_selective_scan_bwd_workspace_size, s)
     s.fwd.seqlen = 65
     assert rc == 0 and size_of(lib.mm_selective_scan_bwd_workspace_size, s)[1] > one > 0
+
+
+def test_scan_gradient_of_no_channels_asks_for_what_it_clears():
+    """dB and dC have a size of their own; with no channels they are zeros that the call has to write."""
+    s = _lib.MMScanBwdArgs()
+    s.fwd.dtype, s.fwd.batch, s.fwd.dim, s.fwd.dstate, s.fwd.seqlen = 1, 2, 0, 4, 40
+    lib = _lib.lib()
+    assert lib.mm_selective_scan_bwd(ctypes.byref(s), None, 0, None) == -1
+    s.fwd.seqlen = 0
+    assert lib.mm_selective_scan_bwd(ctypes.byref(s), None, 0, None) == 0

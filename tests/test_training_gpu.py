@@ -270,6 +270,22 @@ def test_empty_sequences():
     assert training.checkpoint8(torch.empty(3, 0, device=DEV)).restore().shape == (3, 0)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,length", [(4, 40), (24, 33), (16, 1)])
+def test_no_channels(n, length, dtype, monkeypatch):
+    """Gradients of B and C are sums over no channels: zeros, whatever their memory held."""
+    empty = torch.empty
+    monkeypatch.setattr(training.torch, "empty", lambda *a, **k: empty(*a, **k).fill_(7))
+    u, A = empty(2, 0, length, device=DEV, dtype=dtype), empty(0, n, device=DEV)
+    B = torch.ones(2, n, length, device=DEV, dtype=dtype)
+    for z in (None, u):
+        g = training.selective_scan_backward(u, u, u, A, B, B, z=z, delta_softplus=True)
+        assert g["B"].shape == g["C"].shape == B.shape and not g["B"].any() and not g["C"].any()
+        assert g["u"].shape == u.shape and g["A"].shape == A.shape
+    y, state = training.selective_scan(u, u, A, B, B, return_state=True)
+    assert y.shape == u.shape and state.shape == (2, 0, n)
+
+
 # ---- checkpoints -------------------------------------------------------------------------------------------
 
 
