@@ -176,6 +176,14 @@ class Checkpoint8:
         return out if self.codes.dim() <= 3 else out.view(self.shape)
 
 
+def _made(codes: torch.Tensor, exponents: torch.Tensor, dtype: torch.dtype) -> Checkpoint8:
+    """A Checkpoint8 of parts that this module made for each other; they are not checked again, which would take a short
+    call 2 us."""
+    c = object.__new__(Checkpoint8)
+    c.__dict__.update(codes=codes, exponents=exponents, dtype=dtype)
+    return c
+
+
 def _up_to_three(t: torch.Tensor) -> torch.Tensor:
     return t if t.dim() <= 3 else t.flatten(0, -3)
 
@@ -194,7 +202,7 @@ def checkpoint8(x: torch.Tensor) -> Checkpoint8:
     _run("mm_checkpoint8_pack", dev, _checkpoint_args(rows, codes, exponents))
     if x.dim() > 3:
         codes, exponents = codes.unflatten(0, x.shape[:-2]), exponents.unflatten(0, x.shape[:-2])
-    return Checkpoint8(codes, exponents, x.dtype)
+    return _made(codes, exponents, x.dtype)
 
 
 # ---- causal conv1d -----------------------------------------------------------------------------------------
@@ -216,7 +224,7 @@ def conv1d_checkpoint8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
     a = _args(_lib.MMConvCheckpointArgs, _p(x), _p(w), _p(b), _p(out), _p(codes), _p(exponents), _lib.DTYPE_CODE[x.dtype],
               *x.shape, ops.D_CONV, *x.stride(), *out.stride(), *codes.stride(), *exponents.stride(), bool(silu))
     _run("mm_causal_conv1d_fwd_checkpoint8", dev, a)
-    return out, Checkpoint8(codes, exponents, x.dtype)
+    return out, _made(codes, exponents, x.dtype)
 
 
 def causal_conv1d_backward(dout: torch.Tensor, x: torch.Tensor | Checkpoint8, weight: torch.Tensor,
@@ -263,7 +271,7 @@ class _CausalConv1d(torch.autograd.Function):
     def backward(ctx, dout):
         src, exponents, weight, bias = ctx.saved_tensors
         if ctx.held:
-            src = Checkpoint8(src, exponents, dout.dtype)
+            src = _made(src, exponents, dout.dtype)
         dx, dw, db = causal_conv1d_backward(dout, src, weight, bias, silu=ctx.silu)
         return dx, _like(dw, weight), _like(db, bias), None, None
 
@@ -533,7 +541,7 @@ class _Block(torch.autograd.Function):
         x_dbl, in_w, conv_w, conv_b, x_w, dt_w, dt_b, A_log, D, out_w, *held = ctx.saved_tensors
         E, R, N = conv_w.shape[0], dt_w.shape[1], A_log.shape[1]
         dtype = in_w.dtype
-        cx, cxt, cz, cy = (Checkpoint8(held[2 * i], held[2 * i + 1], dtype) for i in range(4))
+        cx, cxt, cz, cy = (_made(held[2 * i], held[2 * i + 1], dtype) for i in range(4))
         by_channel = _by_channel(cx.codes)
         xt, z, y = cxt.restore(), cz.restore(), cy.restore()
         xc = _empty(z.shape, dtype, z.device, by_channel)

@@ -66,7 +66,7 @@ def test_checkpoint_parts_that_do_not_belong_together_are_refused():
     """The kernels find a value's exponent by the codes' shape, so any other shape or type would be read past its end."""
     codes, exponents = torch.zeros(2, 3, 70, dtype=torch.int8), torch.zeros(2, 3, 3, dtype=torch.uint8)
     whole = training.Checkpoint8(codes, exponents, torch.float32)
-    assert whole.shape == (2, 3, 70)
+    assert whole.shape == (2, 3, 70) and whole == training._made(codes, exponents, torch.float32)
     bad = [(codes, exponents[..., :2]), (codes, exponents[:1]), (codes, exponents[:, :2]), (codes, exponents[0]),
            (codes[..., :64], exponents), (codes[..., :0], exponents), (codes.short(), exponents), (codes, exponents.short()),
            (codes.view(torch.uint8), exponents), (codes[0, 0, 0], exponents[0, 0, 0])]
