@@ -33,6 +33,14 @@ struct Params {
   int silu;
 };
 
+// A channel's four weights, in one word where they lie on 16 bytes; a parameter may also be a view into a flat buffer
+// (bf16 4x5120x5601, channels last, forward and backward: 483 us; always one by one 494)
+MM_DEV float4 weights_of(const Params& p, int d) {
+  const float* w = p.w + (long long)d * kW;
+  if ((reinterpret_cast<uintptr_t>(p.w) & 15) == 0) return *reinterpret_cast<const float4*>(w);
+  return make_float4(w[0], w[1], w[2], w[3]);
+}
+
 MM_DEV float act(float v, int silu_on) { return silu_on ? silu(v) : v; }
 // d silu(v) / dv = s (1 + v (1 - s)), s = sigmoid(v). Below -88, s is 0 and so is the product.
 MM_DEV float dact(float v, int silu_on) {
@@ -83,7 +91,7 @@ __global__ void __launch_bounds__(256) fwd_rows_kernel(const Params p, int warps
   float before[3];  // the three steps before the warp's chunk
 #pragma unroll
   for (int k = 0; k < 3; ++k) before[k] = begin > 0 ? ld_f32(xr + (long long)(begin - 3 + k) * p.xs[2]) : 0.f;
-  const float4 w = *reinterpret_cast<const float4*>(p.w + (long long)d * kW);
+  const float4 w = weights_of(p, d);
   const float bb = p.bias ? p.bias[d] : 0.f;
   T* orow = static_cast<T*>(p.out) + b * p.os[0] + d * p.os[1];
   int8_t* crow = p.codes_out + b * p.cs[0] + d * p.cs[1];
@@ -192,7 +200,7 @@ __global__ void __launch_bounds__(256) bwd_rows_kernel(const Params p, int warps
     g[j] = raw_load(grow + (long long)t * p.gs[2], p.gs[2], ACCESS, n);
   }
   float before[3], after[3];  // x before the warp's steps; dpre of the three steps that follow the chunk at hand
-  const float4 w = *reinterpret_cast<const float4*>(p.w + (long long)d * kW);
+  const float4 w = weights_of(p, d);
   const float bb = p.bias ? p.bias[d] : 0.f;
   auto pre = [&](float a, float c, float e, float f) { return fmaf(w.w, f, fmaf(w.z, e, fmaf(w.y, c, fmaf(w.x, a, bb)))); };
 #pragma unroll
@@ -351,8 +359,7 @@ template <int C> MM_DEV void load_weights(const Params& p, const Walk& k, f2_t (
 #pragma unroll
   for (int c = 0; c < C / 2; ++c) {
     const int d = min(k.d + 2 * c * k.step, p.dim - 1), e = min(k.d + (2 * c + 1) * k.step, p.dim - 1);
-    const float4 v = *reinterpret_cast<const float4*>(p.w + (long long)d * kW);
-    const float4 u = *reinterpret_cast<const float4*>(p.w + (long long)e * kW);
+    const float4 v = weights_of(p, d), u = weights_of(p, e);
     w[c][0] = f2_pack(v.x, u.x), w[c][1] = f2_pack(v.y, u.y), w[c][2] = f2_pack(v.z, u.z), w[c][3] = f2_pack(v.w, u.w);
     bb[c] = f2_pack(p.bias ? p.bias[d] : 0.f, p.bias ? p.bias[e] : 0.f);
   }
@@ -733,7 +740,7 @@ extern "C" int mm_causal_conv1d_fwd_checkpoint8(const MMConvCheckpointArgs* a, m
   const int rc = check(a->dtype, a->batch, a->dim, a->seqlen, a->width);
   if (rc != MM_OK) return rc;
   if (a->batch == 0 || a->dim == 0 || a->seqlen == 0) return MM_OK;
-  if (!a->x || !a->weight || !a->out || !a->codes || !a->exponents || !aligned16(a->weight)) return MM_ERR_ARG;
+  if (!a->x || !a->weight || !a->out || !a->codes || !a->exponents) return MM_ERR_ARG;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
     case MM_F32: return launch_fwd<float>(a, s);
@@ -764,7 +771,7 @@ extern "C" int mm_causal_conv1d_bwd(const MMConvBwdArgs* a, void* workspace, siz
     if (a->dbias && cudaMemsetAsync(a->dbias, 0, sizeof(float) * a->dim, s) != cudaSuccess) return MM_ERR_LAUNCH;
     return MM_OK;
   }
-  if ((!a->x && (!a->codes || !a->exponents)) || !a->weight || !a->dout || !a->dx || !aligned16(a->weight)) return MM_ERR_ARG;
+  if ((!a->x && (!a->codes || !a->exponents)) || !a->weight || !a->dout || !a->dx) return MM_ERR_ARG;
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return MM_ERR_WORKSPACE;
   float* part = static_cast<float*>(workspace);
   if (a->x) {

@@ -405,6 +405,26 @@ def test_conv_values_and_checkpoint_are_the_separate_operators():
     assert all(torch.equal(p, q) for p, q in zip(once, again))
 
 
+@pytest.mark.parametrize("held", [False, True])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("first", [1, 2, 3])
+def test_conv_weights_in_a_flat_buffer(first, layout, held):
+    """Weights that begin at any float of a buffer give the bits of weights of their own."""
+    g = torch.Generator().manual_seed(first)
+    d = 24
+    x, dout = put(randn(g, 2, d, 140), torch.bfloat16, layout)[0], put(randn(g, 2, d, 140), torch.bfloat16)[0]
+    flat, b = randn(g, 4 * d + 8).float().to(DEV), randn(g, d).float().to(DEV)
+    view = flat[first:first + 4 * d].view(d, 1, 4)
+    assert view.data_ptr() % 16
+    got = []
+    for w in (view, view.clone()):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        out = training.causal_conv1d(*leaves, checkpoint8=held)
+        got.append([out, *torch.autograd.grad(out, leaves, dout)])
+    for p, q in zip(*got):
+        assert torch.equal(p, q)
+
+
 def test_conv_gradient_against_differences():
     g = torch.Generator().manual_seed(2)
     x, w, b, dout = randn(g, 2, 5, 70), randn(g, 5, 4) / 2, randn(g, 5), randn(g, 2, 5, 70)
