@@ -62,15 +62,18 @@ MM_DEV float ck_value(unsigned w, int i) {
 }
 
 // The element of type T that a code stands for: exact, except past T's largest finite value, which is
-// restored instead (amax near the top of the range can round up to a code past it).
+// restored instead (amax near the top of the range can round up to a code past it). Every reader of codes goes by this
+// or, where a block is known to stay in range, by the product alone.
 template <typename T> struct CkMax;
 template <> struct CkMax<float> { static constexpr float v = 3.40282347e38f; };
 template <> struct CkMax<__half> { static constexpr float v = 65504.f; };
 template <> struct CkMax<__nv_bfloat16> { static constexpr float v = 3.38953139e38f; };
-template <typename T> MM_DEV float ck_restore(float code, float scale) {
-  const float v = code * scale;
-  return v > CkMax<T>::v ? CkMax<T>::v : v < -CkMax<T>::v ? -CkMax<T>::v : v;  // NaN passes both
+template <typename T> MM_DEV float ck_limited(float v) {  // the lesser of the magnitudes, v's sign; NaN stays
+  float r;
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(CkMax<T>::v));
+  return r;
 }
+template <typename T> MM_DEV float ck_restore(float code, float scale) { return ck_limited<T>(code * scale); }
 
 // Whether no code of such a block stands for more than that (127 2^9 = 65024, 127 2^121 = 0x1.fcp127)
 template <typename T> MM_DEV bool ck_in_range(unsigned byte) { return byte <= (std::is_same<T, __half>::value ? 136u : 248u); }

@@ -149,14 +149,14 @@ template <typename T, bool CK> struct Source {
     }
   }
   MM_DEV float at(int t) const {
-    return CK ? (float)codes[t * cs] * ck_scale(exps[(long long)(t / kCkBlock) * es]) : ld_f32(x + t * xs);
+    return CK ? ck_restore<T>((float)codes[t * cs], ck_scale(exps[(long long)(t / kCkBlock) * es])) : ld_f32(x + t * xs);
   }
-  // eight steps as they lie in memory, their scale (1 for the input itself), and a value of them
+  // eight steps as they lie in memory, their scale, and a value of them
   struct Eight {
     Raw8<T> x;
     uint2 c;
     float scale;
-    MM_DEV float at(int k) const { return CK ? ck_converted(k < 4 ? c.x : c.y, k & 3) * scale : raw_at(x, k); }
+    MM_DEV float at(int k) const { return CK ? ck_restore<T>(ck_converted(k < 4 ? c.x : c.y, k & 3), scale) : raw_at(x, k); }
   };
   MM_DEV Eight load(int t0, int access, int n) const {
     Eight r = {};
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int ru
 
 // Backward: step t completes dx[t-3] from the last four dpre; three steps past the run finish its end. Only the
 // run's own steps enter the sums. The loads of the next eight steps are in flight while eight are worked on; two
-// CTAs of an SM (128 registers) hide them best (bf16 4x5120x5601 from the checkpoint 271 us, 2.1 TB/s; what bounds it is
+// CTAs of an SM (128 registers) hide them best (bf16 4x5120x5601 from the checkpoint 246 us, 2.4 TB/s; what bounds it is
 // the instructions of an element, as above).
 template <typename T, bool CK, bool VEC>
 __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int run, int runs) {
@@ -456,7 +456,8 @@ __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int
   };
   auto code_row = [&](int t) { return load_bytes<C, VEC>(codes + (long long)t * p.cs[2], k.step * p.cs[1], k.n); };
   auto value = [&](unsigned v, int c) {
-    return f2_mul(f2_pack(ck_converted(v, 2 * c), ck_converted(v, 2 * c + 1)), scale[c]);
+    const float2 x = f2_unpack(f2_mul(f2_pack(ck_converted(v, 2 * c), ck_converted(v, 2 * c + 1)), scale[c]));
+    return f2_pack(ck_limited<T>(x.x), ck_limited<T>(x.y));
   };
   if (CK && k.t0 > 0) scales(k.t0 - 1);
 #pragma unroll

@@ -425,6 +425,28 @@ def test_conv_weights_in_a_flat_buffer(first, layout, held):
         assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("shape", [(1, 8, 70), (2, 9, 700), (1, 130, 333)])
+def test_conv_gradient_at_the_largest_values(shape, layout, dtype):
+    """Where a code stands for more than the type's largest value, the gradient is taken at that value, as restored: the
+    bits are those of the gradient at the restored tensor."""
+    b, d, n = shape
+    g = torch.Generator().manual_seed(d)
+    x = randn(g, *shape)
+    x[:, ::3, ::37] = float(torch.finfo(dtype).max)
+    x[:, 1::3, 30::41] = -float(torch.finfo(dtype).max)
+    x, dout = put(x, dtype, layout)[0], put(0.01 * randn(g, *shape), dtype)[0]
+    c = training.checkpoint8(x)
+    at = c.restore()
+    assert at.isfinite().all() and at.abs().max() == torch.finfo(dtype).max
+    w, bias = (0.2 * randn(g, d, 4)).clamp(-0.2, 0.2).float().to(DEV), randn(g, d).float().to(DEV)
+    for silu in (True, False):
+        for p, q in zip(training.causal_conv1d_backward(dout, c, w, bias, silu=silu),
+                        training.causal_conv1d_backward(dout, at, w, bias, silu=silu)):
+            assert p.isfinite().all() and torch.equal(p, q)
+
+
 def test_conv_gradient_against_differences():
     g = torch.Generator().manual_seed(2)
     x, w, b, dout = randn(g, 2, 5, 70), randn(g, 5, 4) / 2, randn(g, 5), randn(g, 2, 5, 70)
