@@ -18,6 +18,7 @@ from functools import lru_cache
 
 import torch
 import torch.nn.functional as F
+from torch.amp import custom_bwd, custom_fwd
 from torch.autograd.function import once_differentiable
 
 from mamba_metal_b200 import _lib, ops
@@ -513,9 +514,11 @@ def _outer(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
 
 class _Block(torch.autograd.Function):
     """MambaBlock.forward that keeps its activations (its input, the conv's, the gate, the scan's output) in 8 bits and
-    computes the rest again in the backward pass, from the values they stand for."""
+    computes the rest again in the backward pass, from the values they stand for. Under autocast the projections give
+    activations of its type, and the backward pass runs under it as well."""
 
     @staticmethod
+    @custom_fwd(device_type="cuda")
     def forward(ctx, x, in_w, conv_w, conv_b, x_w, dt_w, dt_b, A_log, D, out_w, by_channel):
         E, R, N = conv_w.shape[0], dt_w.shape[1], A_log.shape[1]
         dtype = in_w.dtype
@@ -530,18 +533,19 @@ class _Block(torch.autograd.Function):
                                         delta_softplus=True)
         out = _proj(out_w, y).transpose(1, 2)
         held = [cx, checkpoint8(xt), checkpoint8(xz[:, E:]), checkpoint8(y)]
-        ctx.x_dtype = x.dtype
+        ctx.x_dtype, ctx.dtypes = x.dtype, tuple(c.dtype for c in held)
         ctx.save_for_backward(x_dbl, in_w, conv_w, conv_b, x_w, dt_w, dt_b, A_log, D, out_w,
                               *(t for c in held for t in (c.codes, c.exponents)))
         return out
 
     @staticmethod
     @once_differentiable
+    @custom_bwd(device_type="cuda")
     def backward(ctx, dout):
         x_dbl, in_w, conv_w, conv_b, x_w, dt_w, dt_b, A_log, D, out_w, *held = ctx.saved_tensors
         E, R, N = conv_w.shape[0], dt_w.shape[1], A_log.shape[1]
-        dtype = in_w.dtype
-        cx, cxt, cz, cy = (_made(held[2 * i], held[2 * i + 1], dtype) for i in range(4))
+        cx, cxt, cz, cy = (_made(held[2 * i], held[2 * i + 1], t) for i, t in enumerate(ctx.dtypes))
+        dtype = cx.dtype  # of the activations
         by_channel = _by_channel(cx.codes)
         xt, z, y = cxt.restore(), cz.restore(), cy.restore()
         xc = _empty(z.shape, dtype, z.device, by_channel)
@@ -559,8 +563,9 @@ class _Block(torch.autograd.Function):
         dxz = _laid_out(torch.cat([dx_in, g["z"]], 1), by_channel)
         d_in_w = _outer(dxz, xt)
         dx = _proj(in_w.t(), dxz).transpose(1, 2)
-        return (_cast(dx, ctx.x_dtype), d_in_w, _like(dw, conv_w), _like(db, conv_b), d_x_w, d_dt_w, _like(g["delta_bias"], dt_b),
-                _cast(g["A"] * A, A_log.dtype), _like(g["D"], D), d_out_w, None)
+        return (_cast(dx, ctx.x_dtype), _like(d_in_w, in_w), _like(dw, conv_w), _like(db, conv_b), _like(d_x_w, x_w),
+                _like(d_dt_w, dt_w), _like(g["delta_bias"], dt_b), _cast(g["A"] * A, A_log.dtype), _like(g["D"], D),
+                _like(d_out_w, out_w), None)
 
 
 def mamba_block(block, x: torch.Tensor, checkpoint8: bool = True) -> torch.Tensor:

@@ -77,6 +77,37 @@ def test_block_values_are_the_inference_blocks():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("low", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("length", [33, 64])
+def test_block_under_autocast(length, low):
+    """float32 parameters, activations of the autocast type; the backward pass called outside. Gradients from 8-bit
+    activations against those without: 2.8e-2 as above, and the type's own factor for what is computed again in it."""
+    block = make_block(torch.float32)
+    g = torch.Generator().manual_seed(length)
+    x, dy = torch.randn(2, length, 40, generator=g).to(DEV), torch.randn(2, length, 40, generator=g).to(DEV)
+    outs, grads = [], []
+    for held in (True, False):
+        leaf = x.detach().requires_grad_(True)
+        with torch.autocast("cuda", dtype=low):
+            outs.append(block.forward_train(leaf, checkpoint8=held))
+        grads.append(torch.autograd.grad(outs[-1], [leaf, *block.parameters()], dy.to(outs[-1].dtype)))
+    assert outs[0].dtype == low and torch.equal(*outs)
+    for n, a, r in zip(["x", *(n for n, _ in block.named_parameters())], *grads):
+        assert a.dtype == torch.float32 and a.shape == r.shape
+        assert_close_lowp(a, r, f"d{n}", rel_l2=2.8e-2 + RTOL[str(low).split(".")[-1]])
+
+
+def test_model_trains_under_autocast():
+    cfg = MambaConfig(d_model=64, n_layer=2, vocab_size=50)
+    model = init_weights_(MambaModel(cfg, dtype=torch.float32, device=DEV), seed=1)
+    ids = torch.randint(0, 50, (2, 40), device=DEV)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = model.forward_train(ids, checkpoint8=True).float().square().mean()
+    loss.backward()
+    for n, p in model.named_parameters():
+        assert p.grad is not None and p.grad.dtype == p.dtype and torch.isfinite(p.grad).all() and p.grad.abs().max() > 0, n
+
+
 def test_rms_norm_gradient():
     g = torch.Generator().manual_seed(3)
     x, w, dy = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((3, 5, 96), (96,), (3, 5, 96)))
