@@ -121,15 +121,16 @@ def _checkpoint_args(x, codes, exponents):
 
 
 def _checkpoint_buffers(shape, device, by_channel: bool):
-    """Codes and exponents for a tensor of up to three axes, laid out like it. Rows of codes start on multiples of the
-    block, so that they can be written and read in vectors whatever the length."""
+    """Codes and exponents for a tensor of up to three axes, laid out like it. Rows of codes of eight values or more start
+    on multiples of eight bytes, so that they can be written and read in vectors whatever the length; shorter rows have
+    no vectors. So codes and exponents never take up more than 16 bits a value."""
     n = shape[-1]
     blocks = -(-n // CHECKPOINT8_BLOCK)
     if by_channel:
         lead, d = tuple(shape[:-2]), shape[-2]
         return (torch.empty((*lead, n, d), dtype=torch.int8, device=device).transpose(-1, -2),
                 torch.empty((*lead, blocks, d), dtype=torch.uint8, device=device).transpose(-1, -2))
-    pitch, strides = blocks * CHECKPOINT8_BLOCK, [1]
+    pitch, strides = n if n < 8 else (n + 7) // 8 * 8, [1]
     for size in reversed(shape[1:]):
         strides.insert(0, strides[0] * (pitch if len(strides) == 1 else size))
     return (torch.empty_strided(shape, strides, dtype=torch.int8, device=device),
@@ -159,7 +160,8 @@ class Checkpoint8:
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.exponents.numel()
+        """Bytes that codes and exponents take up, with what lies between their rows."""
+        return _span(self.codes) + _span(self.exponents)
 
     def restore(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The values, in ``dtype`` (default: the packed tensor's), laid out like the packed tensor. Exact, but for
@@ -175,6 +177,11 @@ class Checkpoint8:
             out = torch.empty(codes.shape, dtype=dtype, device=dev)
         _run("mm_checkpoint8_unpack", dev, _checkpoint_args(out, codes, exponents))
         return out if self.codes.dim() <= 3 else out.view(self.shape)
+
+
+def _span(t: torch.Tensor) -> int:
+    """Elements from the first to the last of ``t`` in memory."""
+    return 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else 0
 
 
 def _made(codes: torch.Tensor, exponents: torch.Tensor, dtype: torch.dtype) -> Checkpoint8:

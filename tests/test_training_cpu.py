@@ -75,6 +75,21 @@ def test_checkpoint_parts_that_do_not_belong_together_are_refused():
             training.Checkpoint8(c, e, torch.float32)
 
 
+@pytest.mark.parametrize("by_channel", [False, True])
+def test_checkpoints_of_short_rows(by_channel):
+    """At no length do codes and exponents take up more than 16 bits a value, and ``nbytes`` says what they take up, but for
+    the padding after the last row."""
+    for n in [*range(1, 80), 255, 257, 5601]:
+        codes, exponents = training._checkpoint_buffers((2, 96, n), "cpu", by_channel)
+        c = training.Checkpoint8(codes, exponents, torch.bfloat16)
+        held = codes.untyped_storage().nbytes() + exponents.untyped_storage().nbytes()
+        assert held <= 2 * 2 * 96 * n
+        assert held - 8 < c.nbytes <= held
+        assert by_channel or n < 8 or all(s % 8 == 0 for s in codes.stride()[:2])
+    codes, exponents = training._checkpoint_buffers((3, 0), "cpu", False)
+    assert training.Checkpoint8(codes, exponents, torch.float32).nbytes == 0
+
+
 def test_everything_that_a_kernel_reads_is_asked_for_its_device(monkeypatch):
     """Exponents and states too: a pointer of another GPU would be read by this one's kernel."""
     class Stop(Exception):
