@@ -192,9 +192,10 @@ class MambaBlock(nn.Module):
         """x: (B, L, d_model) -> (B, L, d_model) (mamba_block.py:68-102)."""
         return self._run(x, want_state=False)[0]
 
-    def forward_train(self, x: torch.Tensor, checkpoint8: bool = True) -> torch.Tensor:
+    def forward_train(self, x: torch.Tensor, checkpoint8: bool = False) -> torch.Tensor:
         """``forward`` with gradients for x and the parameters; with ``checkpoint8`` the activations that the
-        backward pass needs are held in 8 bits (``mamba_metal_b200.training``)."""
+        backward pass needs are held in 8 bits, and the gradients are those at the values that these stand for
+        (``mamba_metal_b200.training``)."""
         from mamba_metal_b200 import training
 
         return training.mamba_block(self, x, checkpoint8)

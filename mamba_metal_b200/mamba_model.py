@@ -119,9 +119,10 @@ class MambaModel(nn.Module):
         """input_ids: (B, L) -> logits (B, L, vocab_size)."""
         return self._stack(input_ids, "forward")[0]
 
-    def forward_train(self, input_ids: torch.Tensor, checkpoint8: bool = True) -> torch.Tensor:
+    def forward_train(self, input_ids: torch.Tensor, checkpoint8: bool = False) -> torch.Tensor:
         """``forward`` with gradients for all parameters: input_ids (B, L) -> logits (B, L, vocab_size). With
-        ``checkpoint8`` every block holds the activations that its backward pass needs in 8 bits."""
+        ``checkpoint8`` every block holds the activations that its backward pass needs in 8 bits, and its gradients
+        are those at the values that these stand for. Every norm keeps the float32 residual that it reads."""
         from mamba_metal_b200 import training
 
         eps = self.cfg.rms_norm_eps

@@ -575,11 +575,13 @@ class _Block(torch.autograd.Function):
                 _like(d_out_w, out_w), None)
 
 
-def mamba_block(block, x: torch.Tensor, checkpoint8: bool = True) -> torch.Tensor:
+def mamba_block(block, x: torch.Tensor, checkpoint8: bool = False) -> torch.Tensor:
     """Differentiable ``MambaBlock`` forward: x (batch, length, d_model) to the same, with gradients for x and all of the
-    block's parameters (``MambaBlock.forward_train`` calls it). With ``checkpoint8`` the activations that the
-    backward pass needs are held in 8 bits, about 1.03 bytes an element of its input, the conv's input, the gate and
-    the scan's output; without it autograd holds them, and every intermediate, as they are."""
+    block's parameters (``MambaBlock.forward_train`` calls it). Autograd holds the activations that the backward pass
+    needs, and every intermediate, as they are. With ``checkpoint8`` its input, the conv's input, the gate and the
+    scan's output are held in 8 bits instead (1.03 bytes an element, a little more for rows of few steps, and
+    never more than two), and the rest is computed again; the output is the same, the gradients are those at the
+    values that the 8 bits stand for."""
     if block.tp_reduce is not None:
         raise ValueError("tensor-parallel blocks have no training pass")
     _lib.require_cuda(x, block.in_proj.weight)

@@ -108,6 +108,21 @@ def test_model_trains_under_autocast():
         assert p.grad is not None and p.grad.dtype == p.dtype and torch.isfinite(p.grad).all() and p.grad.abs().max() > 0, n
 
 
+def test_exact_activations_are_the_default():
+    """A lossy form is asked for: by default the gradients are those of the activations as they are."""
+    cfg = MambaConfig(d_model=64, n_layer=2, vocab_size=50)
+    model = init_weights_(MambaModel(cfg, dtype=torch.float32, device=DEV), seed=2)
+    ids = torch.randint(0, 50, (2, 40), device=DEV)
+    x = torch.randn(2, 40, 64, device=DEV)
+    grads = []
+    for asked in ({}, {"checkpoint8": False}):
+        loss = model.forward_train(ids, **asked).square().mean() + model.layers[0].mixer.forward_train(x, **asked).square().mean()
+        grads.append(torch.autograd.grad(loss, list(model.parameters())))
+    # the embeddings' gradient is torch's own, whose order of additions is free
+    for (n, _), a, b in zip(model.named_parameters(), *grads):
+        assert n.startswith("embeddings") or torch.equal(a, b), n
+
+
 def test_rms_norm_gradient():
     g = torch.Generator().manual_seed(3)
     x, w, dy = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((3, 5, 96), (96,), (3, 5, 96)))
