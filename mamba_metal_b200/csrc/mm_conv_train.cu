@@ -179,8 +179,10 @@ template <typename T, bool CK> struct Source {
 
 // The chunks from the last to the first, so that the three dpre after a chunk are known. Bound by instructions rather
 // than memory: an element takes its pre-activation again, silu', four taps for dx and five sums (f16 8x1536x4096 from
-// the checkpoint 105 us, 2.4 TB/s; from x itself 85, 3.6).
-template <typename T, bool CK, int ACCESS, int CPT>
+// the checkpoint 105 us, 2.4 TB/s; from x itself 83, 3.6; without SiLU 79 and 62).
+// Past the row's end dpre is 0, but its window may hold a last value that is no number, and 0 times that is not 0. With SiLU
+// such a value has made the last dpre, and with it every sum, NaN already; without, those steps are left out.
+template <typename T, bool CK, int ACCESS, int CPT, bool SILU>
 __global__ void __launch_bounds__(256) bwd_rows_kernel(const Params p, int warps_per_row) {
   const int lane = threadIdx.x & 31;
   const long long gw = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(256) bwd_rows_kernel(const Params p, int warps
 #pragma unroll
     for (int k = 0; k < 3; ++k)
       after[k] = end + k < p.seqlen ? ld_f32(grow + (long long)(end + k) * p.gs[2]) *
-                                          dact(pre(v[k], v[k + 1], v[k + 2], v[k + 3]), p.silu)
+                                          dact(pre(v[k], v[k + 1], v[k + 2], v[k + 3]), SILU)
                                     : 0.f;
   }
   T* orow = static_cast<T*>(p.out) + b * p.os[0] + d * p.os[1];
@@ -232,10 +234,12 @@ __global__ void __launch_bounds__(256) bwd_rows_kernel(const Params p, int warps
     }
 #pragma unroll
     for (int k = 0; k < kE; ++k) {
-      dp[k] = raw_at(g[j], k) * dact(pre(win[k], win[k + 1], win[k + 2], win[k + 3]), p.silu);
+      dp[k] = raw_at(g[j], k) * dact(pre(win[k], win[k + 1], win[k + 2], win[k + 3]), SILU);
+      if (SILU || k < n) {
 #pragma unroll
-      for (int i = 0; i < kW; ++i) sum[i] = fmaf(dp[k], win[k + i], sum[i]);
-      sum[4] += dp[k];
+        for (int i = 0; i < kW; ++i) sum[i] = fmaf(dp[k], win[k + i], sum[i]);
+        sum[4] += dp[k];
+      }
     }
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
@@ -720,8 +724,11 @@ template <typename T, bool CK> int launch_bwd(const MMConvBwdArgs* a, float* par
       access = kAnyStride;
     auto run = [&](auto level) {
       constexpr int A = decltype(level)::value;
-      pl.run == 256 ? bwd_rows_kernel<T, CK, A, 1><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts)
-                    : bwd_rows_kernel<T, CK, A, 4><<<(unsigned)grid, 256, 0, s>>>(p, pl.parts);
+      auto launch = [&](auto kernel) { kernel<<<(unsigned)grid, 256, 0, s>>>(p, pl.parts); };
+      if (p.silu)
+        pl.run == 256 ? launch(bwd_rows_kernel<T, CK, A, 1, true>) : launch(bwd_rows_kernel<T, CK, A, 4, true>);
+      else
+        pl.run == 256 ? launch(bwd_rows_kernel<T, CK, A, 1, false>) : launch(bwd_rows_kernel<T, CK, A, 4, false>);
     };
     with_access(access, run);
   }

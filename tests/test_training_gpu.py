@@ -447,6 +447,23 @@ def test_conv_gradient_at_the_largest_values(shape, layout, dtype):
             assert p.isfinite().all() and torch.equal(p, q)
 
 
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("length", [5, 70, 257, 1003])
+def test_conv_weights_that_the_last_steps_do_not_reach(length, layout, bad):
+    """Without SiLU the first tap's gradient is a sum over values that end three steps before the last: what is no number
+    among those three does not enter it, nor dx."""
+    g = torch.Generator().manual_seed(length)
+    x, dout = put(randn(g, 2, 9, length), torch.float16, layout)[0], put(randn(g, 2, 9, length), torch.float16)[0]
+    w = randn(g, 9, 4).float().to(DEV)
+    x[..., -3:] = 0
+    dx, dw, db = training.causal_conv1d_backward(dout, x, w, None, silu=False)
+    x[..., -3:] = bad
+    dx2, dw2, db2 = training.causal_conv1d_backward(dout, x, w, None, silu=False)
+    assert torch.equal(dx, dx2) and torch.equal(dw[:, 0], dw2[:, 0]) and torch.equal(db, db2)
+    assert not dw2[:, 1:].isfinite().any()
+
+
 def test_conv_gradient_against_differences():
     g = torch.Generator().manual_seed(2)
     x, w, b, dout = randn(g, 2, 5, 70), randn(g, 5, 4) / 2, randn(g, 5), randn(g, 2, 5, 70)
