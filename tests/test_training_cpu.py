@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from mamba_metal_b200 import _lib, training
+from tests.test_training_gpu import LARGE
 
 
 def size_of(fn, a):
@@ -156,3 +157,54 @@ def test_scan_gradient_of_no_channels_asks_for_what_it_clears():
     assert lib.mm_selective_scan_bwd(ctypes.byref(s), None, 0, None) == -1
     s.fwd.seqlen = 0
     assert lib.mm_selective_scan_bwd(ctypes.byref(s), None, 0, None) == 0
+
+
+def scan_plan(dtype, batch, dim, n, length):
+    """How the scan's training pass cuts a call: (chunks of a long chunk, long chunks, whether the forward pass walks whole
+    sequences, tiles that a block of the gradient works off, blocks beside each other over the channels)."""
+    chunks = -(-length // 32)
+    if n <= 16 and length <= 256:
+        per_long = chunks
+    else:
+        per_long = 4
+        while chunks > 2 and per_long > 1 and batch * -(-dim // 32) * -(-chunks // per_long) < 12 * 148:
+            per_long //= 2
+    whole = n <= 16 and (length <= 256 or batch * dim >= 8192)
+    every = dim * batch * chunks
+    width = 16 if (dtype == torch.float32 and n <= 16) or every < 3 * 148 * 32 else 32
+    tiles = 1 if n > 16 else min(max(every // (4 * 3 * 148) // width, 1), 512 // width)
+    return per_long, -(-chunks // per_long), whole, tiles, -(-dim // (width * tiles))
+
+
+def scan_sizes(dtype, batch, dim, n, length):
+    """The workspaces' sizes that follow from the plan."""
+    _, longs, whole, _, groups = scan_plan(dtype, batch, dim, n, length)
+    room = lambda *floats: sum(-(-4 * f // 256) * 256 for f in floats)
+    chunks, np4, passes = -(-length // 32), -(-n // 4) * 4, -(-n // 16)
+    rows, lrows = batch * chunks * dim, batch * longs * dim
+    cut = lrows if longs > 1 and not whole else 0
+    bc = batch * chunks * groups * passes * 16 * 32
+    many = chunks > 1
+    return room(cut * np4, cut), 256 + room(many * rows * np4, many * rows, many * lrows * np4, many * lrows, bc, bc, rows * np4,
+                                            rows, rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scan_plans(dtype):
+    """The plan restated above is the library's (whose workspaces follow from it), and the gradient tests reach all of its
+    kinds: long chunks of two and of four chunks, the last of them ragged, with both forward passes; several tiles a block."""
+    sizes = [(1, 1536, 16, 48), (1, 1536, 16, 5601), (8, 1536, 16, 4096), (1, 5120, 16, 16384), (2, 100, 40, 700)] + LARGE
+    for s in sizes:
+        a = _lib.MMScanBwdArgs()
+        f = a.fwd
+        f.dtype, (f.batch, f.dim, f.dstate, f.seqlen) = _lib.DTYPE_CODE[dtype], s
+        rc, forward = size_of(_lib.lib().mm_selective_scan_train_workspace_size, f)
+        assert rc == 0 and size_of(_lib.lib().mm_selective_scan_bwd_workspace_size, a)[0] == 0
+        assert (forward, size_of(_lib.lib().mm_selective_scan_bwd_workspace_size, a)[1]) == scan_sizes(dtype, *s), s
+    plans = [(s, *scan_plan(dtype, *s)) for s in LARGE]
+    ragged = [(per, longs, whole, tiles) for (_, _, _, length), per, longs, whole, tiles, _ in plans
+              if longs > 2 and length % 32 and -(-length // 32) % per]
+    assert {(4, False), (2, False), (4, True)} <= {(per, whole) for per, _, whole, _ in ragged}
+    assert any(n > 16 and per == 4 for (_, _, n, _), per, *_ in plans)
+    in_words = [(s, tiles) for s, *_, tiles, groups in plans if s[1] % 8 == 0 and s[3] % 8 == 0 and groups > 1]
+    assert max(tiles for _, tiles in in_words) >= 4 and any(s[1] % 8 and tiles > 1 for s, *_, tiles, _ in plans)

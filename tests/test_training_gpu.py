@@ -127,6 +127,29 @@ def test_scan_gradient_many_tiles():
     check_scan((8, 1000, 4, 330), torch.float32, "channel_first", ALL, seed=5)
 
 
+# (batch, channels, states, steps) at which the cut walks join long chunks of two or four chunks, the last one ragged, and a
+# block of the gradient works off several tiles, copied ahead where rows lie on 16 bytes. test_training_cpu.py holds
+# them to that.
+LARGE = [(4, 2000, 2, 936), (4, 2000, 16, 456), (4, 2000, 20, 936), (8, 1536, 16, 1192), (4, 2001, 3, 937), (8, 1021, 5, 1001)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["channel_first", "channels_last"])
+@pytest.mark.parametrize("shape", LARGE)
+def test_scan_gradient_large(shape, layout, dtype):
+    """Sizes that training runs at, against the float64 definition on the GPU."""
+    gpu, cpu, dy, dstate = scan_inputs(shape, dtype, layout, ALL, seed=17)
+    y, state, grads = run_scan(gpu, dy[0], dstate[0], ALL)
+    with torch.device(DEV):
+        leaves = {k: cpu[k].to(DEV).requires_grad_(True) for k in NAMES}
+        yr, hr = scan_ref(*(leaves[k] for k in NAMES), True)
+        ref = torch.autograd.grad((yr * dy[1].to(DEV)).sum() + (hr * dstate[1].to(DEV)).sum(), list(leaves.values()))
+    assert_close(y, yr, RTOL[name(dtype)], "y")
+    assert_close(state, hr, RTOL["float32"], "state")
+    for k, r in zip(leaves, ref):
+        assert_close(grads[k], r, RTOL[name(grads[k].dtype)], f"d{k}")
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("shape", [(2, 9, 16, 256), (2, 9, 16, 257), (1, 33, 7, 255), (1, 8191, 2, 263), (1, 8197, 9, 259)])
