@@ -342,9 +342,9 @@ int mm_linear_status(const void* workspace, mm_stream_t stream);
  * MM_CHECKPOINT8_BLOCK; a block keeps one exponent byte and one signed byte per value:
  *   e    = the least integer >= -126 with 127 * 2^e >= max |x| over the block (-126 for a block of zeros)
  *   code = x * 2^-e rounded to the nearest integer, ties to even (|code| <= 127);  exponent byte = e + 127
- * so a value is off by at most 2^(e-1), and code * 2^e is exact in every element type (where it passes
- * the type's largest finite value, that value is restored). A block that holds an infinity or a NaN gets
- * the exponent byte 255 and is restored as NaN.
+ * so a value is off by at most 2^(e-1) (less than max |x| / 127 for e > -126), and code * 2^e is exact in the type of
+ * x, in fp32 and in bf16 (where it passes the type's largest finite value, that value is restored). A block that
+ * holds an infinity or a NaN gets the exponent byte 255 and is restored as NaN.
  * x: (batch, dim, length) of `dtype`, codes alike in int8, exponents (batch, dim, ceil(length / 32)) in
  * uint8, any element strides. Vectorised paths: every tensor contiguous along time, rows of x 16-byte and
  * rows of codes 8-byte aligned; or every tensor contiguous along channels. Pack reads x and writes the

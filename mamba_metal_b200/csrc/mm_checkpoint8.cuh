@@ -61,7 +61,7 @@ MM_DEV float ck_value(unsigned w, int i) {
   return __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7650 + i)) - 8388736.f;
 }
 
-// The element of type T that a code stands for: exact, except past T's largest finite value, which is
+// The element of type T that a code stands for: exact in the type that was packed, except past T's largest finite value, which is
 // restored instead (amax near the top of the range can round up to a code past it). Every reader of codes goes by this
 // or, where a block is known to stay in range, by the product alone.
 template <typename T> struct CkMax;

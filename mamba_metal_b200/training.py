@@ -164,8 +164,9 @@ class Checkpoint8:
         return _span(self.codes) + _span(self.exponents)
 
     def restore(self, dtype: torch.dtype | None = None) -> torch.Tensor:
-        """The values, in ``dtype`` (default: the packed tensor's), laid out like the packed tensor. Exact, but for
-        values past the type's largest finite one, which is returned instead."""
+        """The values, in ``dtype`` (default: the packed tensor's), laid out like the packed tensor. Exact in the packed
+        tensor's type, in float32 and in bfloat16; in float16 rounded where its small values are too far apart. Past the
+        type's largest finite value that one is returned instead."""
         dtype = dtype or self.dtype
         if dtype not in _lib.DTYPE_CODE:
             raise TypeError(f"unsupported dtype {dtype}")
@@ -199,8 +200,8 @@ def _up_to_three(t: torch.Tensor) -> torch.Tensor:
 def checkpoint8(x: torch.Tensor) -> Checkpoint8:
     """Packs ``x`` (float32, float16 or bfloat16, one axis or more) into 8 bits a value: blocks of 32 values of the last
     axis share the smallest power of two of which 127 reach their largest magnitude, and every value becomes a whole
-    multiple of it, ties to even. No value moves by more than half that power of two, 1/128 of the block's
-    largest magnitude at most."""
+    multiple of it, ties to even. No value moves by more than half that power of two: by less than 1/127 of the block's
+    largest magnitude, where that is at least 127 * 2 ** -126 (the power of two is never less than 2 ** -126)."""
     assert x.dim() >= 1, "a checkpoint holds a tensor of one axis or more"
     if x.dtype not in _lib.DTYPE_CODE:
         raise TypeError(f"unsupported dtype {x.dtype}")

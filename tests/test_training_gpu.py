@@ -379,6 +379,32 @@ def test_checkpoint_extremes():
         assert got[0, 32:64].isnan().all() and torch.equal(got[0, :32], x[0, :32]) and torch.equal(got[1], x[1])
 
 
+def test_checkpoint_error_bound():
+    """Less than 1/127 of a block's largest magnitude, and more than 1/128 where that lies just above 127 steps: its step is
+    twice the one before."""
+    g = torch.Generator().manual_seed(9)
+    top = torch.cat([torch.full((40,), 127 * (1 + 2.0 ** -12)), torch.rand(400, generator=g) + 1, torch.full((40,), 1.99)])
+    x = (2 * torch.rand(480, 32, generator=g) - 1) * top[:, None]
+    x[:, 0] = top
+    x[:40, 1], x[440:, 1] = 0.99999, 0.0156  # just under half a step
+    off = (training.checkpoint8(x.to(DEV)).restore().cpu().double() - x.double()).abs().amax(1) / top.double()
+    assert (off < 1 / 127).all() and (off[:40] > 1 / 128).all() and (off[440:] > 1 / 128).all()
+
+
+@pytest.mark.parametrize("packed", DTYPES)
+def test_checkpoint_restored_in_other_types(packed):
+    """Exact in float32 and bfloat16, rounded to float16, in all of the packed type's range."""
+    g = torch.Generator().manual_seed(10)
+    top = torch.ldexp(torch.ones(250), torch.arange(-126, 124)) if packed != torch.float16 else torch.ldexp(torch.ones(40), torch.arange(-24, 16))
+    x = ((2 * torch.rand(len(top), 32, generator=g) - 1) * top[:, None]).to(packed)
+    c = training.checkpoint8(x.to(DEV))
+    values = checkpoint_ref(x.double())[0]
+    for dtype in (torch.float32, torch.bfloat16):
+        assert np.array_equal(c.restore(dtype).double().cpu().numpy(), values)
+    half = torch.as_tensor(values).clamp(-65504, 65504).half()
+    assert torch.equal(c.restore(torch.float16).cpu(), half)
+
+
 # ---- conv --------------------------------------------------------------------------------------------------
 
 
